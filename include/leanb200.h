@@ -402,6 +402,72 @@ int ls_spec_accept(int64_t* ids, const int64_t* verdict, int64_t batch, int64_t 
                    int32_t* accepted, int32_t* cache_pos, int32_t* draft_cache_pos, int64_t* out_tokens,
                    int32_t* out_len, int64_t out_cap, ls_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * A batch of different requests: a prefix they share, an adapter each, rules
+ * on their next token.  (No counterpart in the reference, which runs one
+ * request, or copies of it, without any of the three.)
+ * ------------------------------------------------------------------------- */
+
+/* GQA attention of m = batch * q_len tokens behind a prefix that every sequence
+ * of the batch shares and that is held once.  Query token i of sequence b sees
+ * keys 0 .. prefix_len - 1 of the prefix, then keys 0 .. cache_pos[b] + i of its
+ * own cache strip, one softmax over both: the mask of
+ * src/leanstack/runtime/qwen_explicit.py:551-563 with the prefix in front.
+ *   k_prefix/v_prefix  [Hkv, prefix_cap, D], the first prefix_len rows of each
+ *                      head in use (the rest is never used); NULL with prefix_len 0
+ *   k_cache/v_cache    [batch, Hkv, max_seq, D]; position j of a strip is
+ *                      position prefix_len + j of its sequence
+ *   out                [m, Hq * D]
+ * A cursor outside the cache raises LS_ERR_KV_OVERFLOW in the device error flag
+ * and that row sees what is inside; a row that sees no key gives zeros. */
+int ls_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t q_len, int64_t num_heads, int64_t num_kv_heads,
+                                               int64_t head_dim, int64_t prefix_len, int64_t* bytes);
+int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
+                               int64_t prefix_cap, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
+                               int64_t uniform_past, int64_t batch, int64_t q_len, int64_t num_heads,
+                               int64_t num_kv_heads, int64_t head_dim, int64_t max_seq, float scale, void* out,
+                               void* workspace, int64_t workspace_bytes, ls_stream_t stream);
+
+/* Low-rank adapters beside a projection that all sequences share: for every
+ * token t of sequence b = t / q_len with id = adapter_ids[b] (int32 [batch] on
+ * the device; negative: no adapter, zeros),
+ *   out[t] = scaling[id] * B[id] (A[id] x[t])     (accumulate: out[t] += ...)
+ * with a [adapters, rank, k], b [adapters, n, rank] (bf16), scaling fp32
+ * [adapters], out fp32 [m, n]: the layout of one split partial of
+ * LS_EPI_SPLIT_F32, so the kernel that adds the projection's partials adds the
+ * adapter and both round once.  k, n and rank multiples of 8, rank <= 128.  An
+ * id past the bank counts as none and raises LS_ERR_INVALID_ARGUMENT in the
+ * device error flag.  The workspace is zero-filled once by the caller. */
+int ls_lora_delta_workspace_bytes(int64_t batch, int64_t q_len, int64_t k, int64_t n, int64_t rank, int64_t* bytes);
+int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const void* a, const void* b,
+                  const float* scaling, int64_t adapters, int64_t n, int64_t rank, const int32_t* adapter_ids,
+                  int accumulate, float* out, void* workspace, int64_t workspace_bytes, ls_stream_t stream);
+
+/* Greedy pick under rules, one row of logits (bf16, or fp32 with logits_f32)
+ * per sequence.  For every allowed token v, in fp32 and in this order:
+ *   seen:       l = l > 0 ? l / repetition : l * repetition
+ *   count > 0:  l = (l - frequency * count) - presence
+ *   l = l + (the biases of v, added in list order)
+ * out_ids[b] = the lowest id of the largest l, -1 where no token is allowed;
+ * out_logits (fp32 [m, vocab], NULL: not wanted) = l, -inf where not allowed.
+ *   counts    int32 [m, vocab]: how often the answer holds each token
+ *   seen      uint32 [m, ceil(vocab / 32)], bit v % 32 of word v / 32: v is in
+ *             the prompt or the answer (set for every token with a count)
+ *   repetition, frequency, presence   fp32 [m] or NULL (1, 0, 0)
+ *   bias_ids, bias_values  [m, bias_cap]; ids outside the vocabulary are skipped
+ *   allowed   uint32 [m, ceil(vocab / 32)] or NULL (every token)
+ *   record    count the picked token and mark it seen
+ * NaN logits are never picked.  ls_token_stats_add enters ids [batch, len]
+ * (negative: padding) into seen and, unless counts is NULL (a prompt), counts;
+ * an id past the vocabulary raises LS_ERR_INVALID_ARGUMENT in the device error
+ * flag and is skipped. */
+int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t vocab, int32_t* counts, uint32_t* seen,
+                          const float* repetition, const float* frequency, const float* presence,
+                          const int32_t* bias_ids, const float* bias_values, int64_t bias_cap, const uint32_t* allowed,
+                          int record, int64_t* out_ids, float* out_logits, ls_stream_t stream);
+int ls_token_stats_add(const int64_t* ids, int64_t batch, int64_t len, int64_t vocab, int32_t* counts, uint32_t* seen,
+                       ls_stream_t stream);
+
 #ifdef LEANB200_PROFILING
 /* Measurement hooks, compiled only into a library built with
  * -DLEANB200_PROFILING (python -m leanstack_b200.build --profiling); the

@@ -107,6 +107,13 @@ SIGNATURES: dict[str, list] = {
     "ls_allreduce_residual_splits": [_p, _i64, _i64, _i64, _p, _p, _p, _p],
     "ls_sum_splits_f32": [_p, _i64, _i64, _p, _p],
     "ls_advance_cursors": [_p, _p, _i64, _i64, _p],
+    "ls_shared_prefix_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "ls_shared_prefix_attention": [_p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
+                                   _p, _p, _i64, _p],
+    "ls_lora_delta_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "ls_lora_delta": [_p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _int, _p, _p, _i64, _p],
+    "ls_constrained_argmax": [_p, _int, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _int, _p, _p, _p],
+    "ls_token_stats_add": [_p, _i64, _i64, _i64, _p, _p, _p],
 }
 _RESTYPES = {"ls_last_error": ctypes.c_char_p}
 # Measurement hooks, present only in a library built with --profiling (LEANB200_PROFILING).

@@ -406,11 +406,6 @@ int launch_tc_tile(const void* w, int64_t n_rows, int64_t k, int silu, void* out
 
 using namespace lsb_host;
 
-#define LS_REQUIRE(cond, code, ...) \
-  do {                              \
-    if (!(cond)) return set_error(code, __VA_ARGS__); \
-  } while (0)
-
 extern "C" {
 
 int ls_version(void) { return LS_ABI_VERSION; }

@@ -262,3 +262,9 @@ int sm_count();
 bool aligned16(const void* p);
 int* device_error_ptr();
 }  // namespace lsb_host
+
+// Argument check of a C entry point: records the message and returns the code.
+#define LS_REQUIRE(cond, code, ...) \
+  do {                              \
+    if (!(cond)) return lsb_host::set_error(code, __VA_ARGS__); \
+  } while (0)

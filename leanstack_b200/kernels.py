@@ -594,3 +594,190 @@ def spec_accept(ids: torch.Tensor, verdict: torch.Tensor, batch: int, k: int, *,
 def advance_cursors(cache_pos: torch.Tensor, q_len: int, delta: torch.Tensor | None = None) -> None:
     _check(cache_pos, "cache_pos", torch.int32)
     nat.call("ls_advance_cursors", cache_pos.data_ptr(), _ptr(delta), cache_pos.numel(), int(q_len), _stream())
+
+
+# ---------------------------------------------------------------------------
+# a batch of different requests: shared prefix, adapters, rules on the next token
+# ---------------------------------------------------------------------------
+def _call_on(ref: torch.Tensor, name: str, *args) -> None:
+    """Enqueue a C call on the current stream of ``ref``'s device (which need not be the current device)."""
+    dev = ref.device.index
+    if dev == torch.cuda.current_device():
+        nat.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        return
+    with torch.cuda.device(dev):
+        nat.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _check_on(ref: torch.Tensor, t: torch.Tensor | None, name: str, dtype, shape: tuple | None = None) -> None:
+    """:func:`_check` for an optional operand that must sit beside ``ref`` and have ``shape``."""
+    if t is None:
+        return
+    _check(t, name, dtype)
+    if t.device != ref.device:
+        raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def shared_prefix_attention_workspace_bytes(batch: int, q_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                            prefix_len: int) -> int:
+    v = ctypes.c_int64(0)
+    nat.call("ls_shared_prefix_attention_workspace_bytes", batch, q_len, num_heads, num_kv_heads, head_dim, prefix_len,
+             ctypes.byref(v))
+    return v.value
+
+
+def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, batch: int, q_len: int, num_heads: int, num_kv_heads: int,
+                            head_dim: int, prefix_len: int, max_seq: int, scale: float, *,
+                            cache_pos: torch.Tensor | None = None, uniform_past: int = 0,
+                            out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA attention of ``batch * q_len`` tokens behind a prefix held once.
+
+    ``k_prefix`` / ``v_prefix`` ``[Hkv, capacity, D]`` hold the shared keys and
+    values in their first ``prefix_len`` rows; ``k_cache`` / ``v_cache``
+    ``[batch, Hkv, max_seq, D]`` each sequence's own.  Token i of sequence b
+    sees the whole prefix, then its own keys 0 .. ``cache_pos[b] + i``.
+    ``workspace``: zero-filled once, ``shared_prefix_attention_workspace_bytes``
+    long; calls on one stream may share it.
+    """
+    _check(q, "q")
+    if q.numel() != batch * q_len * num_heads * head_dim:
+        raise ValueError(f"q holds {q.numel()} elements, expected {batch} x {q_len} x {num_heads} x {head_dim}")
+    if k_prefix.dim() != 3:
+        raise ValueError("k_prefix must be [num_kv_heads, capacity, head_dim]")
+    cap = k_prefix.shape[1]
+    for name, t, shape in (("k_prefix", k_prefix, (num_kv_heads, cap, head_dim)),
+                           ("v_prefix", v_prefix, (num_kv_heads, cap, head_dim)),
+                           ("k_cache", k_cache, (batch, num_kv_heads, max_seq, head_dim)),
+                           ("v_cache", v_cache, (batch, num_kv_heads, max_seq, head_dim))):
+        _check_on(q, t, name, BF16, shape)
+    _check_on(q, cache_pos, "cache_pos", torch.int32, (batch,))
+    m = batch * q_len
+    if out is None:
+        out = torch.empty((m, num_heads * head_dim), device=q.device, dtype=BF16)
+    else:
+        _check_on(q, out, "out", BF16, (m, num_heads * head_dim))
+    if workspace is None:
+        need = shared_prefix_attention_workspace_bytes(batch, q_len, num_heads, num_kv_heads, head_dim, prefix_len)
+        workspace = torch.zeros(max(need, 256), device=q.device, dtype=torch.uint8)
+    else:
+        _check_on(q, workspace, "workspace", torch.uint8)
+    _call_on(q, "ls_shared_prefix_attention", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), int(prefix_len),
+             cap, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(cache_pos), int(uniform_past), batch, q_len, num_heads,
+             num_kv_heads, head_dim, max_seq, float(scale), out.data_ptr(), workspace.data_ptr(),
+             workspace.numel())
+    return out
+
+
+def lora_delta_workspace_bytes(batch: int, q_len: int, k: int, n: int, rank: int) -> int:
+    v = ctypes.c_int64(0)
+    nat.call("ls_lora_delta_workspace_bytes", batch, q_len, k, n, rank, ctypes.byref(v))
+    return v.value
+
+
+def lora_delta(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, adapter_ids: torch.Tensor,
+               q_len: int = 1, *, accumulate: bool = False, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Low-rank adapters of many requests at once: ``out[t] = scaling[id] * b[id] @ (a[id] @ x[t])`` in fp32.
+
+    ``x [batch * q_len, k]``, ``a [adapters, rank, k]``, ``b [adapters, n, rank]``,
+    ``scaling`` fp32 ``[adapters]``, ``adapter_ids`` int32 ``[batch]`` (negative:
+    no adapter, zeros).  ``out`` fp32 ``[batch * q_len, n]`` has the layout of one
+    split partial of :func:`gemm_tc_splits`, so the partials' consumer adds it to
+    the shared projection before the one rounding; ``accumulate`` adds to ``out``
+    instead.  ``workspace``: zero-filled once; calls on one stream may share it.
+    """
+    _check(x, "x")
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError("lora_delta takes x [m, k], a [adapters, rank, k] and b [adapters, n, rank]")
+    m, k = x.shape
+    adapters, rank, n = a.shape[0], a.shape[1], b.shape[1]
+    if q_len < 1 or m % q_len:
+        raise ValueError(f"{m} tokens are not sequences of {q_len}")
+    _check_on(x, a, "a", BF16, (adapters, rank, k))
+    _check_on(x, b, "b", BF16, (adapters, n, rank))
+    _check_on(x, scaling, "scaling", torch.float32, (adapters,))
+    _check_on(x, adapter_ids, "adapter_ids", torch.int32, (m // q_len,))
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate adds to out: give one")
+        out = torch.empty((m, n), device=x.device, dtype=torch.float32)
+    else:
+        _check_on(x, out, "out", torch.float32, (m, n))
+    if workspace is None:
+        workspace = torch.zeros(lora_delta_workspace_bytes(m // q_len, q_len, k, n, rank), device=x.device,
+                                dtype=torch.uint8)
+    else:
+        _check_on(x, workspace, "workspace", torch.uint8)
+    _call_on(x, "ls_lora_delta", x.data_ptr(), m // q_len, q_len, k, a.data_ptr(), b.data_ptr(), scaling.data_ptr(),
+             adapters, n, rank, adapter_ids.data_ptr(), int(accumulate), out.data_ptr(), workspace.data_ptr(),
+             workspace.numel())
+    return out
+
+
+def constrained_argmax(logits: torch.Tensor, *, counts: torch.Tensor | None = None, seen: torch.Tensor | None = None,
+                       repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                       presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                       bias_values: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                       record: bool = False, out_ids: torch.Tensor | None = None,
+                       out_logits: torch.Tensor | None = None) -> torch.Tensor:
+    """Greedy pick of each row of ``logits [m, vocab]`` (bf16 or fp32) under its rules -> int64 ``[m]``.
+
+    Seen tokens are divided (positive logit) or multiplied by ``repetition``,
+    lose ``frequency`` per occurrence in the answer (``counts`` int32 ``[m,
+    vocab]``) and ``presence`` once; biases (``bias_ids`` int32 / ``bias_values``
+    fp32 ``[m, n]``, ids outside the vocabulary skipped) are added; tokens whose
+    ``allowed`` bit is clear are no candidates.  ``seen`` / ``allowed`` are int32
+    words ``[m, ceil(vocab / 32)]``, bit ``v % 32`` of word ``v // 32``.  Lowest
+    id on ties, -1 where nothing is allowed.  ``record`` enters the pick into
+    ``counts`` and ``seen``; ``out_logits`` fp32 ``[m, vocab]`` receives the
+    processed logits (-inf where not allowed).
+    """
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (BF16, torch.float32):
+        raise TypeError("logits must be a bf16 or fp32 tensor")
+    _check(logits, "logits", logits.dtype)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [m, vocab]")
+    m, vocab = logits.shape
+    words = (m, (vocab + 31) // 32)
+    _check_on(logits, counts, "counts", torch.int32, (m, vocab))
+    _check_on(logits, seen, "seen", torch.int32, words)
+    _check_on(logits, allowed, "allowed", torch.int32, words)
+    _check_on(logits, repetition, "repetition", torch.float32, (m,))
+    _check_on(logits, frequency, "frequency", torch.float32, (m,))
+    _check_on(logits, presence, "presence", torch.float32, (m,))
+    cap = 0
+    if bias_ids is not None and bias_values is not None:
+        if bias_ids.dim() != 2:
+            raise ValueError("bias_ids must be [m, n]")
+        cap = bias_ids.shape[1]
+        _check_on(logits, bias_ids, "bias_ids", torch.int32, (m, cap))
+        _check_on(logits, bias_values, "bias_values", torch.float32, (m, cap))
+    elif bias_ids is not None or bias_values is not None:
+        raise ValueError("bias_ids and bias_values come together")
+    _check_on(logits, out_logits, "out_logits", torch.float32, (m, vocab))
+    if out_ids is None:
+        out_ids = torch.empty((m,), device=logits.device, dtype=torch.int64)
+    else:
+        _check_on(logits, out_ids, "out_ids", torch.int64, (m,))
+    _call_on(logits, "ls_constrained_argmax", logits.data_ptr(), int(logits.dtype == torch.float32), m, vocab,
+             _ptr(counts), _ptr(seen), _ptr(repetition), _ptr(frequency), _ptr(presence),
+             _ptr(bias_ids) if cap else None, _ptr(bias_values) if cap else None, cap, _ptr(allowed), int(record),
+             out_ids.data_ptr(), _ptr(out_logits))
+    return out_ids
+
+
+def token_stats_add(ids: torch.Tensor, seen: torch.Tensor, vocab: int, *, counts: torch.Tensor | None = None) -> None:
+    """Enter the tokens ``ids [batch, len]`` (int64; negative: padding) into ``seen`` and, given ``counts``
+    (an answer's tokens rather than a prompt's), into the counts of :func:`constrained_argmax`."""
+    _check(ids, "ids", torch.int64)
+    if ids.dim() != 2:
+        raise ValueError("ids must be [batch, len]")
+    batch, n = ids.shape
+    _check_on(ids, seen, "seen", torch.int32, (batch, (vocab + 31) // 32))
+    _check_on(ids, counts, "counts", torch.int32, (batch, vocab))
+    if n == 0:
+        return
+    _call_on(ids, "ls_token_stats_add", ids.data_ptr(), batch, n, vocab, _ptr(counts), seen.data_ptr())
