@@ -41,6 +41,7 @@ constexpr int kTaMergeBytes = kTaWarps * kTaRows * (kTaHeadDim + 2) * 4;  // reu
 constexpr int kTaRecvBytes = kTaRows * kTaHeadDim * 4 + 2 * kTaMaxSplits * kTaRows * 4;
 constexpr int kTaSmemBytes = kTaRingBytes + kTaRecvBytes;
 constexpr int kTaQStageBytes = kTaRows * kTaHeadDim * 2;  // fused mode: the CTA's normalised query rows
+constexpr int kTaMaxPart = 512;  // key splits of a shared prefix that the join holds weights for
 static_assert(kTaMergeBytes <= kTaRingBytes, "merge buffers must fit in the ring");
 
 struct TaParams {
@@ -65,6 +66,11 @@ struct TaParams {
   __nv_bfloat16* v_store;
   int rope_len, rope_offset;
   float eps;
+  // Join with the key splits of a shared prefix (shared_prefix.cu): per kv head
+  // and batch-wide row, n_part groups of unnormalised O and (m, l).
+  const float* part_o;    // [Hkv][B q_len G][n_part][D]
+  const float2* part_ml;  // [Hkv][B q_len G][n_part]
+  int n_part;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
@@ -119,7 +125,11 @@ __device__ __forceinline__ uint32_t ta_swz(int key, int chunk) {
   return (uint32_t)(key * (kTaHeadDim * 2) + ((chunk ^ (key & 7)) << 4));
 }
 
-template <bool FUSED>
+// PREFIX: the rows also attend over a shared prefix, whose key splits the
+// previous kernel forms; this one reads its own inputs and keys while that runs
+// (it starts only after every CTA of it has seen the kernels before complete)
+// and waits for it before the join.
+template <bool FUSED, bool PREFIX = false>
 __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParams p) {
   extern __shared__ __align__(128) unsigned char ta_smem[];
   float* recv_o = reinterpret_cast<float*>(ta_smem + kTaRingBytes);  // [splits][16][128/splits]
@@ -132,7 +142,7 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   // table and the norm weights are written by no kernel that can still be
   // running (the cursor and accept kernels let their dependents start only at
   // their own end), so the first K/V copies go out under the projection's tail.
-  if (!FUSED) grid_dep_wait();
+  if (!FUSED && (!PREFIX || p.n_part == 0)) grid_dep_wait();
   grid_dep_launch();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -140,8 +150,8 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   const int b = blockIdx.z;
   const int hkv = blockIdx.y / p.RG, rg = blockIdx.y - hkv * p.RG;
   const int s = p.splits > 1 ? (int)ta_cluster_rank() : 0;
-  const int cp = p.cache_pos ? (FUSED ? __ldcg(p.cache_pos + b) : p.cache_pos[b]) : p.uniform_past;
-  int L = cp + p.q_len;
+  const int cp = p.cache_pos ? (FUSED || PREFIX ? __ldcg(p.cache_pos + b) : p.cache_pos[b]) : p.uniform_past;
+  int L = min(cp, p.max_seq) + p.q_len;
   if (L > p.max_seq || cp < 0) {
     if (threadIdx.x == 0 && s == 0) raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
     L = min(max(L, 0), p.max_seq);
@@ -245,13 +255,14 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
     const bool valid = row < p.R;
     const int i = valid ? row / p.G : 0;
     const int gq = valid ? row - i * p.G : 0;
-    lim[hr] = valid ? cp + i : -1;
+    lim[hr] = valid ? min(cp, p.max_seq) + i : -1;
     const __nv_bfloat16* qp = fused ? qs + (size_t)(row - r0) * kTaHeadDim
                                     : p.q + ((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
-      qa[ks][hr] = valid ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + 2 * t4) : 0u;
-      qa[ks][2 + hr] = valid ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + 8 + 2 * t4) : 0u;
+      const uint32_t* q2 = reinterpret_cast<const uint32_t*>(qp + ks * 16 + 2 * t4);
+      qa[ks][hr] = valid ? (PREFIX ? __ldcg(q2) : q2[0]) : 0u;
+      qa[ks][2 + hr] = valid ? (PREFIX ? __ldcg(q2 + 4) : q2[4]) : 0u;
     }
   }
 
@@ -379,6 +390,56 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   __syncthreads();
   if (p.splits > 1) ta_cluster_wait();  // every CTA of the cluster has started: remote stores are safe
 
+  // PREFIX: the weights of the row's groups, own keys first.  The row's shared
+  // maximum over own splits is known only after they meet, so the weights of a
+  // cluster are formed there; with one split, here.
+  float* wgt = reinterpret_cast<float*>(ta_smem + kTaMergeBytes);  // [16][1 + n_part], own weight first
+  float* wsum = wgt + kTaRows * (1 + (PREFIX ? p.n_part : 0));     // [16]: the sum of all weights
+  const size_t prow0 = PREFIX ? (size_t)hkv * gridDim.z * p.R + (size_t)b * p.R + r0 : 0;
+  auto prefix_weights = [&](int r, float m_own, float l_own) {  // one warp per row
+    const float2* ml = p.part_ml + (prow0 + r) * p.n_part;
+    float mx = m_own;
+    for (int c = lane; c < p.n_part; c += 32) mx = fmaxf(mx, __ldcg(ml + c).x);
+    mx = warp_max(mx);
+    const float f = m_own == -INFINITY ? 0.f : exp2f(m_own - mx);
+    float sum = 0.f;
+    for (int c = lane; c < p.n_part; c += 32) {
+      const float2 v = __ldcg(ml + c);
+      const float fc = v.x == -INFINITY ? 0.f : exp2f(v.x - mx);
+      wgt[r * (1 + p.n_part) + 1 + c] = fc;
+      sum += v.y * fc;
+    }
+    sum = warp_sum(sum) + l_own * f;
+    if (lane == 0) {
+      wgt[r * (1 + p.n_part)] = f;
+      wsum[r] = sum;
+    }
+  };
+  auto prefix_join = [&](int r, int dim, float acc) -> float {  // the finished output of dim `dim` of row r
+    const float* wr = wgt + r * (1 + p.n_part);
+    const float* po = p.part_o + (prow0 + r) * p.n_part * kTaHeadDim + dim;
+    float o = wr[0] != 0.f ? acc * wr[0] : 0.f;
+#pragma unroll 4
+    for (int c = 0; c < p.n_part; ++c) {
+      const float v = __ldcg(po + (size_t)c * kTaHeadDim);
+      o += wr[1 + c] != 0.f ? v * wr[1 + c] : 0.f;
+    }
+    return wsum[r] > 0.f ? o / wsum[r] : 0.f;
+  };
+  if (PREFIX) {
+    if (p.n_part > 0) grid_dep_wait();
+    if (p.splits == 1) {
+      for (int r = warp; r < nrows; r += kTaWarps) {
+        float mx = -INFINITY, ls = 0.f;
+        for (int k = 0; k < kTaWarps; ++k) mx = fmaxf(mx, wm[k * kTaRows + r]);
+        if (mx != -INFINITY)
+          for (int k = 0; k < kTaWarps; ++k) ls += wl[k * kTaRows + r] * exp2f(wm[k * kTaRows + r] - mx);
+        prefix_weights(r, mx, ls);
+      }
+      __syncthreads();
+    }
+  }
+
   const int d = threadIdx.x;  // one output dimension per thread (kTaThreads == kTaHeadDim)
   const int w = kTaHeadDim / p.splits;  // dims each cluster CTA finishes
   for (int r = 0; r < nrows; ++r) {
@@ -397,7 +458,8 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
     if (p.splits == 1) {
       const int row = r0 + r;
       const int i = row / p.G, gq = row - (row / p.G) * p.G;
-      p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + d] = f_to_bf16(acc / ls);
+      p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + d] =
+          f_to_bf16(PREFIX ? prefix_join(r, d, acc) : acc / ls);
     } else {
       const int owner = d / w;
       ta_st_remote(recv_o + ((size_t)s * kTaRows + r) * w + (d - owner * w), (uint32_t)owner, acc);
@@ -409,6 +471,17 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   }
   if (p.splits == 1) return;
   ta_cluster_sync();  // release this CTA's remote stores, acquire the others'
+  if (PREFIX) {
+    for (int r = warp; r < nrows; r += kTaWarps) {
+      float mx = -INFINITY, ls = 0.f;
+      for (int c = 0; c < p.splits; ++c) mx = fmaxf(mx, recv_m[c * kTaRows + r]);
+      if (mx != -INFINITY)
+        for (int c = 0; c < p.splits; ++c)
+          if (recv_m[c * kTaRows + r] != -INFINITY) ls += recv_l[c * kTaRows + r] * exp2f(recv_m[c * kTaRows + r] - mx);
+      prefix_weights(r, mx, ls);
+    }
+    __syncthreads();
+  }
 
   for (int idx = threadIdx.x; idx < nrows * w; idx += kTaThreads) {
     const int r = idx / w, dd = idx - r * w;
@@ -424,7 +497,8 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
     }
     const int row = r0 + r;
     const int i = row / p.G, gq = row - (row / p.G) * p.G;
-    p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + s * w + dd] = f_to_bf16(acc / ls);
+    p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + s * w + dd] =
+        f_to_bf16(PREFIX ? prefix_join(r, s * w + dd, acc) : acc / ls);
   }
 }
 
@@ -455,15 +529,15 @@ static TaPlan ta_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   return pl;
 }
 
-template <bool FUSED>
+template <bool FUSED, bool PREFIX = false>
 static int launch_ta(const TaParams& p, const TaPlan& pl, int64_t batch, int64_t hkv, cudaStream_t stream) {
   constexpr size_t smem = kTaSmemBytes + (FUSED ? kTaQStageBytes : 0);
   static bool attrs_set = false;
   if (!attrs_set) {
     cudaError_t e =
-        cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED, PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      e = cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED, PREFIX>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "attention_tc attributes: %s", cudaGetErrorString(e));
     attrs_set = true;
   }
@@ -481,7 +555,7 @@ static int launch_ta(const TaParams& p, const TaPlan& pl, int64_t batch, int64_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attention_tc_kernel<FUSED>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attention_tc_kernel<FUSED, PREFIX>, p);
   if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "decode_attention_tc launch: %s", cudaGetErrorString(e));
   return LS_OK;
 }
@@ -518,6 +592,26 @@ int launch_decode_attention_tc(const void* q, const void* k_cache, const void* v
   TaParams p = ta_params(pl, k_cache, v_cache, cache_pos, uniform_past, q_len, hq, hkv, max_seq, scale, out);
   p.q = static_cast<const __nv_bfloat16*>(q);
   return launch_ta<false>(p, pl, batch, hkv, stream);
+}
+
+// The same rows behind a shared prefix of n_part key splits (shared_prefix.cu).
+int launch_decode_attention_prefix(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
+                                   int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
+                                   int64_t max_seq, float scale, const float* part_o, const float2* part_ml, int n_part,
+                                   void* out, cudaStream_t stream) {
+  const TaPlan pl = ta_plan(batch, q_len, hq, hkv, max_seq);
+  if ((int64_t)hkv * pl.RG > 65535)
+    return set_error(LS_ERR_UNSUPPORTED_SHAPE, "shared_prefix_attention: %lld kv heads x %d row groups exceed the grid",
+                     (long long)hkv, pl.RG);
+  static_assert(kTaMergeBytes + kTaRows * (1 + kTaMaxPart + 1) * 4 <= kTaRingBytes, "weights must fit in the ring");
+  if (n_part > kTaMaxPart)
+    return set_error(LS_ERR_UNSUPPORTED_SHAPE, "shared_prefix_attention: %d key splits", n_part);
+  TaParams p = ta_params(pl, k_cache, v_cache, cache_pos, uniform_past, q_len, hq, hkv, max_seq, scale, out);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.part_o = part_o;
+  p.part_ml = part_ml;
+  p.n_part = n_part;
+  return launch_ta<false, true>(p, pl, batch, hkv, stream);
 }
 
 // One decode token per sequence (q_len 1) straight from the raw fused QKV

@@ -32,11 +32,8 @@
 // accumulators) and rounds after the projection, after SiLU and after the
 // product.  Every mbarrier wait is bounded (LS_ERR_TIMEOUT).
 // The file also holds the large-M prefill GEMM (gemm_big_kernel) and the causal
-// prefill attention on tcgen05 (prefill_attention_tc_kernel), which share the
-// TMA, UMMA-descriptor and TMEM helpers below.
-#include <cuda.h>
-
-#include "common.cuh"
+// prefill attention on tcgen05 (prefill_attention_tc_kernel).
+#include "tcgen05.cuh"
 
 namespace lsb {
 
@@ -80,48 +77,6 @@ struct TcParams {
   unsigned long long* trace;  // optional profiling: per CTA 8 globaltimer stamps
   int aligned;  // N % 8 == 0 and out / residual 16-byte aligned: vector stores, bulk residual rows
 };
-
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
-  // K-major, 128-byte swizzle: 8-row groups 1024 B apart (SBO), LBO unused,
-  // descriptor version 1, layout type 2 (SWIZZLE_128B).
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
-          tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float v[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // First unit of CTA c and the CTA that owns unit u (units split evenly).
 __device__ __forceinline__ long long tc_unit_begin(long long U, int G, int c) { return U * c / G; }
@@ -925,7 +880,7 @@ static EncodeTiledFn encode_fn() {
 }
 
 // 2-D bf16 tensor map over a row-major [rows, cols] matrix, box [box_rows, 64], 128-byte swizzle.
-static int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows) {
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(LS_ERR_NOT_SUPPORTED, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -1350,40 +1305,6 @@ struct PtParams {
   int q_len, Hq, Hkv, G, R, max_seq;
   float scale_log2;
 };
-
-__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t lbo_bytes) {
-  // MN-major, 128-byte swizzle: 64-element MN chunks lbo_bytes apart (LBO),
-  // 8-row K groups 1024 B apart (SBO), descriptor version 1, SWIZZLE_128B.
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(lbo_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-         (2ull << 61);
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float v[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-          taddr),
-      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
-      "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
-      "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])),
-      "r"(__float_as_uint(v[11])), "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])),
-      "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// 2^x with the hardware's approximate exp2 (MUFU); 2^-inf = 0.  The softmax
-// probabilities are rounded to about 16 bits afterwards.
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Byte offset of 16-byte chunk c of row r in a K-major tile stored as 64-wide
-// halves of `half` bytes each (128-byte swizzle; c >> 3 selects the half).
-__device__ __forceinline__ uint32_t pt_off(int r, int c, int half) {
-  return (uint32_t)((c >> 3) * half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-}
 
 __global__ void __launch_bounds__(kPtThreads, 1)
     prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,

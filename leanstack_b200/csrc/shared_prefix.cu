@@ -5,72 +5,422 @@
 // static cache strip, one softmax over both (the mask of
 // src/leanstack/runtime/qwen_explicit.py:551-563 with the prefix in front).
 //
-// One CTA per (token, query head): four warps take every fourth key, each lane
-// four of the 128 dims, online softmax in fp32 (base 2), merged in shared
-// memory.  Every row reads the prefix for itself.
-#include "common.cuh"
+// The softmax splits over the keys: with m the maximum of a group of scores,
+// l = sum e^(s - m) and O = sum e^(s - m) v, groups join as
+//   M = max m,  o = sum_g e^(m_g - M) O_g / sum_g e^(m_g - M) l_g.
+// So the prefix is one group per key split, formed once for ALL query rows of a
+// kv head (B q_len G rows, whatever sequence they belong to), and the cache
+// strip of a sequence is another, formed by the decode-attention kernel, which
+// joins the groups in its epilogue (attention_tc.cu).  Per prefix key and kv
+// head 512 bytes are read once for R rows and 4 D R flops done on them: memory
+// is the bound below about 250 rows, the tensor cores above.
+//
+// prefix_tc_kernel, one CTA per SM:
+//   * warp 8 streams 128-key K and V tiles with TMA (128-byte swizzle, boxes of
+//     32 keys so that a split's last tile fetches no more than it needs) through
+//     a ring of 32 KB slots;
+//   * warp 9 issues S = Q K^T into TMEM (fp32, 128 columns) and O += P V with P
+//     taken from TMEM, where it replaces the S it came from;
+//   * warps 0-7 are two softmax streams of 128 threads, one thread per row, a
+//     whole 128-key row of S in registers: no shuffles, no shared memory on the
+//     way from S to P.  While one stream exponentiates, the tensor core works
+//     for the other.  Rows (kRows): the streams hold two 128-row tiles and share
+//     every K/V tile.  Keys (kKeys, at most 128 rows): they hold the same rows
+//     and take alternate K/V tiles; their results join in the epilogue.
+//   * P is rounded to bf16 (2^-8 of each probability, independent from key to
+//     key, against one more 2^-8 when the output is rounded), the row sum is
+//     taken before that rounding in fp32.  The maximum in use moves only when a
+//     score exceeds it by 2^8; then O is rescaled in TMEM.
+//   * kFull: a prompt's rows.  A CTA owns 256 rows of one (sequence, kv head)
+//     and walks the prefix tiles, then the sequence's own tiles with the causal
+//     mask, and writes the finished rows: no partials.
+#include "tcgen05.cuh"
 
 namespace lsb {
 
 constexpr int kSpHeadDim = 128;
+constexpr int kSpRows = 128;                       // rows of one stream (MMA M)
+constexpr int kSpKeys = 128;                       // keys per tile
+constexpr int kSpBox = 32;                         // keys per TMA box
+constexpr int kSpQHalf = kSpRows * 128;            // 64 dims of 128 rows: 16 KB
+constexpr int kSpQ = 2 * kSpQHalf;                 // one 128-row Q tile: 32 KB
+constexpr int kSpKvHalf = kSpKeys * 128;           // 64 dims of 128 keys: 16 KB
+constexpr int kSpSlot = 2 * kSpKvHalf;             // one K or V tile: 32 KB
+constexpr int kSpThreads = 320;
+constexpr int kSpSoft = 256;
+constexpr float kSpRescaleLog2 = 8.f;
+enum SpMode { kKeys = 0, kRows = 1, kFull = 2 };
+constexpr int sp_slots(int mode) { return mode == kKeys ? 5 : 4; }
+constexpr int sp_ring(int mode) { return mode == kKeys ? kSpQ : 2 * kSpQ; }  // ring offset, behind Q
+constexpr int sp_bars(int mode) { return sp_ring(mode) + sp_slots(mode) * kSpSlot; }
+constexpr int sp_smem(int mode) { return 1024 + sp_bars(mode) + 256; }
 
 struct SpParams {
-  const __nv_bfloat16* q;         // [M, Hq, D]
-  const __nv_bfloat16* k_prefix;  // [Hkv, prefix_cap, D]
-  const __nv_bfloat16* v_prefix;
-  const __nv_bfloat16* k_cache;   // [B, Hkv, S, D]
-  const __nv_bfloat16* v_cache;
-  const int* cache_pos;           // [B] or null (then uniform_past)
+  const __nv_bfloat16* q;  // [M, Hq, D]
+  const int* cache_pos;    // [B] or null (then uniform_past); kFull only
   int uniform_past;
-  __nv_bfloat16* out;             // [M, Hq * D]
+  float* part_o;           // [Hkv][rows][splits][D]: unnormalised O of each key split
+  float2* part_ml;         // [Hkv][rows][splits]: (m, l)
+  __nv_bfloat16* out;      // kFull: [M, Hq * D]
   int* err;
-  int q_len, Hq, Hkv, G, P, prefix_cap, max_seq;
+  int rows;                // kKeys / kRows: B q_len G; kFull: q_len G
+  int q_len, Hq, Hkv, G, P, prefix_cap, max_seq, splits;
   float scale_log2;
 };
 
-__global__ void __launch_bounds__(128) shared_prefix_attention_kernel(SpParams p) {
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][kSpHeadDim];
+template <int MODE>
+__global__ void __launch_bounds__(kSpThreads, 1)
+    prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
+                     const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc, SpParams p) {
+  constexpr int kSlots = sp_slots(MODE);
+  extern __shared__ unsigned char sp_smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(sp_smem_raw) + 1023) & ~size_t(1023));
+  unsigned char* ring = smem + sp_ring(MODE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + sp_bars(MODE));
+  uint64_t* empty = full + kSlots;
+  uint64_t* s_full = empty + kSlots;  // [2]: a stream's scores are in TMEM (and all its earlier products done)
+  uint64_t* p_full = s_full + 2;      // [2]: a stream's probabilities are in TMEM
+  uint64_t* q_full = p_full + 2;
+  uint64_t* o_done = q_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 1);
+  __shared__ int s_abort;
+  __shared__ float2 s_ml[2][kSpRows];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], kSpRows);
+    }
+    mbar_init(q_full, kSpSoft);
+    mbar_init(o_done, 1);
+    s_abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S of the streams: columns 0, 128; O: 256, 384
+
+  // Every CTA waits before it lets the next kernel start: what that kernel reads
+  // besides this one's results was complete before.
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = blockIdx.x, h = blockIdx.y, hkv = h / p.G;
-  const int b = t / p.q_len, i = t - b * p.q_len;
-  const int cp = p.cache_pos ? p.cache_pos[b] : p.uniform_past;
-  if ((cp < 0 || cp > p.max_seq - p.q_len) && threadIdx.x == 0) raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
-  const int own = min(max(min(cp, p.max_seq) + i + 1, 0), p.max_seq);
-  const size_t pbase = (size_t)hkv * p.prefix_cap * kSpHeadDim;
-  const size_t cbase = ((size_t)b * p.Hkv + hkv) * p.max_seq * kSpHeadDim;
-  const uint2 qu = *reinterpret_cast<const uint2*>(p.q + ((size_t)t * p.Hq + h) * kSpHeadDim + lane * 4);
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-  for (int j = warp; j < p.P + own; j += 4) {
-    const size_t off = (j < p.P ? pbase + (size_t)j * kSpHeadDim : cbase + (size_t)(j - p.P) * kSpHeadDim) + lane * 4;
-    const uint2 ku = *reinterpret_cast<const uint2*>((j < p.P ? p.k_prefix : p.k_cache) + off);
-    const uint2 vu = *reinterpret_cast<const uint2*>((j < p.P ? p.v_prefix : p.v_cache) + off);
-    float s = bf16_lo(qu.x) * bf16_lo(ku.x) + bf16_hi(qu.x) * bf16_hi(ku.x) + bf16_lo(qu.y) * bf16_lo(ku.y) +
-              bf16_hi(qu.y) * bf16_hi(ku.y);
-    s = warp_sum(s) * p.scale_log2;
-    const float mn = fmaxf(m, s);
-    if (mn == -INFINITY) continue;
-    const float c = exp2f(m - mn), e = exp2f(s - mn);
-    m = mn;
-    l = l * c + e;
-    o0 = o0 * c + e * bf16_lo(vu.x);
-    o1 = o1 * c + e * bf16_hi(vu.x);
-    o2 = o2 * c + e * bf16_lo(vu.y);
-    o3 = o3 * c + e * bf16_hi(vu.y);
+
+  // This CTA's rows and keys.
+  const int h = MODE == kFull ? blockIdx.y : blockIdx.z;
+  const int b = MODE == kFull ? blockIdx.z : 0;
+  const int row_blk = MODE == kFull ? gridDim.x - 1 - blockIdx.x : blockIdx.y;  // kFull: the longest first
+  const int r0 = row_blk * (MODE == kKeys ? kSpRows : 2 * kSpRows);
+  const int split = MODE == kFull ? 0 : blockIdx.x;
+  int k0 = 0, k1 = p.P;  // prefix keys
+  if (MODE != kFull) {   // 16-key units, evenly over the splits
+    const int units = (p.P + 15) / 16;
+    k0 = (int)((long long)units * split / p.splits) * 16;
+    k1 = min((int)((long long)units * (split + 1) / p.splits) * 16, p.P);
   }
-  if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
-  *reinterpret_cast<float4*>(&sm_o[warp][lane * 4]) = make_float4(o0, o1, o2, o3);
-  __syncthreads();
-  const float mx = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-  float ls = 0.f, acc = 0.f;
-  if (mx != -INFINITY)
-    for (int w = 0; w < 4; ++w) {
-      const float c = exp2f(sm_m[w] - mx);
-      ls += sm_l[w] * c;
-      acc += sm_o[w][threadIdx.x] * c;
+  const int n_pre = (k1 - k0 + kSpKeys - 1) / kSpKeys;
+  int cp = 0, own = 0;  // kFull: cursor, and own keys that the last row of the block sees
+  if (MODE == kFull) {
+    cp = p.cache_pos ? __ldcg(p.cache_pos + b) : p.uniform_past;
+    if ((cp < 0 || cp > p.max_seq - p.q_len) && threadIdx.x == 0 && blockIdx.x == 0)
+      raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
+    cp = min(cp, p.max_seq);
+    own = min(max(cp + (min(r0 + 2 * kSpRows, p.rows) - 1) / p.G + 1, 0), p.max_seq);
+  }
+  const int ntiles = n_pre + (MODE == kFull ? (own + kSpKeys - 1) / kSpKeys : 0);
+  const bool two = MODE == kKeys ? ntiles > 1 : r0 + kSpRows < p.rows;  // the second stream has work
+  // Keys of tile t, and its first row in the K/V tensor maps.
+  auto tile_keys = [&](int t) -> int {
+    return t < n_pre ? min(kSpKeys, k1 - k0 - t * kSpKeys) : min(kSpKeys, own - (t - n_pre) * kSpKeys);
+  };
+  // Ring position of tile t's K and V: the order in which the MMA warp uses them.
+  auto idx_k = [](int t) { return MODE == kKeys ? (t == 0 ? 0 : 2 * t - 1) : 2 * t; };
+  auto idx_v = [&](int t) { return MODE == kKeys && t + 1 < ntiles ? 2 * t + 2 : 2 * t + 1; };
+
+  if (warp == 8) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      auto load = [&](int t, bool key) {
+        const int s = it % kSlots;
+        if (!ok || *(volatile int*)&s_abort ||
+            (it >= kSlots && !mbar_wait(&empty[s], (uint32_t)(it / kSlots - 1) & 1u, p.err, 0x31))) {
+          ok = false;
+          return;
+        }
+        const bool pre = t < n_pre;
+        const CUtensorMap* map = pre ? (key ? &tm_kp : &tm_vp) : (key ? &tm_kc : &tm_vc);
+        const int y = pre ? h * p.prefix_cap + k0 + t * kSpKeys : (b * p.Hkv + h) * p.max_seq + (t - n_pre) * kSpKeys;
+        const int boxes = (tile_keys(t) + kSpBox - 1) / kSpBox;
+        unsigned char* st = ring + s * kSpSlot;
+        mbar_arrive_expect_tx(&full[s], (uint32_t)boxes * kSpBox * 256);
+        for (int x = 0; x < boxes; ++x) {
+          tma_load_2d(st + x * kSpBox * 128, map, 0, y + x * kSpBox, &full[s]);
+          tma_load_2d(st + kSpKvHalf + x * kSpBox * 128, map, 64, y + x * kSpBox, &full[s]);
+        }
+        ++it;
+      };
+      if (MODE == kKeys && ntiles > 0) load(0, true);
+      for (int t = 0; t < ntiles; ++t) {
+        if (MODE != kKeys) load(t, true);
+        else if (t + 1 < ntiles) load(t + 1, true);
+        load(t, false);
+      }
+      // After a timeout nobody reads the last copies: wait until they have landed.
+      for (int j = max(0, it - kSlots); !ok && j < it; ++j) mbar_wait(&full[j % kSlots], (uint32_t)(j / kSlots) & 1u, p.err, 0x32);
     }
-  p.out[((size_t)t * p.Hq + h) * kSpHeadDim + threadIdx.x] = f_to_bf16(ls > 0.f ? acc / ls : 0.f);
+  } else if (warp == 9) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0 && ntiles > 0) {
+      constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kSpKeys >> 3) << 17) |
+                                   ((uint32_t)(kSpRows >> 4) << 24);
+      constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                                    ((uint32_t)(kSpHeadDim >> 3) << 17) | ((uint32_t)(kSpRows >> 4) << 24);  // V MN-major
+      auto wait_full = [&](int it) { return mbar_wait(&full[it % kSlots], (uint32_t)(it / kSlots) & 1u, p.err, 0x33); };
+      auto issue_s = [&](int w, int t) -> bool {  // S_w = Q K_t^T
+        if (!wait_full(idx_k(t))) return false;
+        tc_fence_after();
+        const uint32_t sQ = smem_u32(smem) + (MODE == kKeys ? 0 : w * kSpQ);
+        const uint32_t sK = smem_u32(ring + (idx_k(t) % kSlots) * kSpSlot);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_f16(tmem + w * 128, umma_desc_sw128(sQ + (kk >> 2) * kSpQHalf + (kk & 3) * 32),
+                   umma_desc_sw128(sK + (kk >> 2) * kSpKvHalf + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[w]);
+        return true;
+      };
+      auto issue_pv = [&](int w, int j, int t) -> bool {  // O_w += P_w V_t, the stream's j-th tile
+        if (!mbar_wait(&p_full[w], (uint32_t)j & 1u, p.err, 0x34) || !wait_full(idx_v(t))) return false;
+        tc_fence_after();
+        const uint32_t sV = smem_u32(ring + (idx_v(t) % kSlots) * kSpSlot);
+        const int steps = (tile_keys(t) + 15) / 16;
+        for (int kk = 0; kk < steps; ++kk)
+          umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, umma_desc_sw128_mn(sV + kk * 2048, kSpKvHalf),
+                      idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+        return true;
+      };
+      bool ok = mbar_wait(q_full, 0u, p.err, 0x35) && issue_s(0, 0);
+      if (MODE == kKeys) {
+        if (ok) umma_commit(&empty[idx_k(0) % kSlots]);
+        if (ok && two) {
+          ok = issue_s(1, 1);
+          if (ok) umma_commit(&empty[idx_k(1) % kSlots]);
+        }
+        for (int t = 0; ok && t < ntiles; ++t) {
+          ok = issue_pv(t & 1, t >> 1, t);
+          if (ok) umma_commit(&empty[idx_v(t) % kSlots]);
+          if (ok && t + 2 < ntiles) {
+            ok = issue_s(t & 1, t + 2);
+            if (ok) umma_commit(&empty[idx_k(t + 2) % kSlots]);
+          }
+        }
+      } else {
+        if (ok && two) ok = issue_s(1, 0);
+        if (ok) umma_commit(&empty[idx_k(0) % kSlots]);
+        for (int t = 0; ok && t < ntiles; ++t) {
+          for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
+            ok = issue_pv(w, t, t);
+            if (ok && t + 1 < ntiles) ok = issue_s(w, t + 1);
+          }
+          if (!ok) break;
+          umma_commit(&empty[idx_v(t) % kSlots]);
+          if (t + 1 < ntiles) umma_commit(&empty[idx_k(t + 1) % kSlots]);
+        }
+      }
+      if (!ok) s_abort = 1;
+      umma_commit(o_done);
+      mbar_wait(o_done, 0u, p.err, 0x36);  // every product issued here is done before TMEM is given back
+    }
+  } else {
+    // ---------------- softmax streams: warps 0-3 and 4-7, one thread per row ----------------
+    const int w = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const int row = r0 + (MODE == kKeys ? r : w * kSpRows + r);
+    const bool valid = row < p.rows;
+    const bool warp_valid = __any_sync(0xffffffffu, valid);
+    // Query rows into the swizzled tiles: 16 lanes a row, zeros behind the end.
+    for (int c = threadIdx.x; c < (MODE == kKeys ? 1 : 2) * kSpRows * 16; c += kSpSoft) {
+      const int rr = c >> 4, cc = c & 15, gr = r0 + rr;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (gr < p.rows) {
+        const int t = gr / p.G;
+        v = __ldcg(reinterpret_cast<const uint4*>(
+                       p.q + (((size_t)b * p.q_len + t) * p.Hq + h * p.G + (gr - t * p.G)) * kSpHeadDim) + cc);
+      }
+      *reinterpret_cast<uint4*>(smem + (rr >> 7) * kSpQ + pt_off(rr & 127, cc, kSpQHalf)) = v;
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
+
+    const int lim = MODE == kFull ? (valid ? cp + row / p.G : -1) : 0;  // kFull: the row's last own key
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t tS = tmem + w * 128 + lane_off, tO = tmem + 256 + w * 128 + lane_off;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    const int step = MODE == kKeys ? 2 : 1;
+    const int t_end = w == 0 || two ? ntiles : 0;
+    for (int t = MODE == kKeys ? w : 0, j = 0; t < t_end; t += step, ++j) {
+      // Wait results are made warp-uniform: the TMEM accesses are warp-collective.
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], (uint32_t)j & 1u, p.err, 0x37))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int nk = tile_keys(t);
+      if (warp_valid) {
+        const int vis = t < n_pre ? nk : min(nk, lim + 1 - (t - n_pre) * kSpKeys);  // keys of the tile the row sees
+        uint32_t sv[kSpKeys];
+        tmem_ld128(tS, sv);
+        if (!__all_sync(0xffffffffu, vis >= kSpKeys)) {
+#pragma unroll
+          for (int e = 0; e < kSpKeys; ++e)
+            if (e >= vis) sv[e] = 0xff800000u;  // -inf
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kSpKeys; e += 4) {
+#pragma unroll
+          for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], __uint_as_float(sv[e + a]));
+        }
+        const float mraw = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float mt = mraw == -INFINITY ? -INFINITY : mraw * p.scale_log2;
+        float corr = 1.f;
+        if (m_run == -INFINITY) {
+          m_run = mt;  // the row's first visible keys: nothing accumulated yet
+        } else if (mt > m_run + kSpRescaleLog2) {
+          corr = ex2_approx(m_run - mt);
+          m_run = mt;
+        }
+        // O is complete up to the tile before (s_full covers it); the whole warp
+        // joins when any of its rows needs the new scale.
+        if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            float ov[16];
+            tmem_ld16(tO + (uint32_t)(c * 16), ov);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ov[e] *= corr;
+            tmem_st16(tO + (uint32_t)(c * 16), ov);
+          }
+        }
+        const float neg_m = m_run == -INFINITY ? 0.f : -m_run;  // a row without keys so far: exp2(-inf) = 0
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x0 = ex2_approx(fmaf(__uint_as_float(sv[c * 64 + 2 * e]), p.scale_log2, neg_m));
+            const float x1 = ex2_approx(fmaf(__uint_as_float(sv[c * 64 + 2 * e + 1]), p.scale_log2, neg_m));
+            ls[(2 * e) & 3] += x0;
+            ls[(2 * e + 1) & 3] += x1;
+            const __nv_bfloat162 v2 = __floats2bfloat162_rn(x0, x1);
+            pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
+          }
+          tmem_st32(tS + c * 32, pk);
+        }
+        l_run = l_run * corr + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+        tmem_st_wait();
+      }
+      if ((nk & 15) && (MODE == kKeys || w == 0)) {
+        // The last product step of this tile takes 16 keys: clear the V rows past
+        // the end (the memory there is the caller's, and 0 x NaN is NaN).
+        const int it = idx_v(t);
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[it % kSlots], (uint32_t)(it / kSlots) & 1u, p.err, 0x38))) {
+          ok = false;
+          break;
+        }
+        unsigned char* vt = ring + (it % kSlots) * kSpSlot;
+        const int pad = 16 - (nk & 15);
+        for (int c = r; c < pad * 16; c += kSpRows)
+          *reinterpret_cast<uint4*>(vt + pt_off(nk + (c >> 4), c & 15, kSpKvHalf)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
+      tc_fence_before();
+      mbar_arrive(&p_full[w]);
+    }
+    if (!ok) s_abort = 1;
+    // ---------------- epilogue ----------------
+    const bool fin = ntiles > 0 && __all_sync(0xffffffffu, ok && mbar_wait(o_done, 0u, p.err, 0x39));
+    tc_fence_after();
+    if (MODE == kKeys) {
+      // Join the two streams: each writes one half of the dims of its rows.
+      s_ml[w][r] = make_float2(m_run, l_run);
+      named_bar_sync(1, kSpSoft);
+      if (fin && warp_valid) {
+        const float2 a = s_ml[0][r], c = s_ml[1][r];
+        const float m = fmaxf(a.x, c.x);
+        const float fa = a.x == -INFINITY ? 0.f : ex2_approx(a.x - m), fc = c.x == -INFINITY ? 0.f : ex2_approx(c.x - m);
+        const size_t at = ((size_t)h * p.rows + (valid ? row : 0)) * p.splits + split;
+        float4* dst = reinterpret_cast<float4*>(p.part_o + at * kSpHeadDim + w * 64);
+        if (w == 0 && valid) p.part_ml[at] = make_float2(m, a.y * fa + c.y * fc);
+#pragma unroll 1
+        for (int c16 = 0; c16 < 4; ++c16) {
+          float o0[16], o1[16];
+          tmem_ld16(tmem + 256 + lane_off + (uint32_t)(w * 64 + c16 * 16), o0);
+          if (two) tmem_ld16(tmem + 384 + lane_off + (uint32_t)(w * 64 + c16 * 16), o1);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o0[e] = (fa != 0.f ? o0[e] * fa : 0.f) + (two && fc != 0.f ? o1[e] * fc : 0.f);
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[c16 * 4 + e] = make_float4(o0[4 * e], o0[4 * e + 1], o0[4 * e + 2], o0[4 * e + 3]);
+          }
+          __syncwarp();
+        }
+      }
+    } else if (fin && warp_valid) {
+      const size_t at = ((size_t)h * p.rows + (valid ? row : 0)) * p.splits + split;
+      const int tok = valid ? row / p.G : 0;
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      if (MODE == kRows && valid) p.part_ml[at] = make_float2(m_run, l_run);
+#pragma unroll 1
+      for (int c16 = 0; c16 < 8; ++c16) {
+        float ov[16];
+        tmem_ld16(tO + (uint32_t)(c16 * 16), ov);
+        if (MODE == kRows && valid) {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + at * kSpHeadDim + c16 * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[e] = make_float4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
+        } else if (MODE == kFull && valid) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const __nv_bfloat162 v2 = __floats2bfloat162_rn(l_run > 0.f ? ov[2 * e] * inv : 0.f,
+                                                            l_run > 0.f ? ov[2 * e + 1] * inv : 0.f);
+            pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
+          }
+          uint4* dst = reinterpret_cast<uint4*>(
+              p.out + (((size_t)b * p.q_len + tok) * p.Hq + h * p.G + (row - tok * p.G)) * kSpHeadDim + c16 * 16);
+          dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+        }
+        __syncwarp();
+      }
+    } else if (MODE == kFull && ntiles == 0 && valid) {  // no key at all (a cursor outside the cache): zeros
+      const int tok = row / p.G;
+      uint4* dst = reinterpret_cast<uint4*>(
+          p.out + (((size_t)b * p.q_len + tok) * p.Hq + h * p.G + (row - tok * p.G)) * kSpHeadDim);
+      for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
 }
 
 }  // namespace lsb
@@ -78,29 +428,89 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(SpParams p
 namespace lsb_host {
 using namespace lsb;
 
+// Cache strips plus the join with the prefix's key splits (attention_tc.cu).
+int launch_decode_attention_prefix(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
+                                   int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
+                                   int64_t max_seq, float scale, const float* part_o, const float2* part_ml, int n_part,
+                                   void* out, cudaStream_t stream);
+
+struct SpPlan {
+  int mode, row_blocks, splits;
+  int64_t ml_bytes, bytes;
+};
+
+// kFull when the prompt rows alone give three quarters of the SMs a CTA (one
+// launch, nothing written in between); else the prefix is split over the SMs.
+static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len) {
+  SpPlan pl = {};
+  const int64_t g = hq / hkv, sms = sm_count();
+  const int64_t own_blocks = (q_len * g + 2 * kSpRows - 1) / (2 * kSpRows);
+  if (q_len * g >= 2 * kSpRows && own_blocks * hkv * batch * 4 >= sms * 3) {
+    pl.mode = kFull;
+    pl.row_blocks = (int)own_blocks;
+    return pl;
+  }
+  const int64_t rows = batch * q_len * g;
+  pl.mode = rows <= kSpRows ? kKeys : kRows;
+  const int64_t per = pl.mode == kKeys ? kSpRows : 2 * kSpRows;
+  pl.row_blocks = (int)((rows + per - 1) / per);
+  // As many splits as fill the SMs once, at least one 128-key tile each.
+  const int64_t tiles = (prefix_len + kSpKeys - 1) / kSpKeys;
+  int64_t splits = sms / (hkv * pl.row_blocks);
+  if (splits > tiles) splits = tiles;
+  if (splits < 1) splits = 1;
+  pl.splits = (int)splits;
+  pl.ml_bytes = (hkv * rows * pl.splits * 8 + 255) / 256 * 256;
+  pl.bytes = prefix_len > 0 ? pl.ml_bytes + hkv * rows * pl.splits * kSpHeadDim * 4 : 0;
+  return pl;
+}
+
 int shared_prefix_workspace_bytes(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len,
                                   int64_t* bytes) {
-  (void)batch, (void)q_len, (void)hq, (void)hkv, (void)prefix_len;
-  *bytes = 0;
+  *bytes = sp_plan(batch, q_len, hq, hkv, prefix_len).bytes;
   return LS_OK;
 }
 
-int launch_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
-                                   int64_t prefix_cap, const void* k_cache, const void* v_cache,
-                                   const int32_t* cache_pos, int64_t uniform_past, int64_t batch, int64_t q_len,
-                                   int64_t hq, int64_t hkv, int64_t max_seq, float scale, void* out, void* workspace,
-                                   cudaStream_t stream) {
-  (void)workspace;
+template <int MODE>
+static int launch_prefix_tc(const CUtensorMap& kp, const CUtensorMap& vp, const CUtensorMap& kc, const CUtensorMap& vc,
+                            const SpParams& p, dim3 grid, cudaStream_t stream) {
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, sp_smem(MODE));
+    if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "shared_prefix_attention attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kSpThreads);
+  cfg.dynamicSmemBytes = sp_smem(MODE);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_tc_kernel<MODE>, kp, vp, kc, vc, p);
+  return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "shared_prefix_attention launch: %s", cudaGetErrorString(e));
+}
+
+static int launch_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
+                                          int64_t prefix_cap, const void* k_cache, const void* v_cache,
+                                          const int32_t* cache_pos, int64_t uniform_past, int64_t batch, int64_t q_len,
+                                          int64_t hq, int64_t hkv, int64_t max_seq, float scale, void* out,
+                                          void* workspace, cudaStream_t stream) {
+  const SpPlan pl = sp_plan(batch, q_len, hq, hkv, prefix_len);
   SpParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k_prefix = static_cast<const __nv_bfloat16*>(k_prefix);
-  p.v_prefix = static_cast<const __nv_bfloat16*>(v_prefix);
-  p.k_cache = static_cast<const __nv_bfloat16*>(k_cache);
-  p.v_cache = static_cast<const __nv_bfloat16*>(v_cache);
   p.cache_pos = cache_pos;
   p.uniform_past = (int)uniform_past;
+  p.part_ml = static_cast<float2*>(workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pl.ml_bytes);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.err = device_error_ptr();
+  p.rows = (int)((pl.mode == kFull ? 1 : batch) * q_len * (hq / hkv));
   p.q_len = (int)q_len;
   p.Hq = (int)hq;
   p.Hkv = (int)hkv;
@@ -108,18 +518,31 @@ int launch_shared_prefix_attention(const void* q, const void* k_prefix, const vo
   p.P = (int)prefix_len;
   p.prefix_cap = (int)prefix_cap;
   p.max_seq = (int)max_seq;
+  p.splits = pl.splits;
   p.scale_log2 = scale * 1.4426950408889634f;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(batch * q_len), (unsigned)hq);
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, shared_prefix_attention_kernel, p);
-  return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "shared_prefix_attention launch: %s", cudaGetErrorString(e));
+  CUtensorMap kp, vp, kc, vc;
+  int rc = LS_OK;
+  if (prefix_len > 0) {
+    rc = make_map(&kp, k_prefix, hkv * prefix_cap, kSpHeadDim, kSpBox);
+    if (!rc) rc = make_map(&vp, v_prefix, hkv * prefix_cap, kSpHeadDim, kSpBox);
+  }
+  if (pl.mode == kFull) {
+    if (!rc) rc = make_map(&kc, k_cache, batch * hkv * max_seq, kSpHeadDim, kSpBox);
+    if (!rc) rc = make_map(&vc, v_cache, batch * hkv * max_seq, kSpHeadDim, kSpBox);
+    if (rc) return rc;
+    if (prefix_len == 0) kp = kc, vp = vc;  // no tile of it is read
+    return launch_prefix_tc<kFull>(kp, vp, kc, vc, p, dim3((unsigned)pl.row_blocks, (unsigned)hkv, (unsigned)batch),
+                                   stream);
+  }
+  if (rc) return rc;
+  if (prefix_len > 0) {
+    const dim3 grid((unsigned)pl.splits, (unsigned)pl.row_blocks, (unsigned)hkv);
+    rc = pl.mode == kKeys ? launch_prefix_tc<kKeys>(kp, vp, kp, vp, p, grid, stream)
+                          : launch_prefix_tc<kRows>(kp, vp, kp, vp, p, grid, stream);
+    if (rc) return rc;
+  }
+  return launch_decode_attention_prefix(q, k_cache, v_cache, cache_pos, uniform_past, batch, q_len, hq, hkv, max_seq,
+                                        scale, p.part_o, p.part_ml, prefix_len > 0 ? pl.splits : 0, out, stream);
 }
 
 }  // namespace lsb_host
@@ -153,8 +576,12 @@ int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* 
              "ls_shared_prefix_attention: prefix_len=%lld without prefix pointers", (long long)prefix_len);
   LS_REQUIRE(prefix_len <= prefix_cap && prefix_cap < (1ll << 30), LS_ERR_KV_OVERFLOW,
              "prefix_len=%lld beyond prefix_cap=%lld", (long long)prefix_len, (long long)prefix_cap);
-  LS_REQUIRE(max_seq > 0 && max_seq < (1ll << 30) && batch * q_len < (1ll << 31), LS_ERR_INVALID_ARGUMENT,
-             "ls_shared_prefix_attention: bad sizes");
+  LS_REQUIRE(max_seq > 0 && max_seq < (1ll << 30), LS_ERR_INVALID_ARGUMENT, "ls_shared_prefix_attention: bad sizes");
+  LS_REQUIRE(batch * num_kv_heads * max_seq < (1ll << 31) - 256 && num_kv_heads * prefix_cap < (1ll << 31) - 256 &&
+                 batch * q_len * num_heads < (1ll << 31) - 256,
+             LS_ERR_UNSUPPORTED_SHAPE, "ls_shared_prefix_attention: %lld x %lld strips of %lld or %lld positions, %lld rows",
+             (long long)batch, (long long)num_kv_heads, (long long)max_seq, (long long)prefix_cap,
+             (long long)(batch * q_len * num_heads));
   LS_REQUIRE(cache_pos || (uniform_past >= 0 && uniform_past + q_len <= max_seq), LS_ERR_KV_OVERFLOW,
              "uniform_past=%lld + q_len=%lld beyond max_seq=%lld", (long long)uniform_past, (long long)q_len,
              (long long)max_seq);

@@ -97,6 +97,10 @@ def test_decode_and_verify_rows(hq, hkv, batch, q_len, prefix, lens, slots):
     (2, 70, 32, 8, 500, 128),  # 280 rows per sequence and kv head: prompts
     (3, 129, 16, 8, 333, 200),
     (1, 300, 8, 2, 0, 301),  # a prompt without a prefix
+    (8, 100, 32, 8, 700, 260),  # prompts that fill the GPU by their rows: 400 rows per sequence and kv head
+    (20, 140, 16, 8, 129, 200),
+    (9, 65, 32, 8, 0, 130),
+    (40, 257, 8, 4, 64, 300),
 ])
 def test_wide_batches_and_prompts(batch, q_len, hq, hkv, prefix, slots):
     lens = [(37 * b) % max(1, slots - q_len) for b in range(batch)]
