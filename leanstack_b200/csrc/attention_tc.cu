@@ -41,7 +41,6 @@ constexpr int kTaMergeBytes = kTaWarps * kTaRows * (kTaHeadDim + 2) * 4;  // reu
 constexpr int kTaRecvBytes = kTaRows * kTaHeadDim * 4 + 2 * kTaMaxSplits * kTaRows * 4;
 constexpr int kTaSmemBytes = kTaRingBytes + kTaRecvBytes;
 constexpr int kTaQStageBytes = kTaRows * kTaHeadDim * 2;  // fused mode: the CTA's normalised query rows
-constexpr int kTaMaxPart = 512;  // key splits of a shared prefix that the join holds weights for
 static_assert(kTaMergeBytes <= kTaRingBytes, "merge buffers must fit in the ring");
 
 struct TaParams {
@@ -66,10 +65,10 @@ struct TaParams {
   __nv_bfloat16* v_store;
   int rope_len, rope_offset;
   float eps;
-  // Join with the key splits of a shared prefix (shared_prefix.cu): per kv head
-  // and batch-wide row, n_part groups of unnormalised O and (m, l).
-  const float* part_o;    // [Hkv][B q_len G][n_part][D]
-  const float2* part_ml;  // [Hkv][B q_len G][n_part]
+  // Rows behind a shared prefix (shared_prefix.cu): the strip is one more group
+  // of keys, its unnormalised O and (m, l) go to the last of n_part groups.
+  float* part_o;    // [Hkv][B q_len G][n_part][D]
+  float2* part_ml;  // [Hkv][B q_len G][n_part]
   int n_part;
 };
 
@@ -125,10 +124,10 @@ __device__ __forceinline__ uint32_t ta_swz(int key, int chunk) {
   return (uint32_t)(key * (kTaHeadDim * 2) + ((chunk ^ (key & 7)) << 4));
 }
 
-// PREFIX: the rows also attend over a shared prefix, whose key splits the
-// previous kernel forms; this one reads its own inputs and keys while that runs
-// (it starts only after every CTA of it has seen the kernels before complete)
-// and waits for it before the join.
+// PREFIX: the rows also attend over a shared prefix, whose groups the previous
+// kernel is forming.  Nothing here needs them: that kernel's CTAs let this one
+// start only after the kernels before are complete, so it runs beside it; one
+// CTA waits for it at the end, so that whoever waits for this kernel has both.
 template <bool FUSED, bool PREFIX = false>
 __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParams p) {
   extern __shared__ __align__(128) unsigned char ta_smem[];
@@ -142,7 +141,7 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   // table and the norm weights are written by no kernel that can still be
   // running (the cursor and accept kernels let their dependents start only at
   // their own end), so the first K/V copies go out under the projection's tail.
-  if (!FUSED && (!PREFIX || p.n_part == 0)) grid_dep_wait();
+  if (!FUSED && (!PREFIX || p.n_part == 1)) grid_dep_wait();
   grid_dep_launch();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -390,55 +389,12 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   __syncthreads();
   if (p.splits > 1) ta_cluster_wait();  // every CTA of the cluster has started: remote stores are safe
 
-  // PREFIX: the weights of the row's groups, own keys first.  The row's shared
-  // maximum over own splits is known only after they meet, so the weights of a
-  // cluster are formed there; with one split, here.
-  float* wgt = reinterpret_cast<float*>(ta_smem + kTaMergeBytes);  // [16][1 + n_part], own weight first
-  float* wsum = wgt + kTaRows * (1 + (PREFIX ? p.n_part : 0));     // [16]: the sum of all weights
-  const size_t prow0 = PREFIX ? (size_t)hkv * gridDim.z * p.R + (size_t)b * p.R + r0 : 0;
-  auto prefix_weights = [&](int r, float m_own, float l_own) {  // one warp per row
-    const float2* ml = p.part_ml + (prow0 + r) * p.n_part;
-    float mx = m_own;
-    for (int c = lane; c < p.n_part; c += 32) mx = fmaxf(mx, __ldcg(ml + c).x);
-    mx = warp_max(mx);
-    const float f = m_own == -INFINITY ? 0.f : exp2f(m_own - mx);
-    float sum = 0.f;
-    for (int c = lane; c < p.n_part; c += 32) {
-      const float2 v = __ldcg(ml + c);
-      const float fc = v.x == -INFINITY ? 0.f : exp2f(v.x - mx);
-      wgt[r * (1 + p.n_part) + 1 + c] = fc;
-      sum += v.y * fc;
-    }
-    sum = warp_sum(sum) + l_own * f;
-    if (lane == 0) {
-      wgt[r * (1 + p.n_part)] = f;
-      wsum[r] = sum;
-    }
+  const size_t prow0 = PREFIX ? ((size_t)hkv * gridDim.z + b) * p.R + r0 : 0;
+  auto own_group = [&](int r) { return (prow0 + r) * p.n_part + p.n_part - 1; };
+  auto wait_for_prefix = [&]() {
+    if (p.n_part > 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+      grid_dep_wait();
   };
-  auto prefix_join = [&](int r, int dim, float acc) -> float {  // the finished output of dim `dim` of row r
-    const float* wr = wgt + r * (1 + p.n_part);
-    const float* po = p.part_o + (prow0 + r) * p.n_part * kTaHeadDim + dim;
-    float o = wr[0] != 0.f ? acc * wr[0] : 0.f;
-#pragma unroll 4
-    for (int c = 0; c < p.n_part; ++c) {
-      const float v = __ldcg(po + (size_t)c * kTaHeadDim);
-      o += wr[1 + c] != 0.f ? v * wr[1 + c] : 0.f;
-    }
-    return wsum[r] > 0.f ? o / wsum[r] : 0.f;
-  };
-  if (PREFIX) {
-    if (p.n_part > 0) grid_dep_wait();
-    if (p.splits == 1) {
-      for (int r = warp; r < nrows; r += kTaWarps) {
-        float mx = -INFINITY, ls = 0.f;
-        for (int k = 0; k < kTaWarps; ++k) mx = fmaxf(mx, wm[k * kTaRows + r]);
-        if (mx != -INFINITY)
-          for (int k = 0; k < kTaWarps; ++k) ls += wl[k * kTaRows + r] * exp2f(wm[k * kTaRows + r] - mx);
-        prefix_weights(r, mx, ls);
-      }
-      __syncthreads();
-    }
-  }
 
   const int d = threadIdx.x;  // one output dimension per thread (kTaThreads == kTaHeadDim)
   const int w = kTaHeadDim / p.splits;  // dims each cluster CTA finishes
@@ -455,11 +411,13 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
         acc += wo[((size_t)k * kTaRows + r) * kTaHeadDim + d] * sc;
       }
     }
-    if (p.splits == 1) {
+    if (PREFIX && p.splits == 1) {
+      p.part_o[own_group(r) * kTaHeadDim + d] = acc;
+      if (d == 0) p.part_ml[own_group(r)] = make_float2(mx, ls);
+    } else if (p.splits == 1) {
       const int row = r0 + r;
       const int i = row / p.G, gq = row - (row / p.G) * p.G;
-      p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + d] =
-          f_to_bf16(PREFIX ? prefix_join(r, d, acc) : acc / ls);
+      p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + d] = f_to_bf16(acc / ls);
     } else {
       const int owner = d / w;
       ta_st_remote(recv_o + ((size_t)s * kTaRows + r) * w + (d - owner * w), (uint32_t)owner, acc);
@@ -469,20 +427,11 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
       }
     }
   }
-  if (p.splits == 1) return;
-  ta_cluster_sync();  // release this CTA's remote stores, acquire the others'
-  if (PREFIX) {
-    for (int r = warp; r < nrows; r += kTaWarps) {
-      float mx = -INFINITY, ls = 0.f;
-      for (int c = 0; c < p.splits; ++c) mx = fmaxf(mx, recv_m[c * kTaRows + r]);
-      if (mx != -INFINITY)
-        for (int c = 0; c < p.splits; ++c)
-          if (recv_m[c * kTaRows + r] != -INFINITY) ls += recv_l[c * kTaRows + r] * exp2f(recv_m[c * kTaRows + r] - mx);
-      prefix_weights(r, mx, ls);
-    }
-    __syncthreads();
+  if (p.splits == 1) {
+    if (PREFIX) wait_for_prefix();
+    return;
   }
-
+  ta_cluster_sync();  // release this CTA's remote stores, acquire the others'
   for (int idx = threadIdx.x; idx < nrows * w; idx += kTaThreads) {
     const int r = idx / w, dd = idx - r * w;
     float mx = -INFINITY;
@@ -495,11 +444,16 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
       ls += recv_l[c * kTaRows + r] * sc;
       acc += recv_o[((size_t)c * kTaRows + r) * w + dd] * sc;
     }
+    if (PREFIX) {
+      p.part_o[own_group(r) * kTaHeadDim + s * w + dd] = acc;
+      if (s == 0 && dd == 0) p.part_ml[own_group(r)] = make_float2(mx, ls);
+      continue;
+    }
     const int row = r0 + r;
     const int i = row / p.G, gq = row - (row / p.G) * p.G;
-    p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + s * w + dd] =
-        f_to_bf16(PREFIX ? prefix_join(r, s * w + dd, acc) : acc / ls);
+    p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + s * w + dd] = f_to_bf16(acc / ls);
   }
+  if (PREFIX) wait_for_prefix();
 }
 
 }  // namespace lsb
@@ -594,19 +548,17 @@ int launch_decode_attention_tc(const void* q, const void* k_cache, const void* v
   return launch_ta<false>(p, pl, batch, hkv, stream);
 }
 
-// The same rows behind a shared prefix of n_part key splits (shared_prefix.cu).
-int launch_decode_attention_prefix(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
-                                   int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
-                                   int64_t max_seq, float scale, const float* part_o, const float2* part_ml, int n_part,
-                                   void* out, cudaStream_t stream) {
+// The strips' groups of rows behind a shared prefix (shared_prefix.cu), into the
+// last of n_part groups; n_part > 1: beside the kernel that forms the others.
+int launch_decode_attention_group(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
+                                  int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
+                                  int64_t max_seq, float scale, float* part_o, float2* part_ml, int n_part,
+                                  cudaStream_t stream) {
   const TaPlan pl = ta_plan(batch, q_len, hq, hkv, max_seq);
   if ((int64_t)hkv * pl.RG > 65535)
     return set_error(LS_ERR_UNSUPPORTED_SHAPE, "shared_prefix_attention: %lld kv heads x %d row groups exceed the grid",
                      (long long)hkv, pl.RG);
-  static_assert(kTaMergeBytes + kTaRows * (1 + kTaMaxPart + 1) * 4 <= kTaRingBytes, "weights must fit in the ring");
-  if (n_part > kTaMaxPart)
-    return set_error(LS_ERR_UNSUPPORTED_SHAPE, "shared_prefix_attention: %d key splits", n_part);
-  TaParams p = ta_params(pl, k_cache, v_cache, cache_pos, uniform_past, q_len, hq, hkv, max_seq, scale, out);
+  TaParams p = ta_params(pl, k_cache, v_cache, cache_pos, uniform_past, q_len, hq, hkv, max_seq, scale, nullptr);
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.part_o = part_o;
   p.part_ml = part_ml;

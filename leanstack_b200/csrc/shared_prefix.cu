@@ -9,48 +9,53 @@
 // l = sum e^(s - m) and O = sum e^(s - m) v, groups join as
 //   M = max m,  o = sum_g e^(m_g - M) O_g / sum_g e^(m_g - M) l_g.
 // So the prefix is one group per key split, formed once for ALL query rows of a
-// kv head (B q_len G rows, whatever sequence they belong to), and the cache
-// strip of a sequence is another, formed by the decode-attention kernel, which
-// joins the groups in its epilogue (attention_tc.cu).  Per prefix key and kv
-// head 512 bytes are read once for R rows and 4 D R flops done on them: memory
-// is the bound below about 250 rows, the tensor cores above.
+// kv head (B q_len G rows, whatever sequence they belong to) by prefix_tc_kernel;
+// the cache strip of a sequence is another, formed beside it by the decode
+// attention (attention_tc.cu); prefix_join_kernel joins them.  Per prefix key
+// and kv head 512 bytes are read once for R rows and 4 D R flops done on them:
+// memory is the bound below about 250 rows, the tensor cores above.
 //
-// prefix_tc_kernel, one CTA per SM:
-//   * warp 8 streams 128-key K and V tiles with TMA (128-byte swizzle, boxes of
-//     32 keys so that a split's last tile fetches no more than it needs) through
-//     a ring of 32 KB slots;
-//   * warp 9 issues S = Q K^T into TMEM (fp32, 128 columns) and O += P V with P
-//     taken from TMEM, where it replaces the S it came from;
+// prefix_tc_kernel:
+//   * warp 8 streams 64-key K and V tiles with TMA (128-byte swizzle, boxes of
+//     32 keys so that a split's last tile fetches little more than it needs)
+//     through a ring of 16 KB slots;
+//   * warps 9 and 10, one per softmax stream, issue S = Q K^T into TMEM (fp32, 64
+//     columns) and O += P V with P taken from TMEM, where it replaces the S it
+//     came from (a warp needs about 1100 cycles to wait for and issue a tile's
+//     two products, more than they take: one warp for both streams was the bound);
 //   * warps 0-7 are two softmax streams of 128 threads, one thread per row, a
-//     whole 128-key row of S in registers: no shuffles, no shared memory on the
-//     way from S to P.  While one stream exponentiates, the tensor core works
-//     for the other.  Rows (kRows): the streams hold two 128-row tiles and share
-//     every K/V tile.  Keys (kKeys, at most 128 rows): they hold the same rows
-//     and take alternate K/V tiles; their results join in the epilogue.
+//     whole 64-key row of S in registers: no shuffles, no shared memory on the
+//     way from S to P.  Each stream has two S buffers, so the scores of its next
+//     tile are there when it is done with one.  Rows (kRows): the streams hold
+//     two 128-row tiles and share every K/V tile.  Keys (kKeys, at most 128
+//     rows): they hold the same rows and take alternate K/V tiles; their results
+//     join in the epilogue, and 114 KB of shared memory and 120 registers leave
+//     room for a CTA of the decode attention on the same SM.
 //   * P is rounded to bf16 (2^-8 of each probability, independent from key to
 //     key, against one more 2^-8 when the output is rounded), the row sum is
 //     taken before that rounding in fp32.  The maximum in use moves only when a
 //     score exceeds it by 2^8; then O is rescaled in TMEM.
 //   * kFull: a prompt's rows.  A CTA owns 256 rows of one (sequence, kv head)
 //     and walks the prefix tiles, then the sequence's own tiles with the causal
-//     mask, and writes the finished rows: no partials.
+//     mask, and writes the finished rows: no partials, no join.
 #include "tcgen05.cuh"
 
 namespace lsb {
 
 constexpr int kSpHeadDim = 128;
 constexpr int kSpRows = 128;                       // rows of one stream (MMA M)
-constexpr int kSpKeys = 128;                       // keys per tile
+constexpr int kSpKeys = 64;                        // keys per tile
 constexpr int kSpBox = 32;                         // keys per TMA box
 constexpr int kSpQHalf = kSpRows * 128;            // 64 dims of 128 rows: 16 KB
 constexpr int kSpQ = 2 * kSpQHalf;                 // one 128-row Q tile: 32 KB
-constexpr int kSpKvHalf = kSpKeys * 128;           // 64 dims of 128 keys: 16 KB
-constexpr int kSpSlot = 2 * kSpKvHalf;             // one K or V tile: 32 KB
-constexpr int kSpThreads = 320;
+constexpr int kSpKvHalf = kSpKeys * 128;           // 64 dims of 64 keys: 8 KB
+constexpr int kSpSlot = 2 * kSpKvHalf;             // one K or V tile: 16 KB
+constexpr int kSpThreads = 352;
 constexpr int kSpSoft = 256;
 constexpr float kSpRescaleLog2 = 8.f;
 enum SpMode { kKeys = 0, kRows = 1, kFull = 2 };
-constexpr int sp_slots(int mode) { return mode == kKeys ? 5 : 4; }
+constexpr int sp_slots(int mode) { return mode == kKeys ? 5 : 8; }
+constexpr int sp_ahead(int mode) { return mode == kKeys ? 4 : 2; }  // tiles whose S is issued before the first PV
 constexpr int sp_ring(int mode) { return mode == kKeys ? kSpQ : 2 * kSpQ; }  // ring offset, behind Q
 constexpr int sp_bars(int mode) { return sp_ring(mode) + sp_slots(mode) * kSpSlot; }
 constexpr int sp_smem(int mode) { return 1024 + sp_bars(mode) + 256; }
@@ -59,45 +64,51 @@ struct SpParams {
   const __nv_bfloat16* q;  // [M, Hq, D]
   const int* cache_pos;    // [B] or null (then uniform_past); kFull only
   int uniform_past;
-  float* part_o;           // [Hkv][rows][splits][D]: unnormalised O of each key split
-  float2* part_ml;         // [Hkv][rows][splits]: (m, l)
+  float* part_o;           // [Hkv][rows][n_part][D]: unnormalised O of each key group
+  float2* part_ml;         // [Hkv][rows][n_part]: (m, l)
   __nv_bfloat16* out;      // kFull: [M, Hq * D]
   int* err;
   int rows;                // kKeys / kRows: B q_len G; kFull: q_len G
-  int q_len, Hq, Hkv, G, P, prefix_cap, max_seq, splits;
+  int q_len, Hq, Hkv, G, P, prefix_cap, max_seq, splits, n_part;
   float scale_log2;
 };
 
 template <int MODE>
-__global__ void __launch_bounds__(kSpThreads, 1)
+__global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys: at most 120 registers
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
                      const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc, SpParams p) {
-  constexpr int kSlots = sp_slots(MODE);
+  constexpr int kSlots = sp_slots(MODE), kAhead = sp_ahead(MODE);
   extern __shared__ unsigned char sp_smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(sp_smem_raw) + 1023) & ~size_t(1023));
   unsigned char* ring = smem + sp_ring(MODE);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + sp_bars(MODE));
   uint64_t* empty = full + kSlots;
-  uint64_t* s_full = empty + kSlots;  // [2]: a stream's scores are in TMEM (and all its earlier products done)
-  uint64_t* p_full = s_full + 2;      // [2]: a stream's probabilities are in TMEM
-  uint64_t* q_full = p_full + 2;
-  uint64_t* o_done = q_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 1);
+  uint64_t* s_full = empty + kSlots;  // [stream][buffer]: scores are in TMEM
+  uint64_t* p_full = s_full + 4;      // [stream][buffer]: probabilities are in TMEM
+  uint64_t* o_part = p_full + 4;      // [stream][buffer]: the product that read them is done
+  uint64_t* o_done = o_part + 4;      // [stream]: its last product is done
+  uint64_t* q_full = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   __shared__ int s_abort;
   __shared__ float2 s_ml[2][kSpRows];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row_blk = MODE == kFull ? gridDim.x - 1 - blockIdx.x : blockIdx.y;  // kFull: the longest first
+  const int r0 = row_blk * (MODE == kKeys ? kSpRows : 2 * kSpRows);
+  const bool both = MODE != kKeys && r0 + kSpRows < p.rows;  // two row tiles: both streams use every K/V tile
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], both ? 2 : 1);
     }
-    for (int w = 0; w < 2; ++w) {
+    for (int w = 0; w < 4; ++w) {
       mbar_init(&s_full[w], 1);
       mbar_init(&p_full[w], kSpRows);
+      mbar_init(&o_part[w], 1);
     }
     mbar_init(q_full, kSpSoft);
-    mbar_init(o_done, 1);
+    mbar_init(&o_done[0], 1);
+    mbar_init(&o_done[1], 1);
     s_abort = 0;
     mbar_fence_init();
   }
@@ -110,7 +121,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S of the streams: columns 0, 128; O: 256, 384
+  const uint32_t tmem = *tmem_slot;  // stream w: S buffers at columns 128 w and 128 w + 64, O at 256 + 128 w
 
   // Every CTA waits before it lets the next kernel start: what that kernel reads
   // besides this one's results was complete before.
@@ -120,8 +131,6 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   // This CTA's rows and keys.
   const int h = MODE == kFull ? blockIdx.y : blockIdx.z;
   const int b = MODE == kFull ? blockIdx.z : 0;
-  const int row_blk = MODE == kFull ? gridDim.x - 1 - blockIdx.x : blockIdx.y;  // kFull: the longest first
-  const int r0 = row_blk * (MODE == kKeys ? kSpRows : 2 * kSpRows);
   const int split = MODE == kFull ? 0 : blockIdx.x;
   int k0 = 0, k1 = p.P;  // prefix keys
   if (MODE != kFull) {   // 16-key units, evenly over the splits
@@ -139,14 +148,15 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     own = min(max(cp + (min(r0 + 2 * kSpRows, p.rows) - 1) / p.G + 1, 0), p.max_seq);
   }
   const int ntiles = n_pre + (MODE == kFull ? (own + kSpKeys - 1) / kSpKeys : 0);
-  const bool two = MODE == kKeys ? ntiles > 1 : r0 + kSpRows < p.rows;  // the second stream has work
+  const bool two = MODE == kKeys ? ntiles > 1 : both;  // the second stream has work
   // Keys of tile t, and its first row in the K/V tensor maps.
   auto tile_keys = [&](int t) -> int {
     return t < n_pre ? min(kSpKeys, k1 - k0 - t * kSpKeys) : min(kSpKeys, own - (t - n_pre) * kSpKeys);
   };
-  // Ring position of tile t's K and V: the order in which the MMA warp uses them.
-  auto idx_k = [](int t) { return MODE == kKeys ? (t == 0 ? 0 : 2 * t - 1) : 2 * t; };
-  auto idx_v = [&](int t) { return MODE == kKeys && t + 1 < ntiles ? 2 * t + 2 : 2 * t + 1; };
+  // The ring holds K of the first kAhead tiles, then V_0, K_kAhead, V_1, ...: the
+  // order in which they are used.  Positions of K_t and V_t:
+  auto idx_k = [](int t) { return t < kAhead ? t : 2 * t - kAhead + 1; };
+  auto idx_v = [&](int t) { return min(ntiles, kAhead) + t + max(0, min(t, ntiles - kAhead)); };
 
   if (warp == 8) {
     // ---------------- TMA producer ----------------
@@ -172,76 +182,59 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         ++it;
       };
-      if (MODE == kKeys && ntiles > 0) load(0, true);
+      for (int t = 0; t < min(ntiles, kAhead); ++t) load(t, true);
       for (int t = 0; t < ntiles; ++t) {
-        if (MODE != kKeys) load(t, true);
-        else if (t + 1 < ntiles) load(t + 1, true);
         load(t, false);
+        if (t + kAhead < ntiles) load(t + kAhead, true);
       }
       // After a timeout nobody reads the last copies: wait until they have landed.
       for (int j = max(0, it - kSlots); !ok && j < it; ++j) mbar_wait(&full[j % kSlots], (uint32_t)(j / kSlots) & 1u, p.err, 0x32);
     }
-  } else if (warp == 9) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0 && ntiles > 0) {
+  } else if (warp >= 9) {
+    // ---------------- MMA issuers, one warp per stream, uniformly ----------------
+    const int w = __shfl_sync(0xffffffffu, warp - 9, 0);
+    if (ntiles > 0 && (w == 0 || two)) {
       constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kSpKeys >> 3) << 17) |
                                    ((uint32_t)(kSpRows >> 4) << 24);
       constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
                                     ((uint32_t)(kSpHeadDim >> 3) << 17) | ((uint32_t)(kSpRows >> 4) << 24);  // V MN-major
-      auto wait_full = [&](int it) { return mbar_wait(&full[it % kSlots], (uint32_t)(it / kSlots) & 1u, p.err, 0x33); };
-      auto issue_s = [&](int w, int t) -> bool {  // S_w = Q K_t^T
-        if (!wait_full(idx_k(t))) return false;
-        tc_fence_after();
-        const uint32_t sQ = smem_u32(smem) + (MODE == kKeys ? 0 : w * kSpQ);
-        const uint32_t sK = smem_u32(ring + (idx_k(t) % kSlots) * kSpSlot);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_f16(tmem + w * 128, umma_desc_sw128(sQ + (kk >> 2) * kSpQHalf + (kk & 3) * 32),
-                   umma_desc_sw128(sK + (kk >> 2) * kSpKvHalf + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[w]);
-        return true;
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem) + (MODE == kKeys ? 0 : w * kSpQ));
+      const uint64_t k_desc = umma_desc_sw128(smem_u32(ring)), v_desc = umma_desc_sw128_mn(smem_u32(ring), kSpKvHalf);
+      const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
+      bool ok = mbar_wait(q_full, 0u, p.err, 0x35);
+      auto wait_full = [&](int it) { ok = ok && mbar_wait(&full[it % kSlots], (uint32_t)(it / kSlots) & 1u, p.err, 0x33); };
+      // The stream's j-th tile t: S = Q K_t^T into buffer j & 1.  A stream's products
+      // run in the order of issue, so the P that the buffer held has been read.
+      auto issue_s = [&](int j, int t) {
+        const int s = idx_k(t) % kSlots;
+        umma_k128_n64(tS + (j & 1) * kSpKeys, q_desc, k_desc + s * (kSpSlot >> 4), idesc_s, 0u);
+        umma_commit_warp(&s_full[2 * w + (j & 1)]);
+        umma_commit_warp(&empty[s]);
       };
-      auto issue_pv = [&](int w, int j, int t) -> bool {  // O_w += P_w V_t, the stream's j-th tile
-        if (!mbar_wait(&p_full[w], (uint32_t)j & 1u, p.err, 0x34) || !wait_full(idx_v(t))) return false;
+      constexpr int kStep = MODE == kKeys ? 2 : 1;  // the stream's tiles: w, w + 2, ... or all
+      const int t0 = MODE == kKeys ? w : 0;
+      for (int t = t0, j = 0; ok && t < min(ntiles, kAhead); t += kStep, ++j) {
+        wait_full(idx_k(t));
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t sV = smem_u32(ring + (idx_v(t) % kSlots) * kSpSlot);
-        const int steps = (tile_keys(t) + 15) / 16;
-        for (int kk = 0; kk < steps; ++kk)
-          umma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, umma_desc_sw128_mn(sV + kk * 2048, kSpKvHalf),
-                      idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-        return true;
-      };
-      bool ok = mbar_wait(q_full, 0u, p.err, 0x35) && issue_s(0, 0);
-      if (MODE == kKeys) {
-        if (ok) umma_commit(&empty[idx_k(0) % kSlots]);
-        if (ok && two) {
-          ok = issue_s(1, 1);
-          if (ok) umma_commit(&empty[idx_k(1) % kSlots]);
-        }
-        for (int t = 0; ok && t < ntiles; ++t) {
-          ok = issue_pv(t & 1, t >> 1, t);
-          if (ok) umma_commit(&empty[idx_v(t) % kSlots]);
-          if (ok && t + 2 < ntiles) {
-            ok = issue_s(t & 1, t + 2);
-            if (ok) umma_commit(&empty[idx_k(t + 2) % kSlots]);
-          }
-        }
-      } else {
-        if (ok && two) ok = issue_s(1, 0);
-        if (ok) umma_commit(&empty[idx_k(0) % kSlots]);
-        for (int t = 0; ok && t < ntiles; ++t) {
-          for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
-            ok = issue_pv(w, t, t);
-            if (ok && t + 1 < ntiles) ok = issue_s(w, t + 1);
-          }
-          if (!ok) break;
-          umma_commit(&empty[idx_v(t) % kSlots]);
-          if (t + 1 < ntiles) umma_commit(&empty[idx_k(t + 1) % kSlots]);
-        }
+        issue_s(j, t);
       }
-      if (!ok) s_abort = 1;
-      umma_commit(o_done);
-      mbar_wait(o_done, 0u, p.err, 0x36);  // every product issued here is done before TMEM is given back
+      for (int t = t0, j = 0; ok && t < ntiles; t += kStep, ++j) {
+        const bool more = t + kAhead < ntiles;
+        wait_full(idx_v(t));
+        if (more) wait_full(idx_k(t + kAhead));
+        ok = ok && mbar_wait(&p_full[2 * w + (j & 1)], (uint32_t)(j >> 1) & 1u, p.err, 0x34);
+        if (!ok) break;
+        tc_fence_after();
+        const int s = idx_v(t) % kSlots;
+        umma_ta_k64(tO, tS + (j & 1) * kSpKeys, v_desc + s * (kSpSlot >> 4), idesc_pv, j > 0 ? 1u : 0u);  // O += P V_t
+        if (more) issue_s(j + 2, t + kAhead);
+        umma_commit_warp(&o_part[2 * w + (j & 1)]);
+        umma_commit_warp(&empty[s]);
+      }
+      if (!ok && lane == 0) s_abort = 1;
+      umma_commit_warp(&o_done[w]);
+      mbar_wait(&o_done[w], 0u, p.err, 0x36);  // every product issued here is done before TMEM is given back
     }
   } else {
     // ---------------- softmax streams: warps 0-3 and 4-7, one thread per row ----------------
@@ -249,30 +242,37 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     const int row = r0 + (MODE == kKeys ? r : w * kSpRows + r);
     const bool valid = row < p.rows;
     const bool warp_valid = __any_sync(0xffffffffu, valid);
-    // Query rows into the swizzled tiles: 16 lanes a row, zeros behind the end.
-    for (int c = threadIdx.x; c < (MODE == kKeys ? 1 : 2) * kSpRows * 16; c += kSpSoft) {
-      const int rr = c >> 4, cc = c & 15, gr = r0 + rr;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (gr < p.rows) {
-        const int t = gr / p.G;
-        v = __ldcg(reinterpret_cast<const uint4*>(
-                       p.q + (((size_t)b * p.q_len + t) * p.Hq + h * p.G + (gr - t * p.G)) * kSpHeadDim) + cc);
+    // Query rows into the swizzled tiles: 16 lanes a row, zeros behind the end;
+    // eight loads in flight per thread before the first store.
+#pragma unroll
+    for (int tile = 0; tile < (MODE == kKeys ? 1 : 2); ++tile) {
+      uint4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int gr = r0 + tile * kSpRows + (int)(threadIdx.x >> 4) + 16 * u, t = gr / p.G;
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (gr < p.rows)
+          v[u] = __ldcg(reinterpret_cast<const uint4*>(
+                            p.q + (((size_t)b * p.q_len + t) * p.Hq + h * p.G + (gr - t * p.G)) * kSpHeadDim) +
+                        (threadIdx.x & 15));
       }
-      *reinterpret_cast<uint4*>(smem + (rr >> 7) * kSpQ + pt_off(rr & 127, cc, kSpQHalf)) = v;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        *reinterpret_cast<uint4*>(smem + tile * kSpQ + pt_off((threadIdx.x >> 4) + 16 * u, threadIdx.x & 15, kSpQHalf)) = v[u];
     }
     fence_proxy_async_smem();
     mbar_arrive(q_full);
 
     const int lim = MODE == kFull ? (valid ? cp + row / p.G : -1) : 0;  // kFull: the row's last own key
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const uint32_t tS = tmem + w * 128 + lane_off, tO = tmem + 256 + w * 128 + lane_off;
+    const uint32_t tO = tmem + 256 + w * 128 + lane_off;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
     const int step = MODE == kKeys ? 2 : 1;
     const int t_end = w == 0 || two ? ntiles : 0;
     for (int t = MODE == kKeys ? w : 0, j = 0; t < t_end; t += step, ++j) {
       // Wait results are made warp-uniform: the TMEM accesses are warp-collective.
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], (uint32_t)j & 1u, p.err, 0x37))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[2 * w + (j & 1)], (uint32_t)(j >> 1) & 1u, p.err, 0x37))) {
         ok = false;
         break;
       }
@@ -280,8 +280,9 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const int nk = tile_keys(t);
       if (warp_valid) {
         const int vis = t < n_pre ? nk : min(nk, lim + 1 - (t - n_pre) * kSpKeys);  // keys of the tile the row sees
+        const uint32_t tS = tmem + w * 128 + (j & 1) * kSpKeys + lane_off;
         uint32_t sv[kSpKeys];
-        tmem_ld128(tS, sv);
+        tmem_ld64(tS, sv);
         if (!__all_sync(0xffffffffu, vis >= kSpKeys)) {
 #pragma unroll
           for (int e = 0; e < kSpKeys; ++e)
@@ -302,9 +303,14 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           corr = ex2_approx(m_run - mt);
           m_run = mt;
         }
-        // O is complete up to the tile before (s_full covers it); the whole warp
-        // joins when any of its rows needs the new scale.
+        // O is rescaled once the product of the tile before is in it; the whole
+        // warp joins when any of its rows needs the new scale.
         if (__any_sync(0xffffffffu, corr != 1.f)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&o_part[2 * w + ((j - 1) & 1)], (uint32_t)((j - 1) >> 1) & 1u, p.err, 0x3a))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
             float ov[16];
@@ -316,55 +322,57 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         const float neg_m = m_run == -INFINITY ? 0.f : -m_run;  // a row without keys so far: exp2(-inf) = 0
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[kSpKeys / 2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x0 = ex2_approx(fmaf(__uint_as_float(sv[c * 64 + 2 * e]), p.scale_log2, neg_m));
-            const float x1 = ex2_approx(fmaf(__uint_as_float(sv[c * 64 + 2 * e + 1]), p.scale_log2, neg_m));
-            ls[(2 * e) & 3] += x0;
-            ls[(2 * e + 1) & 3] += x1;
-            const __nv_bfloat162 v2 = __floats2bfloat162_rn(x0, x1);
-            pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
-          }
-          tmem_st32(tS + c * 32, pk);
+        for (int e = 0; e < kSpKeys / 2; ++e) {
+          const float x0 = ex2_approx(fmaf(__uint_as_float(sv[2 * e]), p.scale_log2, neg_m));
+          const float x1 = ex2_approx(fmaf(__uint_as_float(sv[2 * e + 1]), p.scale_log2, neg_m));
+          ls[(2 * e) & 3] += x0;
+          ls[(2 * e + 1) & 3] += x1;
+          const __nv_bfloat162 v2 = __floats2bfloat162_rn(x0, x1);
+          pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
         }
+        tmem_st32(tS, pk);
         l_run = l_run * corr + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
         tmem_st_wait();
       }
-      if ((nk & 15) && (MODE == kKeys || w == 0)) {
-        // The last product step of this tile takes 16 keys: clear the V rows past
-        // the end (the memory there is the caller's, and 0 x NaN is NaN).
+      if (nk < kSpKeys) {
+        // The product takes 64 keys: clear the V rows past the tile's end (the
+        // memory there is the caller's or not loaded, and 0 x NaN is NaN).  Two
+        // streams that share the tile both do: neither waits for the other.
         const int it = idx_v(t);
         if (!__all_sync(0xffffffffu, mbar_wait(&full[it % kSlots], (uint32_t)(it / kSlots) & 1u, p.err, 0x38))) {
           ok = false;
           break;
         }
         unsigned char* vt = ring + (it % kSlots) * kSpSlot;
-        const int pad = 16 - (nk & 15);
-        for (int c = r; c < pad * 16; c += kSpRows)
+        for (int c = r; c < (kSpKeys - nk) * 16; c += kSpRows)
           *reinterpret_cast<uint4*>(vt + pt_off(nk + (c >> 4), c & 15, kSpKvHalf)) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
       }
       tc_fence_before();
-      mbar_arrive(&p_full[w]);
+      mbar_arrive(&p_full[2 * w + (j & 1)]);
     }
     if (!ok) s_abort = 1;
     // ---------------- epilogue ----------------
-    const bool fin = ntiles > 0 && __all_sync(0xffffffffu, ok && mbar_wait(o_done, 0u, p.err, 0x39));
+    const bool mine = ntiles > 0 && (w == 0 || two);
+    bool fin = ntiles > 0 && __all_sync(0xffffffffu, ok && (!mine || mbar_wait(&o_done[w], 0u, p.err, 0x39)));
+    if (MODE == kKeys && two) fin = fin && __all_sync(0xffffffffu, mbar_wait(&o_done[w ^ 1], 0u, p.err, 0x39));
     tc_fence_after();
+    // Partials go out through shared memory (the ring, idle now): a thread holds
+    // a row, a warp writes whole 512-byte rows.  16-byte chunk c of row x sits at
+    // chunk c ^ (x mod 32): no bank conflicts either way.
+    float4* stage = reinterpret_cast<float4*>(ring) + (MODE == kKeys ? 0 : w * kSpRows * 32);
     if (MODE == kKeys) {
-      // Join the two streams: each writes one half of the dims of its rows.
+      // Join the two streams: each forms one half of the dims of the rows.
       s_ml[w][r] = make_float2(m_run, l_run);
       named_bar_sync(1, kSpSoft);
       if (fin && warp_valid) {
         const float2 a = s_ml[0][r], c = s_ml[1][r];
         const float m = fmaxf(a.x, c.x);
         const float fa = a.x == -INFINITY ? 0.f : ex2_approx(a.x - m), fc = c.x == -INFINITY ? 0.f : ex2_approx(c.x - m);
-        const size_t at = ((size_t)h * p.rows + (valid ? row : 0)) * p.splits + split;
-        float4* dst = reinterpret_cast<float4*>(p.part_o + at * kSpHeadDim + w * 64);
-        if (w == 0 && valid) p.part_ml[at] = make_float2(m, a.y * fa + c.y * fc);
+        if (w == 0 && valid)
+          p.part_ml[((size_t)h * p.rows + row) * p.n_part + split] = make_float2(m, a.y * fa + c.y * fc);
 #pragma unroll 1
         for (int c16 = 0; c16 < 4; ++c16) {
           float o0[16], o1[16];
@@ -372,27 +380,27 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           if (two) tmem_ld16(tmem + 384 + lane_off + (uint32_t)(w * 64 + c16 * 16), o1);
 #pragma unroll
           for (int e = 0; e < 16; ++e) o0[e] = (fa != 0.f ? o0[e] * fa : 0.f) + (two && fc != 0.f ? o1[e] * fc : 0.f);
-          if (valid) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dst[c16 * 4 + e] = make_float4(o0[4 * e], o0[4 * e + 1], o0[4 * e + 2], o0[4 * e + 3]);
-          }
-          __syncwarp();
+          for (int e = 0; e < 4; ++e)
+            stage[r * 32 + ((w * 16 + c16 * 4 + e) ^ (r & 31))] =
+                make_float4(o0[4 * e], o0[4 * e + 1], o0[4 * e + 2], o0[4 * e + 3]);
         }
       }
+      named_bar_sync(1, kSpSoft);
     } else if (fin && warp_valid) {
-      const size_t at = ((size_t)h * p.rows + (valid ? row : 0)) * p.splits + split;
       const int tok = valid ? row / p.G : 0;
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      if (MODE == kRows && valid) p.part_ml[at] = make_float2(m_run, l_run);
+      if (MODE == kRows && valid) p.part_ml[((size_t)h * p.rows + row) * p.n_part + split] = make_float2(m_run, l_run);
 #pragma unroll 1
       for (int c16 = 0; c16 < 8; ++c16) {
         float ov[16];
         tmem_ld16(tO + (uint32_t)(c16 * 16), ov);
-        if (MODE == kRows && valid) {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + at * kSpHeadDim + c16 * 16);
+        if (MODE == kRows) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dst[e] = make_float4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
-        } else if (MODE == kFull && valid) {
+          for (int e = 0; e < 4; ++e)
+            stage[r * 32 + ((c16 * 4 + e) ^ (r & 31))] =
+                make_float4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
+        } else if (valid) {
           uint32_t pk[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -407,7 +415,16 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         __syncwarp();
       }
-    } else if (MODE == kFull && ntiles == 0 && valid) {  // no key at all (a cursor outside the cache): zeros
+    }
+    if (MODE != kFull && fin) {  // kRows: a warp's own rows; kKeys: 16 of the joined ones
+      const int x0 = MODE == kKeys ? warp * 16 : quad * 32, n = MODE == kKeys ? 16 : 32;
+      const int g0 = r0 + (MODE == kKeys ? 0 : w * kSpRows);
+      float4* dst = reinterpret_cast<float4*>(p.part_o) + (((size_t)h * p.rows + g0) * p.n_part + split) * 32 + lane;
+#pragma unroll 4
+      for (int x = x0; x < x0 + n && g0 + x < p.rows; ++x)
+        dst[(size_t)x * p.n_part * 32] = stage[x * 32 + (lane ^ (x & 31))];
+    }
+    if (MODE == kFull && ntiles == 0 && valid) {  // no key at all (a cursor outside the cache): zeros
       const int tok = row / p.G;
       uint4* dst = reinterpret_cast<uint4*>(
           p.out + (((size_t)b * p.q_len + tok) * p.Hq + h * p.G + (row - tok * p.G)) * kSpHeadDim);
@@ -423,19 +440,74 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   }
 }
 
+// Join of a row's key groups: one warp per row (kv head, token, group member),
+// a lane four dims.  Weights e^(m_g - M) in the lanes, the groups' O as 16-byte
+// vectors, 16 in flight per lane.
+constexpr int kSpJoinWarps = 4;
+__global__ void __launch_bounds__(kSpJoinWarps * 32) prefix_join_kernel(const float* part_o, const float2* part_ml,
+                                                                        int n_part, int rows, int G, int Hq,
+                                                                        __nv_bfloat16* out) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, h = blockIdx.y;
+  const int row = blockIdx.x * kSpJoinWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const size_t at = ((size_t)h * rows + row) * n_part;
+  const float4* po = reinterpret_cast<const float4*>(part_o) + at * (kSpHeadDim / 4) + lane;
+  float M = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 < n_part; c0 += 32) {
+    const int n = min(32, n_part - c0);
+    float4 v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      if (u < n) v[u] = __ldcg(po + (size_t)(c0 + u) * (kSpHeadDim / 4));
+    const float2 ml = lane < n ? __ldcg(part_ml + at + c0 + lane) : make_float2(-INFINITY, 0.f);
+    const float mn = fmaxf(M, warp_max(ml.x));
+    if (mn == -INFINITY) continue;  // no key so far
+    const float corr = exp2f(M - mn), f = exp2f(ml.x - mn);
+    M = mn;
+    l = l * corr + warp_sum(ml.y * f);
+    o.x *= corr, o.y *= corr, o.z *= corr, o.w *= corr;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half) {
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          if (16 + u < n) v[u] = __ldcg(po + (size_t)(c0 + 16 + u) * (kSpHeadDim / 4));
+      }
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const float fu = __shfl_sync(0xffffffffu, f, half * 16 + u);
+        if (half * 16 + u < n && fu != 0.f) {  // a group without weight may hold anything
+          o.x = fmaf(v[u].x, fu, o.x);
+          o.y = fmaf(v[u].y, fu, o.y);
+          o.z = fmaf(v[u].z, fu, o.z);
+          o.w = fmaf(v[u].w, fu, o.w);
+        }
+      }
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const __nv_bfloat162 lo = l > 0.f ? __floats2bfloat162_rn(o.x * inv, o.y * inv) : __floats2bfloat162_rn(0.f, 0.f);
+  const __nv_bfloat162 hi = l > 0.f ? __floats2bfloat162_rn(o.z * inv, o.w * inv) : __floats2bfloat162_rn(0.f, 0.f);
+  const int t = row / G;
+  *reinterpret_cast<uint2*>(out + ((size_t)t * Hq + h * G + (row - t * G)) * kSpHeadDim + lane * 4) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
 }  // namespace lsb
 
 namespace lsb_host {
 using namespace lsb;
 
-// Cache strips plus the join with the prefix's key splits (attention_tc.cu).
-int launch_decode_attention_prefix(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
-                                   int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
-                                   int64_t max_seq, float scale, const float* part_o, const float2* part_ml, int n_part,
-                                   void* out, cudaStream_t stream);
+int launch_decode_attention_group(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
+                                  int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
+                                  int64_t max_seq, float scale, float* part_o, float2* part_ml, int n_part,
+                                  cudaStream_t stream);
 
 struct SpPlan {
-  int mode, row_blocks, splits;
+  int mode, row_blocks, splits, n_part;  // n_part: the prefix's splits and the strip
   int64_t ml_bytes, bytes;
 };
 
@@ -454,14 +526,15 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   pl.mode = rows <= kSpRows ? kKeys : kRows;
   const int64_t per = pl.mode == kKeys ? kSpRows : 2 * kSpRows;
   pl.row_blocks = (int)((rows + per - 1) / per);
-  // As many splits as fill the SMs once, at least one 128-key tile each.
-  const int64_t tiles = (prefix_len + kSpKeys - 1) / kSpKeys;
+  // As many splits as fill the SMs once, of at least 128 keys each.
+  const int64_t most = (prefix_len + 127) / 128;
   int64_t splits = sms / (hkv * pl.row_blocks);
-  if (splits > tiles) splits = tiles;
   if (splits < 1) splits = 1;
+  if (splits > most) splits = most;
   pl.splits = (int)splits;
-  pl.ml_bytes = (hkv * rows * pl.splits * 8 + 255) / 256 * 256;
-  pl.bytes = prefix_len > 0 ? pl.ml_bytes + hkv * rows * pl.splits * kSpHeadDim * 4 : 0;
+  pl.n_part = pl.splits + 1;
+  pl.ml_bytes = (hkv * rows * pl.n_part * 8 + 255) / 256 * 256;
+  pl.bytes = pl.ml_bytes + hkv * rows * pl.n_part * kSpHeadDim * 4;
   return pl;
 }
 
@@ -519,6 +592,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   p.prefix_cap = (int)prefix_cap;
   p.max_seq = (int)max_seq;
   p.splits = pl.splits;
+  p.n_part = pl.n_part;
   p.scale_log2 = scale * 1.4426950408889634f;
   CUtensorMap kp, vp, kc, vc;
   int rc = LS_OK;
@@ -541,8 +615,21 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
                           : launch_prefix_tc<kRows>(kp, vp, kp, vp, p, grid, stream);
     if (rc) return rc;
   }
-  return launch_decode_attention_prefix(q, k_cache, v_cache, cache_pos, uniform_past, batch, q_len, hq, hkv, max_seq,
-                                        scale, p.part_o, p.part_ml, prefix_len > 0 ? pl.splits : 0, out, stream);
+  rc = launch_decode_attention_group(q, k_cache, v_cache, cache_pos, uniform_past, batch, q_len, hq, hkv, max_seq, scale,
+                                     p.part_o, p.part_ml, pl.n_part, stream);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.rows + kSpJoinWarps - 1) / kSpJoinWarps), (unsigned)hkv);
+  cfg.blockDim = dim3(kSpJoinWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_join_kernel, (const float*)p.part_o, (const float2*)p.part_ml,
+                                     pl.n_part, p.rows, p.G, p.Hq, p.out);
+  return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "shared_prefix_attention join launch: %s", cudaGetErrorString(e));
 }
 
 }  // namespace lsb_host

@@ -85,28 +85,76 @@ __device__ __forceinline__ uint32_t pt_off(int r, int c, int half) {
   return (uint32_t)((c >> 3) * half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// D += A B with A read from TMEM (bf16 pairs, 8 columns per 16 of K) and B from shared memory.
-__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// The issue of a whole product by one warp: every lane takes part, an elected
+// one issues, so operands stay in uniform registers (one MMA issued by a lane
+// in a branch of its own measured 73 cycles, more than a 128 x 64 x 16 product
+// takes).  Descriptor offsets are in units of 16 bytes.
+// D (+)= A B^T over K = 128: A [128 rows] and B [64 rows] in two 64-wide swizzled halves, 16 KB and 8 KB apart.
+__device__ __forceinline__ void umma_k128_n64(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          tmem_d),
+      "{\n"
+      " .reg .pred p, q, t;\n"
+      " .reg .b64 a, b;\n"
+      " elect.sync _|q, 0xffffffff;\n"
+      " setp.ne.b32 p, %4, 0;\n"
+      " setp.eq.b32 t, 0, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      " add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 4;\n add.s64 b, %2, 4;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 6;\n add.s64 b, %2, 6;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 1024;\n add.s64 b, %2, 512;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 1026;\n add.s64 b, %2, 514;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 1028;\n add.s64 b, %2, 516;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 1030;\n add.s64 b, %2, 518;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
+// D (+)= A B over K = 64: A in TMEM (bf16 pairs, 8 columns per 16 of K), B MN-major, 16 rows of K 2 KB apart.
+__device__ __forceinline__ void umma_ta_k64(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      " .reg .pred p, q, t;\n"
+      " .reg .b64 b;\n"
+      " .reg .b32 a;\n"
+      " elect.sync _|q, 0xffffffff;\n"
+      " setp.ne.b32 p, %4, 0;\n"
+      " setp.eq.b32 t, 0, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " add.s32 a, %1, 8;\n add.s64 b, %2, 128;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+      " add.s32 a, %1, 16;\n add.s64 b, %2, 256;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+      " add.s32 a, %1, 24;\n add.s64 b, %2, 384;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+      "}\n" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
-// 128 columns of this thread's TMEM lane, complete on return (one asm: the values exist only after the wait).
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+// umma_commit by an elected lane of a converged warp.
+__device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// 64 columns of this thread's TMEM lane, complete on return (one asm: the values exist only after the wait).
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
       "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
-      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
-      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
-      "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
-      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127"
-      "}, [%128];\n"
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
+      "}, [%64];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -115,15 +163,7 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
         "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
         "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
         "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(taddr));
 }
 
