@@ -23,11 +23,10 @@
 //
 // HBM traffic per (sequence, kv head): 512 bytes per visible key (K and V,
 // head_dim 128, bf16), read once; Q and the output are noise.
-#include "common.cuh"
+#include "mma_sync.cuh"
 
 namespace lsb {
 
-constexpr int kTaHeadDim = 128;
 constexpr int kTaWarps = 4;
 constexpr int kTaThreads = kTaWarps * 32;
 constexpr int kTaRows = 16;   // query rows per CTA (MMA M)
@@ -65,42 +64,8 @@ struct TaParams {
   __nv_bfloat16* v_store;
   int rope_len, rope_offset;
   float eps;
-  // Rows behind a shared prefix (shared_prefix.cu): the strip is one more group
-  // of keys, its unnormalised O and (m, l) go to the last of n_part groups.
-  float* part_o;    // [Hkv][B q_len G][n_part][D]
-  float2* part_ml;  // [Hkv][B q_len G][n_part]
-  int n_part;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
 __device__ __forceinline__ uint32_t ta_cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -119,16 +84,7 @@ __device__ __forceinline__ void ta_st_remote(const void* local, uint32_t rank, f
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
-// Byte offset of 16-byte chunk `chunk` (0..15) of key row `key` (0..15) in a tile.
-__device__ __forceinline__ uint32_t ta_swz(int key, int chunk) {
-  return (uint32_t)(key * (kTaHeadDim * 2) + ((chunk ^ (key & 7)) << 4));
-}
-
-// PREFIX: the rows also attend over a shared prefix, whose groups the previous
-// kernel is forming.  Nothing here needs them: that kernel's CTAs let this one
-// start only after the kernels before are complete, so it runs beside it; one
-// CTA waits for it at the end, so that whoever waits for this kernel has both.
-template <bool FUSED, bool PREFIX = false>
+template <bool FUSED>
 __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParams p) {
   extern __shared__ __align__(128) unsigned char ta_smem[];
   float* recv_o = reinterpret_cast<float*>(ta_smem + kTaRingBytes);  // [splits][16][128/splits]
@@ -141,7 +97,7 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   // table and the norm weights are written by no kernel that can still be
   // running (the cursor and accept kernels let their dependents start only at
   // their own end), so the first K/V copies go out under the projection's tail.
-  if (!FUSED && (!PREFIX || p.n_part == 1)) grid_dep_wait();
+  if (!FUSED) grid_dep_wait();
   grid_dep_launch();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -149,8 +105,8 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   const int b = blockIdx.z;
   const int hkv = blockIdx.y / p.RG, rg = blockIdx.y - hkv * p.RG;
   const int s = p.splits > 1 ? (int)ta_cluster_rank() : 0;
-  const int cp = p.cache_pos ? (FUSED || PREFIX ? __ldcg(p.cache_pos + b) : p.cache_pos[b]) : p.uniform_past;
-  int L = min(cp, p.max_seq) + p.q_len;
+  const int cp = p.cache_pos ? (FUSED ? __ldcg(p.cache_pos + b) : p.cache_pos[b]) : p.uniform_past;
+  int L = min(cp, p.max_seq) + p.q_len;  // (a cursor near 2^31 must not wrap)
   if (L > p.max_seq || cp < 0) {
     if (threadIdx.x == 0 && s == 0) raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
     L = min(max(L, 0), p.max_seq);
@@ -259,9 +215,8 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
                                     : p.q + ((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
-      const uint32_t* q2 = reinterpret_cast<const uint32_t*>(qp + ks * 16 + 2 * t4);
-      qa[ks][hr] = valid ? (PREFIX ? __ldcg(q2) : q2[0]) : 0u;
-      qa[ks][2 + hr] = valid ? (PREFIX ? __ldcg(q2 + 4) : q2[4]) : 0u;
+      qa[ks][hr] = valid ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + 2 * t4) : 0u;
+      qa[ks][2 + hr] = valid ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + 8 + 2 * t4) : 0u;
     }
   }
 
@@ -389,13 +344,6 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
   __syncthreads();
   if (p.splits > 1) ta_cluster_wait();  // every CTA of the cluster has started: remote stores are safe
 
-  const size_t prow0 = PREFIX ? ((size_t)hkv * gridDim.z + b) * p.R + r0 : 0;
-  auto own_group = [&](int r) { return (prow0 + r) * p.n_part + p.n_part - 1; };
-  auto wait_for_prefix = [&]() {
-    if (p.n_part > 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
-      grid_dep_wait();
-  };
-
   const int d = threadIdx.x;  // one output dimension per thread (kTaThreads == kTaHeadDim)
   const int w = kTaHeadDim / p.splits;  // dims each cluster CTA finishes
   for (int r = 0; r < nrows; ++r) {
@@ -411,10 +359,7 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
         acc += wo[((size_t)k * kTaRows + r) * kTaHeadDim + d] * sc;
       }
     }
-    if (PREFIX && p.splits == 1) {
-      p.part_o[own_group(r) * kTaHeadDim + d] = acc;
-      if (d == 0) p.part_ml[own_group(r)] = make_float2(mx, ls);
-    } else if (p.splits == 1) {
+    if (p.splits == 1) {
       const int row = r0 + r;
       const int i = row / p.G, gq = row - (row / p.G) * p.G;
       p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + d] = f_to_bf16(acc / ls);
@@ -427,11 +372,9 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
       }
     }
   }
-  if (p.splits == 1) {
-    if (PREFIX) wait_for_prefix();
-    return;
-  }
+  if (p.splits == 1) return;
   ta_cluster_sync();  // release this CTA's remote stores, acquire the others'
+
   for (int idx = threadIdx.x; idx < nrows * w; idx += kTaThreads) {
     const int r = idx / w, dd = idx - r * w;
     float mx = -INFINITY;
@@ -444,16 +387,10 @@ __global__ void __launch_bounds__(kTaThreads) decode_attention_tc_kernel(TaParam
       ls += recv_l[c * kTaRows + r] * sc;
       acc += recv_o[((size_t)c * kTaRows + r) * w + dd] * sc;
     }
-    if (PREFIX) {
-      p.part_o[own_group(r) * kTaHeadDim + s * w + dd] = acc;
-      if (s == 0 && dd == 0) p.part_ml[own_group(r)] = make_float2(mx, ls);
-      continue;
-    }
     const int row = r0 + r;
     const int i = row / p.G, gq = row - (row / p.G) * p.G;
     p.out[((size_t)(b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + s * w + dd] = f_to_bf16(acc / ls);
   }
-  if (PREFIX) wait_for_prefix();
 }
 
 }  // namespace lsb
@@ -483,15 +420,15 @@ static TaPlan ta_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   return pl;
 }
 
-template <bool FUSED, bool PREFIX = false>
+template <bool FUSED>
 static int launch_ta(const TaParams& p, const TaPlan& pl, int64_t batch, int64_t hkv, cudaStream_t stream) {
   constexpr size_t smem = kTaSmemBytes + (FUSED ? kTaQStageBytes : 0);
   static bool attrs_set = false;
   if (!attrs_set) {
     cudaError_t e =
-        cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED, PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED, PREFIX>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      e = cudaFuncSetAttribute(decode_attention_tc_kernel<FUSED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "attention_tc attributes: %s", cudaGetErrorString(e));
     attrs_set = true;
   }
@@ -509,7 +446,7 @@ static int launch_ta(const TaParams& p, const TaPlan& pl, int64_t batch, int64_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attention_tc_kernel<FUSED, PREFIX>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attention_tc_kernel<FUSED>, p);
   if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "decode_attention_tc launch: %s", cudaGetErrorString(e));
   return LS_OK;
 }
@@ -546,24 +483,6 @@ int launch_decode_attention_tc(const void* q, const void* k_cache, const void* v
   TaParams p = ta_params(pl, k_cache, v_cache, cache_pos, uniform_past, q_len, hq, hkv, max_seq, scale, out);
   p.q = static_cast<const __nv_bfloat16*>(q);
   return launch_ta<false>(p, pl, batch, hkv, stream);
-}
-
-// The strips' groups of rows behind a shared prefix (shared_prefix.cu), into the
-// last of n_part groups; n_part > 1: beside the kernel that forms the others.
-int launch_decode_attention_group(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
-                                  int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
-                                  int64_t max_seq, float scale, float* part_o, float2* part_ml, int n_part,
-                                  cudaStream_t stream) {
-  const TaPlan pl = ta_plan(batch, q_len, hq, hkv, max_seq);
-  if ((int64_t)hkv * pl.RG > 65535)
-    return set_error(LS_ERR_UNSUPPORTED_SHAPE, "shared_prefix_attention: %lld kv heads x %d row groups exceed the grid",
-                     (long long)hkv, pl.RG);
-  TaParams p = ta_params(pl, k_cache, v_cache, cache_pos, uniform_past, q_len, hq, hkv, max_seq, scale, nullptr);
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.part_o = part_o;
-  p.part_ml = part_ml;
-  p.n_part = n_part;
-  return launch_ta<false, true>(p, pl, batch, hkv, stream);
 }
 
 // One decode token per sequence (q_len 1) straight from the raw fused QKV

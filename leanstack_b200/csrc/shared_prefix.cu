@@ -10,27 +10,31 @@
 //   M = max m,  o = sum_g e^(m_g - M) O_g / sum_g e^(m_g - M) l_g.
 // So the prefix is one group per key split, formed once for ALL query rows of a
 // kv head (B q_len G rows, whatever sequence they belong to) by prefix_tc_kernel;
-// the cache strip of a sequence is another, formed beside it by the decode
-// attention (attention_tc.cu); prefix_join_kernel joins them.  Per prefix key
-// and kv head 512 bytes are read once for R rows and 4 D R flops done on them:
-// memory is the bound below about 250 rows, the tensor cores above.
+// a sequence's cache strip is a few more, formed beside it by strip_groups_kernel;
+// prefix_join_kernel joins them.  Per prefix key and kv head 512 bytes are read
+// once for R rows and 4 D R flops done on them: memory is the bound below about
+// 250 rows, the tensor cores above.
 //
 // prefix_tc_kernel:
 //   * warp 8 streams 64-key K and V tiles with TMA (128-byte swizzle, boxes of
 //     32 keys so that a split's last tile fetches little more than it needs)
 //     through a ring of 16 KB slots;
-//   * warps 9 and 10, one per softmax stream, issue S = Q K^T into TMEM (fp32, 64
-//     columns) and O += P V with P taken from TMEM, where it replaces the S it
-//     came from (a warp needs about 1100 cycles to wait for and issue a tile's
-//     two products, more than they take: one warp for both streams was the bound);
+//   * warps 9 and 10 issue S = Q K^T into TMEM (fp32, 64 columns) and O += P V
+//     with P taken from TMEM, where it replaces the S it came from.  A warp needs
+//     about 1100 cycles to wait for and issue a tile's two products, more than
+//     they take, so each stream has its own where both use every tile (kRows,
+//     kFull: every slot is then seen, in ring order, and released by both).  With
+//     kKeys one warp issues for both streams: a slot belongs to one of them, and
+//     only a reader that has seen a slot's every use can tell their parities
+//     apart.  There memory (1400 cycles a tile at its share of HBM) is slower;
 //   * warps 0-7 are two softmax streams of 128 threads, one thread per row, a
 //     whole 64-key row of S in registers: no shuffles, no shared memory on the
 //     way from S to P.  Each stream has two S buffers, so the scores of its next
 //     tile are there when it is done with one.  Rows (kRows): the streams hold
 //     two 128-row tiles and share every K/V tile.  Keys (kKeys, at most 128
 //     rows): they hold the same rows and take alternate K/V tiles; their results
-//     join in the epilogue, and 114 KB of shared memory and 120 registers leave
-//     room for a CTA of the decode attention on the same SM.
+//     join in the epilogue, and 114 KB of shared memory and 128 registers leave
+//     room for three strip CTAs on the same SM.
 //   * P is rounded to bf16 (2^-8 of each probability, independent from key to
 //     key, against one more 2^-8 when the output is rounded), the row sum is
 //     taken before that rounding in fp32.  The maximum in use moves only when a
@@ -38,6 +42,7 @@
 //   * kFull: a prompt's rows.  A CTA owns 256 rows of one (sequence, kv head)
 //     and walks the prefix tiles, then the sequence's own tiles with the causal
 //     mask, and writes the finished rows: no partials, no join.
+#include "mma_sync.cuh"
 #include "tcgen05.cuh"
 
 namespace lsb {
@@ -50,10 +55,10 @@ constexpr int kSpQHalf = kSpRows * 128;            // 64 dims of 128 rows: 16 KB
 constexpr int kSpQ = 2 * kSpQHalf;                 // one 128-row Q tile: 32 KB
 constexpr int kSpKvHalf = kSpKeys * 128;           // 64 dims of 64 keys: 8 KB
 constexpr int kSpSlot = 2 * kSpKvHalf;             // one K or V tile: 16 KB
-constexpr int kSpThreads = 352;
 constexpr int kSpSoft = 256;
 constexpr float kSpRescaleLog2 = 8.f;
 enum SpMode { kKeys = 0, kRows = 1, kFull = 2 };
+constexpr int sp_threads(int mode) { return mode == kKeys ? 320 : 352; }
 constexpr int sp_slots(int mode) { return mode == kKeys ? 5 : 8; }
 constexpr int sp_ahead(int mode) { return mode == kKeys ? 4 : 2; }  // tiles whose S is issued before the first PV
 constexpr int sp_ring(int mode) { return mode == kKeys ? kSpQ : 2 * kSpQ; }  // ring offset, behind Q
@@ -74,7 +79,7 @@ struct SpParams {
 };
 
 template <int MODE>
-__global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys: at most 120 registers
+__global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  // kKeys: at most 128 registers
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
                      const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc, SpParams p) {
   constexpr int kSlots = sp_slots(MODE), kAhead = sp_ahead(MODE);
@@ -86,7 +91,7 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
   uint64_t* s_full = empty + kSlots;  // [stream][buffer]: scores are in TMEM
   uint64_t* p_full = s_full + 4;      // [stream][buffer]: probabilities are in TMEM
   uint64_t* o_part = p_full + 4;      // [stream][buffer]: the product that read them is done
-  uint64_t* o_done = o_part + 4;      // [stream]: its last product is done
+  uint64_t* o_done = o_part + 4;      // [issuing warp]: its last product is done
   uint64_t* q_full = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   __shared__ int s_abort;
@@ -154,8 +159,7 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
     return t < n_pre ? min(kSpKeys, k1 - k0 - t * kSpKeys) : min(kSpKeys, own - (t - n_pre) * kSpKeys);
   };
   // The ring holds K of the first kAhead tiles, then V_0, K_kAhead, V_1, ...: the
-  // order in which they are used.  Positions of K_t and V_t:
-  auto idx_k = [](int t) { return t < kAhead ? t : 2 * t - kAhead + 1; };
+  // order in which they are used.  Position of V_t:
   auto idx_v = [&](int t) { return min(ntiles, kAhead) + t + max(0, min(t, ntiles - kAhead)); };
 
   if (warp == 8) {
@@ -191,50 +195,56 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
       for (int j = max(0, it - kSlots); !ok && j < it; ++j) mbar_wait(&full[j % kSlots], (uint32_t)(j / kSlots) & 1u, p.err, 0x32);
     }
   } else if (warp >= 9) {
-    // ---------------- MMA issuers, one warp per stream, uniformly ----------------
-    const int w = __shfl_sync(0xffffffffu, warp - 9, 0);
-    if (ntiles > 0 && (w == 0 || two)) {
+    // ---------------- MMA issuers: the whole warp, uniformly ----------------
+    const int w0 = __shfl_sync(0xffffffffu, warp - 9, 0);
+    if (ntiles > 0 && (w0 == 0 || two)) {
       constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kSpKeys >> 3) << 17) |
                                    ((uint32_t)(kSpRows >> 4) << 24);
       constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
                                     ((uint32_t)(kSpHeadDim >> 3) << 17) | ((uint32_t)(kSpRows >> 4) << 24);  // V MN-major
-      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem) + (MODE == kKeys ? 0 : w * kSpQ));
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem) + w0 * kSpQ);
       const uint64_t k_desc = umma_desc_sw128(smem_u32(ring)), v_desc = umma_desc_sw128_mn(smem_u32(ring), kSpKvHalf);
-      const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
       bool ok = mbar_wait(q_full, 0u, p.err, 0x35);
-      auto wait_full = [&](int it) { ok = ok && mbar_wait(&full[it % kSlots], (uint32_t)(it / kSlots) & 1u, p.err, 0x33); };
-      // The stream's j-th tile t: S = Q K_t^T into buffer j & 1.  A stream's products
-      // run in the order of issue, so the P that the buffer held has been read.
-      auto issue_s = [&](int j, int t) {
-        const int s = idx_k(t) % kSlots;
-        umma_k128_n64(tS + (j & 1) * kSpKeys, q_desc, k_desc + s * (kSpSlot >> 4), idesc_s, 0u);
+      // The ring is consumed in order: the next slot and its parity.
+      int slot = 0;
+      uint32_t parity = 0;
+      auto take = [&]() -> int {
+        const int s = slot;
+        ok = ok && mbar_wait(&full[s], parity, p.err, 0x33);
+        if (++slot == kSlots) slot = 0, parity ^= 1u;
+        return s;
+      };
+      // Stream w's j-th tile: S = Q K^T into buffer j & 1.  Products run in the order
+      // of issue, so the P that the buffer held has been read.
+      auto issue_s = [&](int w, int j, int s) {
+        umma_k128_n64(tmem + w * 128 + (j & 1) * kSpKeys, q_desc, k_desc + s * (kSpSlot >> 4), idesc_s, 0u);
         umma_commit_warp(&s_full[2 * w + (j & 1)]);
         umma_commit_warp(&empty[s]);
       };
-      constexpr int kStep = MODE == kKeys ? 2 : 1;  // the stream's tiles: w, w + 2, ... or all
-      const int t0 = MODE == kKeys ? w : 0;
-      for (int t = t0, j = 0; ok && t < min(ntiles, kAhead); t += kStep, ++j) {
-        wait_full(idx_k(t));
+      for (int t = 0; ok && t < min(ntiles, kAhead); ++t) {
+        const int s = take();
         if (!ok) break;
         tc_fence_after();
-        issue_s(j, t);
+        if (MODE == kKeys) issue_s(t & 1, t >> 1, s);
+        else issue_s(w0, t, s);
       }
-      for (int t = t0, j = 0; ok && t < ntiles; t += kStep, ++j) {
+      for (int t = 0; ok && t < ntiles; ++t) {
+        const int w = MODE == kKeys ? t & 1 : w0, j = MODE == kKeys ? t >> 1 : t;
         const bool more = t + kAhead < ntiles;
-        wait_full(idx_v(t));
-        if (more) wait_full(idx_k(t + kAhead));
+        const int sv = take();
+        const int sk = more ? take() : 0;
         ok = ok && mbar_wait(&p_full[2 * w + (j & 1)], (uint32_t)(j >> 1) & 1u, p.err, 0x34);
         if (!ok) break;
         tc_fence_after();
-        const int s = idx_v(t) % kSlots;
-        umma_ta_k64(tO, tS + (j & 1) * kSpKeys, v_desc + s * (kSpSlot >> 4), idesc_pv, j > 0 ? 1u : 0u);  // O += P V_t
-        if (more) issue_s(j + 2, t + kAhead);
+        umma_ta_k64(tmem + 256 + w * 128, tmem + w * 128 + (j & 1) * kSpKeys, v_desc + sv * (kSpSlot >> 4), idesc_pv,
+                    j > 0 ? 1u : 0u);  // O += P V
+        if (more) issue_s(w, j + 2, sk);
         umma_commit_warp(&o_part[2 * w + (j & 1)]);
-        umma_commit_warp(&empty[s]);
+        umma_commit_warp(&empty[sv]);
       }
       if (!ok && lane == 0) s_abort = 1;
-      umma_commit_warp(&o_done[w]);
-      mbar_wait(&o_done[w], 0u, p.err, 0x36);  // every product issued here is done before TMEM is given back
+      umma_commit_warp(&o_done[w0]);
+      mbar_wait(&o_done[w0], 0u, p.err, 0x36);  // every product issued here is done before TMEM is given back
     }
   } else {
     // ---------------- softmax streams: warps 0-3 and 4-7, one thread per row ----------------
@@ -355,9 +365,8 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
     }
     if (!ok) s_abort = 1;
     // ---------------- epilogue ----------------
-    const bool mine = ntiles > 0 && (w == 0 || two);
-    bool fin = ntiles > 0 && __all_sync(0xffffffffu, ok && (!mine || mbar_wait(&o_done[w], 0u, p.err, 0x39)));
-    if (MODE == kKeys && two) fin = fin && __all_sync(0xffffffffu, mbar_wait(&o_done[w ^ 1], 0u, p.err, 0x39));
+    const int wd = MODE == kKeys ? 0 : w;  // the warp that issued this stream's products
+    const bool fin = ntiles > 0 && __all_sync(0xffffffffu, ok && (wd == 1 && !two ? true : mbar_wait(&o_done[wd], 0u, p.err, 0x39)));
     tc_fence_after();
     // Partials go out through shared memory (the ring, idle now): a thread holds
     // a row, a warp writes whole 512-byte rows.  16-byte chunk c of row x sits at
@@ -374,16 +383,17 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
         if (w == 0 && valid)
           p.part_ml[((size_t)h * p.rows + row) * p.n_part + split] = make_float2(m, a.y * fa + c.y * fc);
 #pragma unroll 1
-        for (int c16 = 0; c16 < 4; ++c16) {
-          float o0[16], o1[16];
-          tmem_ld16(tmem + 256 + lane_off + (uint32_t)(w * 64 + c16 * 16), o0);
-          if (two) tmem_ld16(tmem + 384 + lane_off + (uint32_t)(w * 64 + c16 * 16), o1);
+        for (int c32 = 0; c32 < 2; ++c32) {
+          float o0[32], o1[32];
+          tmem_ld32(tmem + 256 + lane_off + (uint32_t)(w * 64 + c32 * 32), o0);
+          if (two) tmem_ld32(tmem + 384 + lane_off + (uint32_t)(w * 64 + c32 * 32), o1);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o0[e] = (fa != 0.f ? o0[e] * fa : 0.f) + (two && fc != 0.f ? o1[e] * fc : 0.f);
+          for (int e = 0; e < 32; ++e) o0[e] = (fa != 0.f ? o0[e] * fa : 0.f) + (two && fc != 0.f ? o1[e] * fc : 0.f);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            stage[r * 32 + ((w * 16 + c16 * 4 + e) ^ (r & 31))] =
+          for (int e = 0; e < 8; ++e)
+            stage[r * 32 + ((w * 16 + c32 * 8 + e) ^ (r & 31))] =
                 make_float4(o0[4 * e], o0[4 * e + 1], o0[4 * e + 2], o0[4 * e + 3]);
+          __syncwarp();
         }
       }
       named_bar_sync(1, kSpSoft);
@@ -420,7 +430,7 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
       const int x0 = MODE == kKeys ? warp * 16 : quad * 32, n = MODE == kKeys ? 16 : 32;
       const int g0 = r0 + (MODE == kKeys ? 0 : w * kSpRows);
       float4* dst = reinterpret_cast<float4*>(p.part_o) + (((size_t)h * p.rows + g0) * p.n_part + split) * 32 + lane;
-#pragma unroll 4
+#pragma unroll 8
       for (int x = x0; x < x0 + n && g0 + x < p.rows; ++x)
         dst[(size_t)x * p.n_part * 32] = stage[x * 32 + (lane ^ (x & 31))];
     }
@@ -438,6 +448,174 @@ __global__ void __launch_bounds__(MODE == kKeys ? 544 : kSpThreads, 1)  // kKeys
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
+}
+
+// Groups of a sequence's own strip: one warp per (sequence, kv head, 16 query
+// rows, key chunk), mma.sync m16n8k16 on 16-key tiles from a 3-stage cp.async
+// ring, online softmax in registers, P rounded to bf16 as in prefix_tc_kernel.
+// A chunk is a row's share of its sequence's keys, at least kStMinBlocks tiles; a
+// chunk behind the end leaves a group without weight.  Single warps: nothing to
+// merge, and the SM's scheduler evens out strips of different lengths.
+constexpr int kStMinBlocks = 4;
+constexpr int kStStages = 3;
+constexpr int kStTile = 16 * kTaHeadDim * 2;  // 16 keys of K or V: 4 KB
+
+struct StParams {
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k_cache;
+  const __nv_bfloat16* v_cache;
+  const int* cache_pos;
+  int uniform_past;
+  float* part_o;    // groups n_pre .. n_part - 1 are written here
+  float2* part_ml;
+  int* err;
+  int q_len, Hq, Hkv, G, R, RG, max_seq, n_pre, n_part;
+  float scale_log2;
+};
+
+__global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
+  __shared__ __align__(128) unsigned char sm[kStStages * 2 * kStTile + kStTile];
+  // Behind a prefix: that kernel's CTAs let this one start only after every kernel
+  // before is complete, so what is read here is there, and one CTA waits for it at
+  // the end, so that whoever waits for this kernel has both.
+  if (p.n_pre == 0) grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x, g8 = lane >> 2, t4 = lane & 3;
+  const int b = blockIdx.z, hkv = blockIdx.y / p.RG, r0 = (blockIdx.y - hkv * p.RG) * 16;
+  const int nrows = min(16, p.R - r0);
+  int cp = p.cache_pos ? __ldcg(p.cache_pos + b) : p.uniform_past;
+  if ((cp < 0 || cp > p.max_seq - p.q_len) && lane == 0) raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
+  cp = min(cp, p.max_seq);
+  const int L = min(max(cp + p.q_len, 0), p.max_seq);
+  const int blocks = (L + 15) / 16;
+  const int per = max((blocks + (int)gridDim.x - 1) / (int)gridDim.x, kStMinBlocks);
+  const int blk0 = min((int)blockIdx.x * per, blocks), nb = min(per, blocks - blk0);
+  const size_t at = (((size_t)hkv * gridDim.z + b) * p.R + r0) * p.n_part + p.n_pre + blockIdx.x;  // row r: + r n_part
+  if (nb <= 0) {
+    if (lane < nrows) p.part_ml[at + (size_t)lane * p.n_part] = make_float2(-INFINITY, 0.f);
+  } else {
+    const size_t base = ((size_t)b * p.Hkv + hkv) * p.max_seq * kTaHeadDim;
+    const uint32_t ring = smem_u32(sm), sq = ring + kStStages * 2 * kStTile;
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {  // the query rows, zeros behind the end; with the first tiles' copies
+      const int r = (lane >> 4) + 2 * it, row = r0 + (r < nrows ? r : 0);
+      const int i = row / p.G, gq = row - i * p.G;
+      cp_async16(sq + ta_swz(r, lane & 15),
+                 p.q + (((size_t)b * p.q_len + i) * p.Hq + hkv * p.G + gq) * kTaHeadDim + (lane & 15) * 8,
+                 r < nrows ? 16u : 0u);
+    }
+    auto load_block = [&](int n) {
+      const uint32_t st = ring + (n % kStStages) * 2 * kStTile;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int r = (lane >> 4) + 2 * it, j = (blk0 + n) * 16 + r;
+        const bool ok = j < L;
+        const size_t off = base + (size_t)(ok ? j : 0) * kTaHeadDim + (lane & 15) * 8;
+        cp_async16(st + ta_swz(r, lane & 15), p.k_cache + off, ok ? 16u : 0u);
+        cp_async16(st + kStTile + ta_swz(r, lane & 15), p.v_cache + off, ok ? 16u : 0u);
+      }
+    };
+#pragma unroll
+    for (int n = 0; n < kStStages; ++n) {
+      if (n < nb) load_block(n);
+      cp_async_commit();
+    }
+    int lim[2];  // last key the rows g8 and g8 + 8 see
+#pragma unroll
+    for (int hr = 0; hr < 2; ++hr) lim[hr] = g8 + 8 * hr < nrows ? cp + (r0 + g8 + 8 * hr) / p.G : -1;
+    uint32_t qa[8][4];
+    float o[16][4];
+#pragma unroll
+    for (int nt = 0; nt < 16; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    for (int n = 0; n < nb; ++n) {
+      cp_async_wait<kStStages - 1>();
+      __syncwarp();
+      if (n == 0) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+          ldsm_x4(sq + ta_swz((lane & 7) + ((lane >> 3) & 1) * 8, 2 * ks + (lane >> 4)), qa[ks][0], qa[ks][1], qa[ks][2],
+                  qa[ks][3]);
+      }
+      const uint32_t stK = ring + (n % kStStages) * 2 * kStTile, stV = stK + kStTile;
+      const int jb = (blk0 + n) * 16;
+      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t b00, b01, b10, b11;
+        ldsm_x4(stK + ta_swz((lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)), b00, b01, b10, b11);
+        mma_bf16(sc[0], qa[ks], b00, b01);
+        mma_bf16(sc[1], qa[ks], b10, b11);
+      }
+      float corr[2];
+#pragma unroll
+      for (int hr = 0; hr < 2; ++hr) {  // row g8 + 8 hr: elements 2 hr, 2 hr + 1 of both tiles
+        float mx = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 2 * hr; e < 2 * hr + 2; ++e) {
+            const int j = jb + nt * 8 + 2 * t4 + (e & 1);
+            const float v = j < L && j <= lim[hr] ? sc[nt][e] * p.scale_log2 : -INFINITY;
+            sc[nt][e] = v;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m_run[hr], mx);
+        corr[hr] = m_run[hr] == mn ? 1.f : ex2_approx(m_run[hr] - mn);
+        m_run[hr] = mn;
+        const float neg = mn == -INFINITY ? 0.f : -mn;
+        float ps = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 2 * hr; e < 2 * hr + 2; ++e) {
+            sc[nt][e] = ex2_approx(sc[nt][e] + neg);
+            ps += sc[nt][e];
+          }
+        l_run[hr] = l_run[hr] * corr[hr] + ps;
+      }
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+        for (int nt = 0; nt < 16; ++nt) {
+          o[nt][0] *= corr[0];
+          o[nt][1] *= corr[0];
+          o[nt][2] *= corr[1];
+          o[nt][3] *= corr[1];
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) pa[x] = pack_bf16(sc[x >> 1][(x & 1) * 2], sc[x >> 1][(x & 1) * 2 + 1]);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t v0, v1, v2, v3;
+        ldsm_x4_t(stV + ta_swz((lane & 7) + (((lane >> 3) & 1) << 3), 2 * c + (lane >> 4)), v0, v1, v2, v3);
+        mma_bf16(o[2 * c], pa, v0, v1);
+        mma_bf16(o[2 * c + 1], pa, v2, v3);
+      }
+      __syncwarp();
+      if (n + kStStages < nb) load_block(n + kStStages);
+      cp_async_commit();
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int hr = 0; hr < 2; ++hr) {
+      l_run[hr] += __shfl_xor_sync(0xffffffffu, l_run[hr], 1);
+      l_run[hr] += __shfl_xor_sync(0xffffffffu, l_run[hr], 2);
+      const int r = g8 + 8 * hr;
+      if (r >= nrows) continue;
+      const size_t g = at + (size_t)r * p.n_part;
+      if (t4 == 0) p.part_ml[g] = make_float2(m_run[hr], l_run[hr]);
+#pragma unroll
+      for (int nt = 0; nt < 16; ++nt)
+        *reinterpret_cast<float2*>(p.part_o + g * kTaHeadDim + nt * 8 + 2 * t4) =
+            make_float2(o[nt][2 * hr], o[nt][2 * hr + 1]);
+    }
+  }
+  if (p.n_pre > 0 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+    grid_dep_wait();
 }
 
 // Join of a row's key groups: one warp per row (kv head, token, group member),
@@ -501,19 +679,15 @@ __global__ void __launch_bounds__(kSpJoinWarps * 32) prefix_join_kernel(const fl
 namespace lsb_host {
 using namespace lsb;
 
-int launch_decode_attention_group(const void* q, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
-                                  int64_t uniform_past, int64_t batch, int64_t q_len, int64_t hq, int64_t hkv,
-                                  int64_t max_seq, float scale, float* part_o, float2* part_ml, int n_part,
-                                  cudaStream_t stream);
-
 struct SpPlan {
-  int mode, row_blocks, splits, n_part;  // n_part: the prefix's splits and the strip
+  int mode, row_blocks, splits, chunks;  // key groups: the prefix's splits and the strips' chunks
   int64_t ml_bytes, bytes;
 };
 
+constexpr int kSpMaxChunks = 32;
 // kFull when the prompt rows alone give three quarters of the SMs a CTA (one
 // launch, nothing written in between); else the prefix is split over the SMs.
-static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len) {
+static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len, int64_t max_seq) {
   SpPlan pl = {};
   const int64_t g = hq / hkv, sms = sm_count();
   const int64_t own_blocks = (q_len * g + 2 * kSpRows - 1) / (2 * kSpRows);
@@ -531,17 +705,23 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   int64_t splits = sms / (hkv * pl.row_blocks);
   if (splits < 1) splits = 1;
   if (splits > most) splits = most;
-  pl.splits = (int)splits;
-  pl.n_part = pl.splits + 1;
-  pl.ml_bytes = (hkv * rows * pl.n_part * 8 + 255) / 256 * 256;
-  pl.bytes = pl.ml_bytes + hkv * rows * pl.n_part * kSpHeadDim * 4;
+  pl.splits = prefix_len > 0 ? (int)splits : 0;
+  // Strip chunks: about 2048 warps in all (14 an SM, of which 7 fit at once).
+  const int64_t strips = batch * hkv * ((q_len * g + 15) / 16);
+  int64_t chunks = 2048 / strips;
+  const int64_t longest = (max_seq + 16 * kStMinBlocks - 1) / (16 * kStMinBlocks);
+  if (chunks > longest) chunks = longest;
+  if (chunks > kSpMaxChunks) chunks = kSpMaxChunks;
+  pl.chunks = chunks < 1 ? 1 : (int)chunks;
+  const int64_t groups = pl.splits + pl.chunks;
+  pl.ml_bytes = (hkv * rows * groups * 8 + 255) / 256 * 256;
+  pl.bytes = pl.ml_bytes + hkv * rows * groups * kSpHeadDim * 4;
   return pl;
 }
 
-int shared_prefix_workspace_bytes(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len,
-                                  int64_t* bytes) {
-  *bytes = sp_plan(batch, q_len, hq, hkv, prefix_len).bytes;
-  return LS_OK;
+// The workspace serves every max_seq: as many chunks as any length takes.
+static int64_t shared_prefix_workspace(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len) {
+  return sp_plan(batch, q_len, hq, hkv, prefix_len, (int64_t)1 << 30).bytes;
 }
 
 template <int MODE>
@@ -552,12 +732,16 @@ static int launch_prefix_tc(const CUtensorMap& kp, const CUtensorMap& vp, const 
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, sp_smem(MODE));
+    // All of the SM's memory as shared memory, or the strips' kernel does not fit beside this one.
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(prefix_tc_kernel<MODE>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "shared_prefix_attention attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kSpThreads);
+  cfg.blockDim = dim3(sp_threads(MODE));
   cfg.dynamicSmemBytes = sp_smem(MODE);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -574,7 +758,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
                                           const int32_t* cache_pos, int64_t uniform_past, int64_t batch, int64_t q_len,
                                           int64_t hq, int64_t hkv, int64_t max_seq, float scale, void* out,
                                           void* workspace, cudaStream_t stream) {
-  const SpPlan pl = sp_plan(batch, q_len, hq, hkv, prefix_len);
+  const SpPlan pl = sp_plan(batch, q_len, hq, hkv, prefix_len, max_seq);
   SpParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.cache_pos = cache_pos;
@@ -592,7 +776,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   p.prefix_cap = (int)prefix_cap;
   p.max_seq = (int)max_seq;
   p.splits = pl.splits;
-  p.n_part = pl.n_part;
+  p.n_part = pl.splits + pl.chunks;
   p.scale_log2 = scale * 1.4426950408889634f;
   CUtensorMap kp, vp, kc, vc;
   int rc = LS_OK;
@@ -615,21 +799,42 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
                           : launch_prefix_tc<kRows>(kp, vp, kp, vp, p, grid, stream);
     if (rc) return rc;
   }
-  rc = launch_decode_attention_group(q, k_cache, v_cache, cache_pos, uniform_past, batch, q_len, hq, hkv, max_seq, scale,
-                                     p.part_o, p.part_ml, pl.n_part, stream);
-  if (rc) return rc;
+  StParams st = {};
+  st.q = p.q;
+  st.k_cache = static_cast<const __nv_bfloat16*>(k_cache);
+  st.v_cache = static_cast<const __nv_bfloat16*>(v_cache);
+  st.cache_pos = cache_pos;
+  st.uniform_past = p.uniform_past;
+  st.part_o = p.part_o;
+  st.part_ml = p.part_ml;
+  st.err = p.err;
+  st.q_len = p.q_len;
+  st.Hq = p.Hq;
+  st.Hkv = p.Hkv;
+  st.G = p.G;
+  st.R = p.q_len * p.G;
+  st.RG = (st.R + 15) / 16;
+  st.max_seq = p.max_seq;
+  st.n_pre = pl.splits;
+  st.n_part = p.n_part;
+  st.scale_log2 = p.scale_log2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.rows + kSpJoinWarps - 1) / kSpJoinWarps), (unsigned)hkv);
-  cfg.blockDim = dim3(kSpJoinWarps * 32);
+  cfg.gridDim = dim3((unsigned)pl.chunks, (unsigned)(hkv * st.RG), (unsigned)batch);
+  cfg.blockDim = dim3(32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_join_kernel, (const float*)p.part_o, (const float2*)p.part_ml,
-                                     pl.n_part, p.rows, p.G, p.Hq, p.out);
-  return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "shared_prefix_attention join launch: %s", cudaGetErrorString(e));
+  cudaError_t e = cudaLaunchKernelEx(&cfg, strip_groups_kernel, st);
+  if (e == cudaSuccess) {
+    cfg.gridDim = dim3((unsigned)((p.rows + kSpJoinWarps - 1) / kSpJoinWarps), (unsigned)hkv);
+    cfg.blockDim = dim3(kSpJoinWarps * 32);
+    e = cudaLaunchKernelEx(&cfg, prefix_join_kernel, (const float*)p.part_o, (const float2*)p.part_ml, p.n_part, p.rows,
+                           p.G, p.Hq, p.out);
+  }
+  return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "shared_prefix_attention launch: %s", cudaGetErrorString(e));
 }
 
 }  // namespace lsb_host
@@ -646,7 +851,8 @@ int ls_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t q_len, int
   LS_REQUIRE(batch > 0 && batch <= 65535 && q_len > 0 && q_len < (1ll << 31) && num_kv_heads > 0 && num_heads > 0 &&
                  num_heads <= 65535 && num_heads % num_kv_heads == 0 && prefix_len >= 0 && prefix_len < (1ll << 30),
              LS_ERR_INVALID_ARGUMENT, "ls_shared_prefix_attention_workspace_bytes: bad sizes");
-  return shared_prefix_workspace_bytes(batch, q_len, num_heads, num_kv_heads, prefix_len, bytes);
+  *bytes = shared_prefix_workspace(batch, q_len, num_heads, num_kv_heads, prefix_len);
+  return LS_OK;
 }
 
 int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
@@ -664,6 +870,9 @@ int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* 
   LS_REQUIRE(prefix_len <= prefix_cap && prefix_cap < (1ll << 30), LS_ERR_KV_OVERFLOW,
              "prefix_len=%lld beyond prefix_cap=%lld", (long long)prefix_len, (long long)prefix_cap);
   LS_REQUIRE(max_seq > 0 && max_seq < (1ll << 30), LS_ERR_INVALID_ARGUMENT, "ls_shared_prefix_attention: bad sizes");
+  LS_REQUIRE(num_kv_heads * ((q_len * (num_heads / num_kv_heads) + 15) / 16) <= 65535, LS_ERR_UNSUPPORTED_SHAPE,
+             "ls_shared_prefix_attention: %lld query rows per kv head exceed the grid",
+             (long long)(q_len * (num_heads / num_kv_heads)));
   LS_REQUIRE(batch * num_kv_heads * max_seq < (1ll << 31) - 256 && num_kv_heads * prefix_cap < (1ll << 31) - 256 &&
                  batch * q_len * num_heads < (1ll << 31) - 256,
              LS_ERR_UNSUPPORTED_SHAPE, "ls_shared_prefix_attention: %lld x %lld strips of %lld or %lld positions, %lld rows",
