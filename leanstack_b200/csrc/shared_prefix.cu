@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
 // chunk behind the end leaves a group without weight.  Single warps: nothing to
 // merge, and the SM's scheduler evens out strips of different lengths.
 constexpr int kStMinBlocks = 4;
-constexpr int kStStages = 3;
+constexpr int kStStages = 2;
 constexpr int kStTile = 16 * kTaHeadDim * 2;  // 16 keys of K or V: 4 KB
 
 struct StParams {
@@ -618,9 +618,9 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
     grid_dep_wait();
 }
 
-// Join of a row's key groups: one warp per row (kv head, token, group member),
-// a lane four dims.  Weights e^(m_g - M) in the lanes, the groups' O as 16-byte
-// vectors, 16 in flight per lane.
+// Join of a row's key groups: one warp per row (kv head, token, group member) and
+// half of its dims, a lane two of them.  The groups' weights e^(m_g - M) sit in
+// the lanes, their O is read 32 groups at a time.
 constexpr int kSpJoinWarps = 4;
 __global__ void __launch_bounds__(kSpJoinWarps * 32) prefix_join_kernel(const float* part_o, const float2* part_ml,
                                                                         int n_part, int rows, int G, int Hq,
@@ -628,50 +628,39 @@ __global__ void __launch_bounds__(kSpJoinWarps * 32) prefix_join_kernel(const fl
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31, h = blockIdx.y;
-  const int row = blockIdx.x * kSpJoinWarps + (threadIdx.x >> 5);
+  const int row = (blockIdx.x * kSpJoinWarps + (threadIdx.x >> 5)) >> 1;
+  const int dim = ((threadIdx.x >> 5) & 1) * (kSpHeadDim / 2) + lane * 2;
   if (row >= rows) return;
   const size_t at = ((size_t)h * rows + row) * n_part;
-  const float4* po = reinterpret_cast<const float4*>(part_o) + at * (kSpHeadDim / 4) + lane;
+  const float2* po = reinterpret_cast<const float2*>(part_o + at * kSpHeadDim + dim);
   float M = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 o = make_float2(0.f, 0.f);
   for (int c0 = 0; c0 < n_part; c0 += 32) {
     const int n = min(32, n_part - c0);
-    float4 v[16];
+    float2 v[32];
 #pragma unroll
-    for (int u = 0; u < 16; ++u)
-      if (u < n) v[u] = __ldcg(po + (size_t)(c0 + u) * (kSpHeadDim / 4));
+    for (int u = 0; u < 32; ++u)
+      if (u < n) v[u] = __ldcg(po + (size_t)(c0 + u) * (kSpHeadDim / 2));
     const float2 ml = lane < n ? __ldcg(part_ml + at + c0 + lane) : make_float2(-INFINITY, 0.f);
     const float mn = fmaxf(M, warp_max(ml.x));
     if (mn == -INFINITY) continue;  // no key so far
     const float corr = exp2f(M - mn), f = exp2f(ml.x - mn);
     M = mn;
     l = l * corr + warp_sum(ml.y * f);
-    o.x *= corr, o.y *= corr, o.z *= corr, o.w *= corr;
+    o.x *= corr, o.y *= corr;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half) {
-#pragma unroll
-        for (int u = 0; u < 16; ++u)
-          if (16 + u < n) v[u] = __ldcg(po + (size_t)(c0 + 16 + u) * (kSpHeadDim / 4));
-      }
-#pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const float fu = __shfl_sync(0xffffffffu, f, half * 16 + u);
-        if (half * 16 + u < n && fu != 0.f) {  // a group without weight may hold anything
-          o.x = fmaf(v[u].x, fu, o.x);
-          o.y = fmaf(v[u].y, fu, o.y);
-          o.z = fmaf(v[u].z, fu, o.z);
-          o.w = fmaf(v[u].w, fu, o.w);
-        }
+    for (int u = 0; u < 32; ++u) {
+      const float fu = __shfl_sync(0xffffffffu, f, u);
+      if (u < n && fu != 0.f) {  // a group without weight may hold anything
+        o.x = fmaf(v[u].x, fu, o.x);
+        o.y = fmaf(v[u].y, fu, o.y);
       }
     }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  const __nv_bfloat162 lo = l > 0.f ? __floats2bfloat162_rn(o.x * inv, o.y * inv) : __floats2bfloat162_rn(0.f, 0.f);
-  const __nv_bfloat162 hi = l > 0.f ? __floats2bfloat162_rn(o.z * inv, o.w * inv) : __floats2bfloat162_rn(0.f, 0.f);
+  const __nv_bfloat162 v2 = l > 0.f ? __floats2bfloat162_rn(o.x * inv, o.y * inv) : __floats2bfloat162_rn(0.f, 0.f);
   const int t = row / G;
-  *reinterpret_cast<uint2*>(out + ((size_t)t * Hq + h * G + (row - t * G)) * kSpHeadDim + lane * 4) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  *reinterpret_cast<__nv_bfloat162*>(out + ((size_t)t * Hq + h * G + (row - t * G)) * kSpHeadDim + dim) = v2;
 }
 
 }  // namespace lsb
@@ -829,7 +818,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, strip_groups_kernel, st);
   if (e == cudaSuccess) {
-    cfg.gridDim = dim3((unsigned)((p.rows + kSpJoinWarps - 1) / kSpJoinWarps), (unsigned)hkv);
+    cfg.gridDim = dim3((unsigned)((2 * (int64_t)p.rows + kSpJoinWarps - 1) / kSpJoinWarps), (unsigned)hkv);
     cfg.blockDim = dim3(kSpJoinWarps * 32);
     e = cudaLaunchKernelEx(&cfg, prefix_join_kernel, (const float*)p.part_o, (const float2*)p.part_ml, p.n_part, p.rows,
                            p.G, p.Hq, p.out);
