@@ -686,7 +686,11 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
     return pl;
   }
   const int64_t rows = batch * q_len * g;
-  pl.mode = rows <= kSpRows ? kKeys : kRows;
+  // Few rows: each K/V tile serves 128 rows and what little is computed leaves room
+  // for the strips on the same SM; many: 256 rows share a tile.  Measured at 32 / 8
+  // heads and 8192 shared keys, kKeys / kRows: 192 rows 34 / 37 us, 384 rows 53 / 56,
+  // 768 rows 52 / 49.
+  pl.mode = rows <= 512 ? kKeys : kRows;
   const int64_t per = pl.mode == kKeys ? kSpRows : 2 * kSpRows;
   pl.row_blocks = (int)((rows + per - 1) / per);
   // As many splits as fill the SMs once, of at least 128 keys each.
