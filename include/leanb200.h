@@ -457,14 +457,17 @@ int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const 
  *   bias_ids, bias_values  [m, bias_cap]; ids outside the vocabulary are skipped
  *   allowed   uint32 [m, ceil(vocab / 32)] or NULL (every token)
  *   record    count the picked token and mark it seen
- * NaN logits are never picked.  ls_token_stats_add enters ids [batch, len]
+ * NaN logits are never picked; vocab <= 2^20; the workspace needs no filling.
+ * ls_token_stats_add enters ids [batch, len]
  * (negative: padding) into seen and, unless counts is NULL (a prompt), counts;
  * an id past the vocabulary raises LS_ERR_INVALID_ARGUMENT in the device error
  * flag and is skipped. */
+int ls_constrained_argmax_workspace_bytes(int64_t m, int64_t vocab, int64_t* bytes);
 int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t vocab, int32_t* counts, uint32_t* seen,
                           const float* repetition, const float* frequency, const float* presence,
                           const int32_t* bias_ids, const float* bias_values, int64_t bias_cap, const uint32_t* allowed,
-                          int record, int64_t* out_ids, float* out_logits, ls_stream_t stream);
+                          int record, int64_t* out_ids, float* out_logits, void* workspace,
+                          int64_t workspace_bytes, ls_stream_t stream);
 int ls_token_stats_add(const int64_t* ids, int64_t batch, int64_t len, int64_t vocab, int32_t* counts, uint32_t* seen,
                        ls_stream_t stream);
 

@@ -112,7 +112,8 @@ SIGNATURES: dict[str, list] = {
                                    _p, _p, _i64, _p],
     "ls_lora_delta_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "ls_lora_delta": [_p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _int, _p, _p, _i64, _p],
-    "ls_constrained_argmax": [_p, _int, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _int, _p, _p, _p],
+    "ls_constrained_argmax_workspace_bytes": [_i64, _i64, ctypes.POINTER(_i64)],
+    "ls_constrained_argmax": [_p, _int, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _int, _p, _p, _p, _i64, _p],
     "ls_token_stats_add": [_p, _i64, _i64, _i64, _p, _p, _p],
 }
 _RESTYPES = {"ls_last_error": ctypes.c_char_p}

@@ -12,19 +12,24 @@
 // Seen tokens (prompt or answer) and grammars are bit sets of 32-bit words, so
 // an unmasked bf16 row costs 2 bytes and two bits a token and the counts are
 // read only where the seen bit is set; groups of 8 tokens that the grammar
-// bans outright are not read at all.  The groups are aligned in the flattened
-// [m, vocab] array, not in the row, so that every vocabulary size takes 16-byte
-// accesses; a group's bits are cut from two words.  A row is split over a
-// cluster of CTAs whose winners meet in the first CTA's shared memory: no
-// workspace, no counters, so captured graphs share nothing.  A thread keeps
-// several groups in flight: the bound is the chain bits -> logits -> counts of dependent
-// loads for few rows, and HBM for many.
+// bans outright are not read at all.  Where the vocabulary is no multiple of 8 the
+// groups are aligned in the flattened [m, vocab] array, not in the row, so that
+// these sizes take 16-byte accesses too, and a group's bits are cut from two
+// words.  The CTAs of a row leave one key each and a second, tiny kernel picks the
+// row's token and enters it into its state: no counters to zero, no order of
+// arrival, nothing that two captured graphs share.  (With a row as a cluster of
+// CTAs whose winners met in shared memory, 64 rows of 151936 took 17 us instead of
+// 10: clusters are placed slowly and wait for one another.)  What bounds it: for
+// few rows the chain bits -> logits, counts -> pick of dependent latencies; for
+// many, instruction issue, so a group is kept short: bits as bytes, one maximum
+// per group, seen and biased tokens one at a time.
 #include "common.cuh"
 
 namespace lsb {
 
-constexpr int kTrMaxThreads = 512;
-constexpr int kTrMaxCluster = 16;
+constexpr int kTrThreads = 256;
+
+constexpr int64_t kTrNoKey = INT64_MIN;  // below every argmax_key: a CTA without a candidate
 
 struct TrParams {
   const void* logits;        // [M, V] bf16 or fp32
@@ -36,9 +41,9 @@ struct TrParams {
   const int* bias_ids;       // [M, bias_cap] or null; entries outside the vocabulary are skipped
   const float* bias_values;  // [M, bias_cap]
   const uint32_t* allowed;   // [M, W] or null (all)
-  int64_t* out_ids;          // [M]
+  int64_t* keys;             // [M, CTAs of a row]: the workspace
   float* out_logits;         // [M, V] or null
-  int V, W, bias_cap, record;
+  int V, W, bias_cap;
 };
 
 // 8 consecutive logits as loaded, and as fp32.
@@ -75,11 +80,13 @@ struct TrRaw<float> {
   }
 };
 
-// Bits v0 .. v0 + 7 of a set of `words` words (v0 >= -7); bits outside are 0.
-__device__ __forceinline__ uint32_t tr_bits8(const uint32_t* set, int words, int v0) {
+// Bits of group g, tokens v0 .. v0 + 7 (v0 >= -7), of a set of `words` words; bits
+// outside the row come from its edges and are not live.
+template <bool VEC>
+__device__ __forceinline__ uint32_t tr_bits8(const uint32_t* set, int words, int g, int v0) {
+  if (VEC) return reinterpret_cast<const unsigned char*>(set)[g];
   const int w = v0 >> 5, sh = v0 & 31;
-  const uint32_t lo = w >= 0 && w < words ? set[w] : 0u;
-  const uint32_t hi = sh > 24 && w + 1 < words ? set[w + 1] : 0u;
+  const uint32_t lo = set[max(w, 0)], hi = sh > 24 ? set[min(w + 1, words - 1)] : lo;
   return __funnelshift_r(lo, hi, sh) & 0xffu;
 }
 
@@ -87,123 +94,152 @@ __device__ __forceinline__ bool tr_better(float v, int i, float best, int besti)
   return v > best || (v == best && i < besti);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kTrMaxThreads, 2) constrained_argmax_kernel(TrParams p) {
-  extern __shared__ uint32_t tr_bias[];  // bit set of this CTA's biased tokens (bias lists only)
-  __shared__ float bv[kTrMaxThreads / 32], cv[kTrMaxCluster];
-  __shared__ int bi[kTrMaxThreads / 32], ci[kTrMaxCluster];
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA is running
+__device__ __forceinline__ float tr_penalise(float x, float rep, int n, float freq, float pres) {  // a seen token
+  x = x > 0.f ? x / rep : __fmul_rn(x, rep);
+  return n > 0 ? __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)n)), pres) : x;
+}
+__device__ __forceinline__ float tr_value(__nv_bfloat16 v) { return bf16_to_f(v); }
+__device__ __forceinline__ float tr_value(float v) { return v; }
+
+// VEC: the vocabulary is a multiple of 8.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrParams p) {
+  extern __shared__ uint32_t tr_bias[];  // bias lists only: 8 bits for each group of this CTA's tiles
+  __shared__ float bv[kTrThreads / 32];
+  __shared__ int bi[kTrThreads / 32];
   grid_dep_wait();
   grid_dep_launch();
-  const int row = blockIdx.y, c = blockIdx.x, ncta = gridDim.x, nt = blockDim.x;
+  constexpr int U = sizeof(T) == 2 ? 4 : 2;  // groups in flight per thread
+  constexpr int nt = kTrThreads, lg = 8;
+  const int row = blockIdx.y, c = blockIdx.x, ncta = gridDim.x;
   // Groups of 8 flattened indices; the row's first and last group may reach into
-  // its neighbours.  Group g of the row starts at token 8 g - a.
+  // its neighbours.  Group g of the row starts at token 8 g - a.  The CTAs take
+  // tiles of 256 groups in turn: frequent tokens have low ids, and
+  // with them the counts to read.
   const long long row0 = (long long)row * p.V;
-  const int a = (int)(row0 & 7), ngroups = (p.V + a + 7) / 8;
-  // The CTAs take tiles of nt groups (a power of two) in turn: frequent tokens have
-  // low ids, and with them the counts to read.
-  constexpr int kGroups = sizeof(T) == 2 ? 4 : 2;  // groups in flight per thread
-  const int lg = __ffs(nt) - 1, tiles = (ngroups + nt - 1) >> lg;
-  const T* logits = static_cast<const T*>(p.logits) + row0;
+  const int a = VEC ? 0 : (int)(row0 & 7), ngroups = (p.V + a + 7) / 8;
+  const int stride = ncta << lg;  // groups from one own tile to the next
+  const T* logits = static_cast<const T*>(p.logits) + row0 - a;
   const uint32_t* seen = p.seen ? p.seen + (size_t)row * p.W : nullptr;
   const uint32_t* allowed = p.allowed ? p.allowed + (size_t)row * p.W : nullptr;
-  const int* counts = p.counts + row0;
-  float* out = p.out_logits ? p.out_logits + row0 : nullptr;
-  const bool last_row = row == (int)gridDim.y - 1;
+  const int* counts = p.counts + row0 - a;
+  float* out = p.out_logits ? p.out_logits + row0 - a : nullptr;
   const int* bias_ids = p.bias_ids + (size_t)row * p.bias_cap;
-  // Biased tokens as bits of the CTA's own tiles, 8 a group.
-  unsigned char* bias_bits = reinterpret_cast<unsigned char*>(tr_bias);
+  const unsigned char* bias_bits = reinterpret_cast<const unsigned char*>(tr_bias) + threadIdx.x;
+  const int own = (ngroups + stride - 1) / stride;  // tiles, at most
+  int biased = threadIdx.x < p.bias_cap ? bias_ids[threadIdx.x] : -1;
+  const float rep = p.repetition ? p.repetition[row] : 1.f;
+  const float freq = p.frequency ? p.frequency[row] : 0.f;
+  const float pres = p.presence ? p.presence[row] : 0.f;
+
+  // A batch: U groups of this thread, one in each of U successive own tiles.
+  uint32_t ab[U], sb[U];  // allowed bits, allowed and seen bits
+  int n0[U];              // count of the group's first seen token
+  TrRaw<T> raw[U];
+  auto fetch_bits = [&](int gb) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int g = gb + u * stride, v0 = g * 8 - a;
+      ab[u] = sb[u] = 0u;
+      if (g >= ngroups) continue;
+      ab[u] = allowed ? tr_bits8<VEC>(allowed, p.W, g, v0) : 0xffu;
+      if (seen) sb[u] = tr_bits8<VEC>(seen, p.W, g, v0);
+      if (!VEC && v0 < 0) ab[u] &= 0xffu << -v0;
+      if (!VEC && v0 + 8 > p.V) ab[u] &= (1u << (p.V - v0)) - 1u;
+    }
+  };
+  auto fetch_values = [&](int gb) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int g = gb + u * stride;
+      sb[u] &= ab[u];
+      if (ab[u] == 0u) continue;
+      if (!VEC && row == (int)gridDim.y - 1 && g * 8 - a + 8 > p.V) raw[u].load(logits + g * 8, 0, p.V - (g * 8 - a));
+      else raw[u].load(logits + g * 8);  // (the array does not end inside the group)
+      if (sb[u]) n0[u] = counts[g * 8 + __ffs(sb[u]) - 1];
+    }
+  };
+  // The first loads are on their way while the biased tokens are marked: the CTAs
+  // run in several waves, and every wave would pay for one after the other.
+  int gb = (c << lg) + threadIdx.x;
+  fetch_bits(gb);
   if (p.bias_cap) {
-    for (int w = threadIdx.x; w < ((tiles + ncta - 1) / ncta << lg) / 4; w += nt) tr_bias[w] = 0u;
+    for (int w = threadIdx.x; w < own << lg >> 2; w += nt) tr_bias[w] = 0u;
     __syncthreads();
+  }
+  fetch_values(gb);
+  if (p.bias_cap) {
     for (int k = threadIdx.x; k < p.bias_cap; k += nt) {
-      const int v = bias_ids[k], g = (v + a) >> 3, tile = g >> lg;
+      const int v = biased, g = (v + a) >> 3, tile = g >> lg;
+      biased = k + nt < p.bias_cap ? bias_ids[k + nt] : -1;
       if (v < 0 || v >= p.V || tile % ncta != c) continue;
       const int at = (tile / ncta << lg) + (g & (nt - 1));
       atomicOr(&tr_bias[at >> 2], 1u << ((at & 3) * 8 + ((v + a) & 7)));
     }
     __syncthreads();
   }
-  const float rep = p.repetition ? p.repetition[row] : 1.f;
-  const float freq = p.frequency ? p.frequency[row] : 0.f;
-  const float pres = p.presence ? p.presence[row] : 0.f;
   float best = -INFINITY;
-  int besti = 0x7fffffff;
-  for (int tile = c; tile < tiles; tile += kGroups * ncta) {
-    uint32_t ab[kGroups], sb[kGroups];
-    int n0[kGroups];  // count of the group's first seen token
-    TrRaw<T> raw[kGroups];
+  int besti = 0x7fffffff, at = 0;  // at: where this thread's group of the batch's first tile has its bias bits
+#pragma unroll 1
+  for (; gb < ngroups; at += U << lg) {
 #pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-      const int g = ((tile + u * ncta) << lg) + threadIdx.x, v0 = g * 8 - a;
-      const uint32_t live = g >= ngroups ? 0u : (v0 < 0 ? 0xffu << -v0 & 0xffu : p.V - v0 >= 8 ? 0xffu : (1u << (p.V - v0)) - 1u);
-      ab[u] = live && allowed ? tr_bits8(allowed, p.W, v0) & live : live;
-      sb[u] = live && seen ? tr_bits8(seen, p.W, v0) : 0u;
-    }
-#pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-      const int v0 = (((tile + u * ncta) << lg) + (int)threadIdx.x) * 8 - a;
-      sb[u] &= ab[u];
-      if (ab[u] == 0u) continue;
-      if (sb[u]) n0[u] = counts[v0 + __ffs(sb[u]) - 1];
-      if (last_row && v0 + 8 > p.V) raw[u].load(logits + v0, max(-v0, 0), p.V - v0);  // the array ends inside the group
-      else raw[u].load(logits + v0);
-    }
-#pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-      const int lt = (tile + u * ncta) / ncta;  // tile = c + lt ncta
-      const int g = ((tile + u * ncta) << lg) + threadIdx.x, v0 = g * 8 - a;
+    for (int u = 0; u < U; ++u) {
+      const int g = gb + u * stride;
       if (g >= ngroups) break;
       float f[8];
-      if (ab[u]) {
-        raw[u].get(f);
-        // Few tokens are seen or biased: one at a time, not eight predicated divisions.
-        for (uint32_t m = sb[u]; m; m &= m - 1u) {
-          const int j = __ffs(m) - 1, n = m == sb[u] ? n0[u] : counts[v0 + j];
-          float x = 0.f;
+      raw[u].get(f);
+      // Few tokens are seen or biased: one at a time, not eight predicated divisions.
+#pragma unroll 1
+      for (uint32_t m = sb[u]; m; m &= m - 1u) {
+        const int j = __ffs(m) - 1, n = m == sb[u] ? n0[u] : counts[g * 8 + j];
+        float x = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e == j) x = f[e];
-          x = x > 0.f ? x / rep : __fmul_rn(x, rep);
-          if (n > 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)n)), pres);
+        for (int e = 0; e < 8; ++e)
+          if (e == j) x = f[e];
+        x = tr_penalise(x, rep, n, freq, pres);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e == j) f[e] = x;
-        }
-        for (uint32_t m = p.bias_cap ? bias_bits[(lt << lg) + threadIdx.x] & ab[u] : 0u; m; m &= m - 1u) {
-          const int j = __ffs(m) - 1;
-          float add = 0.f;  // the token's biases in list order
-          for (int k = 0; k < p.bias_cap; ++k)
-            if (bias_ids[k] == v0 + j) add = __fadd_rn(add, p.bias_values[(size_t)row * p.bias_cap + k]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e == j) f[e] = __fadd_rn(f[e], add);
-        }
+        for (int e = 0; e < 8; ++e)
+          if (e == j) f[e] = x;
       }
       if (ab[u] != 0xffu) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (!(ab[u] >> j & 1u)) f[j] = -INFINITY;
       }
-      // The group's maximum (NaN drops out); a thread meets its tokens in order, so
-      // a later equal one does not win.  -inf counts while there is nothing else.
-      const float top = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-      if (top > best || (besti == 0x7fffffff && ab[u])) {
-#pragma unroll
-        for (int j = 7; j >= 0; --j)
-          if (f[j] == top && (ab[u] >> j & 1u)) best = top, besti = v0 + j;
-      }
       if (out) {
-        if (v0 >= 0 && v0 + 8 <= p.V) {
-          *reinterpret_cast<float4*>(out + v0) = make_float4(f[0], f[1], f[2], f[3]);
-          *reinterpret_cast<float4*>(out + v0 + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        float* o = out + g * 8;
+        if (VEC || (g * 8 >= a && g * 8 - a + 8 <= p.V)) {
+          *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<float4*>(o + 4) = make_float4(f[4], f[5], f[6], f[7]);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (v0 + j >= 0 && v0 + j < p.V) out[v0 + j] = f[j];
+            if (g * 8 + j >= a && g * 8 - a + j < p.V) o[j] = f[j];
         }
       }
+      if (p.bias_cap) {  // biased tokens are left to the pick
+        const uint32_t bb = bias_bits[at + (u << lg)];
+        ab[u] &= ~bb;
+        if (bb) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (bb >> j & 1u) f[j] = -INFINITY;
+        }
+      }
+      // The group's maximum (NaN drops out); a thread meets its tokens in order, so
+      // a later equal one does not win.  -inf counts while there is nothing else.
+      const float top = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+      if (top > best || (besti == 0x7fffffff && top == -INFINITY)) {
+        best = top;
+#pragma unroll
+        for (int j = 7; j >= 0; --j)
+          if (f[j] == top && (ab[u] >> j & 1u)) besti = g * 8 - a + j;
+      }
     }
+    gb += U * stride;
+    if (gb >= ngroups) break;
+    fetch_bits(gb);
+    fetch_values(gb);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -213,38 +249,73 @@ __global__ void __launch_bounds__(kTrMaxThreads, 2) constrained_argmax_kernel(Tr
   }
   if ((threadIdx.x & 31) == 0) bv[threadIdx.x >> 5] = best, bi[threadIdx.x >> 5] = besti;
   __syncthreads();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA runs: its shared memory may be written
   if (threadIdx.x == 0) {
     for (int w = 1; w < nt / 32; ++w)
       if (tr_better(bv[w], bi[w], best, besti)) best = bv[w], besti = bi[w];
-    uint32_t rv, ri;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(rv) : "r"(smem_u32(&cv[c])));
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(ri) : "r"(smem_u32(&ci[c])));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(rv), "f"(best) : "memory");
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ri), "r"(besti) : "memory");
+    p.keys[(size_t)row * ncta + c] = besti != 0x7fffffff ? argmax_key(best, besti) : kTrNoKey;
   }
-  // Every CTA's winner is in place and every read of the row's state is done.
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (c != 0 || threadIdx.x != 0) return;
-  for (int w = 0; w < ncta; ++w)
-    if (w == 0 || tr_better(cv[w], ci[w], best, besti)) best = cv[w], besti = ci[w];
-  const bool found = besti != 0x7fffffff;
-  p.out_ids[row] = found ? besti : -1;
-  if (p.record && found) {  // atomics only so that nothing waits for the old value
-    atomicAdd(p.counts + row0 + besti, 1);
-    atomicOr(p.seen + (size_t)row * p.W + besti / 32, 1u << (besti & 31));
+}
+
+// The row's token, one warp per row: its CTAs' keys against its biased tokens, which
+// are worked out here, one lane each, at their first place in the list (once a row
+// instead of once a CTA: 60 biases on 128 rows cost 13 us there).  record: into the
+// row's state.
+template <typename T>
+__global__ void __launch_bounds__(32) constrained_pick_kernel(TrParams p, int ncta, int record, int64_t* out_ids) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int row = blockIdx.x, lane = threadIdx.x;
+  int64_t key = kTrNoKey;
+  for (int i = lane; i < ncta; i += 32)
+    key = max(key, (int64_t)__ldcg(reinterpret_cast<const long long*>(p.keys) + (size_t)row * ncta + i));
+  if (p.bias_cap) {
+    const int* ids = p.bias_ids + (size_t)row * p.bias_cap;
+    const float* values = p.bias_values + (size_t)row * p.bias_cap;
+    const float rep = p.repetition ? p.repetition[row] : 1.f;
+    const float freq = p.frequency ? p.frequency[row] : 0.f;
+    const float pres = p.presence ? p.presence[row] : 0.f;
+    for (int k = lane; k < p.bias_cap; k += 32) {
+      const int v = ids[k];
+      if (v < 0 || v >= p.V) continue;
+      const size_t word = (size_t)row * p.W + (v >> 5), at = (size_t)row * p.V + v;
+      const bool free = !p.allowed || (p.allowed[word] >> (v & 31) & 1u);
+      const bool was = p.seen && (p.seen[word] >> (v & 31) & 1u);
+      float x = tr_value(static_cast<const T*>(p.logits)[at]);
+      const int n = was ? p.counts[at] : 0;
+      bool first = true;
+      float add = 0.f;  // its biases in list order
+#pragma unroll 4
+      for (int q = 0; q < p.bias_cap; ++q)
+        if (ids[q] == v) {
+          first = first && q >= k;
+          add = __fadd_rn(add, values[q]);
+        }
+      if (!free || !first) continue;
+      if (was) x = tr_penalise(x, rep, n, freq, pres);
+      x = __fadd_rn(x, add);
+      if (p.out_logits) p.out_logits[at] = x;
+      if (x == x) key = max(key, argmax_key(x, v));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) key = max(key, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)key, o));
+  if (lane != 0) return;
+  const int64_t id = key == kTrNoKey ? -1 : argmax_key_id(key);
+  out_ids[row] = id;
+  if (record && id >= 0) {  // atomics only so that nothing waits for the old value
+    atomicAdd(p.counts + (size_t)row * p.V + id, 1);
+    atomicOr(p.seen + (size_t)row * p.W + id / 32, 1u << (id & 31));
   }
 }
 
 // Tokens of each sequence into its seen bits and, for an answer's tokens, its
 // counts.  Negative ids are padding; ids past the vocabulary are reported.
-constexpr int kTsThreads = 256;
-__global__ void __launch_bounds__(kTsThreads) token_stats_add_kernel(const int64_t* ids, int len, int V, int W,
+__global__ void __launch_bounds__(kTrThreads) token_stats_add_kernel(const int64_t* ids, int len, int V, int W,
                                                                      int* counts, uint32_t* seen, int* err) {
   grid_dep_wait();
   grid_dep_launch();
   const int row = blockIdx.y;
-  for (int i = blockIdx.x * kTsThreads + threadIdx.x; i < len; i += gridDim.x * kTsThreads) {
+  for (int i = blockIdx.x * kTrThreads + threadIdx.x; i < len; i += gridDim.x * kTrThreads) {
     const int64_t v = ids[(size_t)row * len + i];
     if (v < 0) continue;
     if (v >= V) {
@@ -261,45 +332,36 @@ __global__ void __launch_bounds__(kTsThreads) token_stats_add_kernel(const int64
 namespace lsb_host {
 using namespace lsb;
 
-template <typename T>
-static int launch_constrained_argmax(const TrParams& p, int64_t m, cudaStream_t stream) {
-  static bool configured[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    cudaError_t e =
-        cudaFuncSetAttribute(constrained_argmax_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return set_error(LS_ERR_CUDA, "constrained_argmax attribute: %s", cudaGetErrorString(e));
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
-  // Threads of a row: what the GPU holds at once (1024 an SM at 64 registers) over
-  // the rows, between 8 x 128 and 16 x 512.
-  const int64_t share = 1024 * (int64_t)sm_count() / m;
-  const int cluster = share >= 16 * 512 ? 16 : 8;
-  const int threads = share >= 8 * 512 ? 512 : share >= 8 * 256 ? 256 : 128;
+// CTAs of a row: a group per thread while that does not fill the GPU several times,
+// else four (those that a thread has in flight).
+static int64_t tr_ctas(int64_t m, int64_t vocab) {
+  const int64_t tiles = (vocab + 14) / 8 / kTrThreads + 1;
+  return m * tiles <= 8 * (int64_t)sm_count() ? tiles : (tiles + 3) / 4;
+}
+constexpr int64_t kTrMaxVocab = 1 << 20;
+
+template <typename T, bool VEC>
+static int launch_constrained_argmax(const TrParams& p, int64_t m, int record, int64_t* out_ids, cudaStream_t stream) {
+  const int64_t ncta = tr_ctas(m, p.V), tiles = ((int64_t)(p.V + 14) / 8 + kTrThreads - 1) / kTrThreads;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)cluster, (unsigned)m);
-  cfg.blockDim = dim3((unsigned)threads);
-  // One byte of bias bits per group of the CTA's tiles.
-  const int64_t tiles = ((int64_t)(p.V + 14) / 8 + threads - 1) / threads;
-  cfg.dynamicSmemBytes = p.bias_cap ? (size_t)((tiles + cluster - 1) / cluster * threads) : 0;
+  cfg.gridDim = dim3((unsigned)ncta, (unsigned)m);
+  cfg.blockDim = dim3(kTrThreads);
+  cfg.dynamicSmemBytes = p.bias_cap ? (size_t)((tiles + ncta - 1) / ncta * kTrThreads) : 0;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, constrained_argmax_kernel<T>, p);
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, constrained_argmax_kernel<T, VEC>, p);
+  if (e == cudaSuccess) {
+    cfg.gridDim = dim3((unsigned)m);
+    cfg.blockDim = dim3(32);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, constrained_pick_kernel<T>, p, (int)ncta, record, out_ids);
+  }
   return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "constrained_argmax launch: %s", cudaGetErrorString(e));
 }
-
-// Largest vocabulary: the bias bit set of one CTA (vocab / 8 / cluster bytes)
-// stays within the 48 KB of shared memory that need no opt-in.
-constexpr int64_t kTrMaxVocab = 1 << 21;
 
 }  // namespace lsb_host
 
@@ -307,14 +369,24 @@ using namespace lsb_host;
 
 extern "C" {
 
+int ls_constrained_argmax_workspace_bytes(int64_t m, int64_t vocab, int64_t* bytes) {
+  LS_REQUIRE(bytes && m > 0 && m <= 65535 && vocab > 0, LS_ERR_INVALID_ARGUMENT,
+             "ls_constrained_argmax_workspace_bytes: bad arguments");
+  LS_REQUIRE(vocab <= kTrMaxVocab, LS_ERR_UNSUPPORTED_SHAPE, "ls_constrained_argmax: vocab=%lld beyond %lld",
+             (long long)vocab, (long long)kTrMaxVocab);
+  *bytes = m * tr_ctas(m, vocab) * 8;
+  return LS_OK;
+}
+
 int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t vocab, int32_t* counts, uint32_t* seen,
                           const float* repetition, const float* frequency, const float* presence,
                           const int32_t* bias_ids, const float* bias_values, int64_t bias_cap, const uint32_t* allowed,
-                          int record, int64_t* out_ids, float* out_logits, ls_stream_t stream) {
+                          int record, int64_t* out_ids, float* out_logits, void* workspace,
+                          int64_t workspace_bytes, ls_stream_t stream) {
   LS_REQUIRE(logits && out_ids, LS_ERR_INVALID_ARGUMENT, "ls_constrained_argmax: null pointer");
-  LS_REQUIRE(m > 0 && m <= 65535 && vocab > 0, LS_ERR_INVALID_ARGUMENT, "ls_constrained_argmax: bad sizes");
-  LS_REQUIRE(vocab <= kTrMaxVocab, LS_ERR_UNSUPPORTED_SHAPE, "ls_constrained_argmax: vocab=%lld beyond %lld",
-             (long long)vocab, (long long)kTrMaxVocab);
+  int64_t need = 0;
+  int rc = ls_constrained_argmax_workspace_bytes(m, vocab, &need);
+  if (rc) return rc;
   LS_REQUIRE((counts == nullptr) == (seen == nullptr), LS_ERR_INVALID_ARGUMENT,
              "ls_constrained_argmax: counts and seen come together");
   LS_REQUIRE(counts || !(repetition || frequency || presence || record), LS_ERR_INVALID_ARGUMENT,
@@ -324,6 +396,8 @@ int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t
              LS_ERR_INVALID_ARGUMENT, "ls_constrained_argmax: bias_ids, bias_values and bias_cap come together");
   LS_REQUIRE(aligned16(logits) && aligned16(out_logits), LS_ERR_MISALIGNED,
              "ls_constrained_argmax: logits must be 16-byte aligned");
+  LS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, LS_ERR_WORKSPACE,
+             "ls_constrained_argmax: workspace needs %lld bytes, 8-byte aligned", (long long)need);
   TrParams p = {};
   p.logits = logits;
   p.counts = counts;
@@ -334,14 +408,17 @@ int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t
   p.bias_ids = bias_ids;
   p.bias_values = bias_values;
   p.allowed = allowed;
-  p.out_ids = out_ids;
+  p.keys = static_cast<int64_t*>(workspace);
   p.out_logits = out_logits;
   p.V = (int)vocab;
   p.W = (int)((vocab + 31) / 32);
   p.bias_cap = (int)bias_cap;
-  p.record = record ? 1 : 0;
-  return logits_f32 ? launch_constrained_argmax<float>(p, m, (cudaStream_t)stream)
-                    : launch_constrained_argmax<__nv_bfloat16>(p, m, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (vocab % 8 == 0)
+    return logits_f32 ? launch_constrained_argmax<float, true>(p, m, record ? 1 : 0, out_ids, st)
+                      : launch_constrained_argmax<__nv_bfloat16, true>(p, m, record ? 1 : 0, out_ids, st);
+  return logits_f32 ? launch_constrained_argmax<float, false>(p, m, record ? 1 : 0, out_ids, st)
+                    : launch_constrained_argmax<__nv_bfloat16, false>(p, m, record ? 1 : 0, out_ids, st);
 }
 
 int ls_token_stats_add(const int64_t* ids, int64_t batch, int64_t len, int64_t vocab, int32_t* counts, uint32_t* seen,
@@ -349,10 +426,10 @@ int ls_token_stats_add(const int64_t* ids, int64_t batch, int64_t len, int64_t v
   LS_REQUIRE(ids && seen, LS_ERR_INVALID_ARGUMENT, "ls_token_stats_add: null pointer");
   LS_REQUIRE(batch > 0 && batch <= 65535 && len > 0 && len < (1ll << 31) && vocab > 0 && vocab <= kTrMaxVocab,
              LS_ERR_INVALID_ARGUMENT, "ls_token_stats_add: bad sizes");
-  const int64_t blocks = (len + kTsThreads - 1) / kTsThreads;
+  const int64_t blocks = (len + kTrThreads - 1) / kTrThreads;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks < 64 ? blocks : 64), (unsigned)batch);
-  cfg.blockDim = dim3(kTsThreads);
+  cfg.blockDim = dim3(kTrThreads);
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

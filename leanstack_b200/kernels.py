@@ -717,12 +717,19 @@ def lora_delta(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch
     return out
 
 
+def constrained_argmax_workspace_bytes(m: int, vocab: int) -> int:
+    v = ctypes.c_int64(0)
+    nat.call("ls_constrained_argmax_workspace_bytes", m, vocab, ctypes.byref(v))
+    return v.value
+
+
 def constrained_argmax(logits: torch.Tensor, *, counts: torch.Tensor | None = None, seen: torch.Tensor | None = None,
                        repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
                        presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
                        bias_values: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
                        record: bool = False, out_ids: torch.Tensor | None = None,
-                       out_logits: torch.Tensor | None = None) -> torch.Tensor:
+                       out_logits: torch.Tensor | None = None,
+                       workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Greedy pick of each row of ``logits [m, vocab]`` (bf16 or fp32) under its rules -> int64 ``[m]``.
 
     Seen tokens are divided (positive logit) or multiplied by ``repetition``,
@@ -733,7 +740,8 @@ def constrained_argmax(logits: torch.Tensor, *, counts: torch.Tensor | None = No
     words ``[m, ceil(vocab / 32)]``, bit ``v % 32`` of word ``v // 32``.  Lowest
     id on ties, -1 where nothing is allowed.  ``record`` enters the pick into
     ``counts`` and ``seen``; ``out_logits`` fp32 ``[m, vocab]`` receives the
-    processed logits (-inf where not allowed).
+    processed logits (-inf where not allowed).  ``workspace`` needs no filling;
+    calls on one stream may share it.
     """
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (BF16, torch.float32):
         raise TypeError("logits must be a bf16 or fp32 tensor")
@@ -762,10 +770,14 @@ def constrained_argmax(logits: torch.Tensor, *, counts: torch.Tensor | None = No
         out_ids = torch.empty((m,), device=logits.device, dtype=torch.int64)
     else:
         _check_on(logits, out_ids, "out_ids", torch.int64, (m,))
+    if workspace is None:
+        workspace = torch.empty(constrained_argmax_workspace_bytes(m, vocab), device=logits.device, dtype=torch.uint8)
+    else:
+        _check_on(logits, workspace, "workspace", torch.uint8)
     _call_on(logits, "ls_constrained_argmax", logits.data_ptr(), int(logits.dtype == torch.float32), m, vocab,
              _ptr(counts), _ptr(seen), _ptr(repetition), _ptr(frequency), _ptr(presence),
              _ptr(bias_ids) if cap else None, _ptr(bias_values) if cap else None, cap, _ptr(allowed), int(record),
-             out_ids.data_ptr(), _ptr(out_logits))
+             out_ids.data_ptr(), _ptr(out_logits), workspace.data_ptr(), workspace.numel())
     return out_ids
 
 

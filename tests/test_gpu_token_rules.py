@@ -77,7 +77,7 @@ def _call(st, **kw):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("vocab", [1, 7, 31, 32, 33, 64, 1000, 4096, 32001, 151936])
-@pytest.mark.parametrize("m,allowed,biases", [(1, None, 0), (3, 0.9, 5), (5, 0.01, 40)])
+@pytest.mark.parametrize("m,allowed,biases", [(1, None, 0), (3, 0.9, 5), (5, 0.01, 40), (36, None, 2)])
 def test_processed_logits_and_pick(dtype, vocab, m, allowed, biases):
     st = _state(m, vocab, dtype, allowed, 50, biases)
     out = torch.full((m, vocab), float("nan"), device=DEV)
@@ -96,6 +96,16 @@ def test_processed_logits_and_pick(dtype, vocab, m, allowed, biases):
         i = int(ids[r])
         assert want[r, i].item() >= want[r].max().item() - 2 * bound[r].max().item()
     assert torch.equal(_call(st), ids)  # without the written logits
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,vocab", [(1, 1 << 20), (20, 1 << 20), (33, 700001), (300, 9999)])
+def test_large_vocabularies_and_many_rows(dtype, m, vocab):
+    st = _state(m, vocab, dtype, 0.5, 40, 3)
+    want, s = _rules(st)
+    ids = _call(st)
+    at = want.gather(1, ids[:, None])[:, 0]
+    assert (at >= want.amax(1) - 2 * 11 * 2 ** -24 * s.amax(1)).all()
 
 
 def test_plain_argmax_without_rules():
@@ -126,6 +136,16 @@ def test_infinities_and_nan():
         assert ids.tolist() == [2, -1, 1, 0, 0, 0]
     none = K.constrained_argmax(rows, allowed=torch.zeros(6, 1, device=DEV, dtype=torch.int32))
     assert none.tolist() == [-1] * 6
+
+
+def test_a_far_minus_infinity_behind_nan():
+    """Whole groups of NaN before the only candidates, which are -inf: the lowest of those is picked."""
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.full((3, 9000), float("nan"), device=DEV, dtype=dtype)
+        logits[0, 8500] = logits[0, 8999] = float("-inf")
+        logits[1, 17] = float("-inf")
+        logits[1, 4000] = -2.0
+        assert K.constrained_argmax(logits).tolist() == [8500, 4000, -1]
 
 
 def test_a_bias_of_minus_infinity_bans_and_plus_infinity_forces():

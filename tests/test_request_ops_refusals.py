@@ -55,12 +55,12 @@ def test_lora_delta(lib):
 
 
 def test_constrained_argmax(lib):
-    #       logits f32 m vocab counts seen rep freq pres bias_ids bias_vals cap allowed record out logits stream
-    args = [P, 0, 4, 151936, P, P, P, P, P, P, P, 3, P, 1, P, P, None]
+    #       logits f32 m vocab counts seen rep freq pres bias_ids bias_vals cap allowed record out logits ws bytes stream
+    args = [P, 0, 4, 151936, P, P, P, P, P, P, P, 3, P, 1, P, P, P, 1 << 40, None]
     fn = lib.ls_constrained_argmax
     for changes, code in (({0: None}, 1), ({14: None}, 1), ({2: 0}, 1), ({3: 0}, 1), ({4: None}, 1), ({5: None}, 1),
                           ({4: None, 5: None}, 1), ({9: None}, 1), ({11: 0}, 1), ({3: (1 << 21) + 1}, 2),
-                          ({0: P + 2}, 3), ({15: P + 4}, 3)):
+                          ({0: P + 2}, 3), ({15: P + 4}, 3), ({16: None}, 4), ({17: 8}, 4)):
         _refused(fn, args, changes, code)
     fn = lib.ls_token_stats_add
     args = [P, 4, 10, 1000, P, P, None]
