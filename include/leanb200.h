@@ -419,7 +419,8 @@ int ls_spec_accept(int64_t* ids, const int64_t* verdict, int64_t batch, int64_t 
  *                      position prefix_len + j of its sequence
  *   out                [m, Hq * D]
  * A cursor outside the cache raises LS_ERR_KV_OVERFLOW in the device error flag
- * and that row sees what is inside; a row that sees no key gives zeros. */
+ * and that row sees what is inside; a row that sees no key gives zeros.  The
+ * workspace needs no filling. */
 int ls_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t q_len, int64_t num_heads, int64_t num_kv_heads,
                                                int64_t head_dim, int64_t prefix_len, int64_t* bytes);
 int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
@@ -437,7 +438,7 @@ int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* 
  * LS_EPI_SPLIT_F32, so the kernel that adds the projection's partials adds the
  * adapter and both round once.  k, n and rank multiples of 8, rank <= 128.  An
  * id past the bank counts as none and raises LS_ERR_INVALID_ARGUMENT in the
- * device error flag.  The workspace is zero-filled once by the caller. */
+ * device error flag.  The workspace needs no filling. */
 int ls_lora_delta_workspace_bytes(int64_t batch, int64_t q_len, int64_t k, int64_t n, int64_t rank, int64_t* bytes);
 int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const void* a, const void* b,
                   const float* scaling, int64_t adapters, int64_t n, int64_t rank, const int32_t* adapter_ids,

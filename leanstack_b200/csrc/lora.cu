@@ -5,24 +5,47 @@
 // a sequence without an adapter (id < 0) get zeros.  The fp32 result has the
 // layout of one more split partial of the shared projection (LS_EPI_SPLIT_F32),
 // so the kernel that adds the partials adds the adapter too and the projection
-// plus its adapter round once.  u stays in fp32 (workspace).
+// plus its adapter round once.
 //
-// Shrink: one CTA per token, one warp per rank row.  Expand: one thread per
-// output.
-#include "common.cuh"
+// Two launches, both on mma.sync m16n8k16 (16 tokens x 8 ranks or outputs); the
+// operands go from global memory straight into the fragments, since both sides may
+// take k in any order as long as it is the same one: a lane's 16 (8) bytes of a
+// row are its k's of two (one) MMA steps.
+//   * Shrink, u over k splits: fp32 partials in the workspace, added in split order
+//     by whoever reads them.
+//   * Expand: u keeps its 24 bits as a sum of three bf16 (8 bits each), three
+//     products per step; the outputs of a lane are four neighbours, one 16-byte
+//     store a row.
+// Short sequences (decode, verify): the CTA of a sequence works for every sequence
+// with the same adapter if it is the first of them (within a window of 1024), so an
+// adapter is read once for all its tokens; long ones (prompts, q_len >= 16): a CTA
+// takes tokens of one sequence.
+// What bounds it: memory -- A and B of the adapters in use for short sequences
+// (where two dependent launches of a few MB are latency), x and the fp32 output for
+// prompts.  Tensor cores of the tcgen05 kind would wait: 2 r flops per byte of x.
+#include "mma_sync.cuh"
 
 namespace lsb {
 
+constexpr int kLoThreads = 128;
+constexpr int kLoWarps = 4;
+constexpr int kLoWindow = 1024;   // sequences among which equal adapters share a CTA
+constexpr int kLoPrompt = 16;     // q_len from which a CTA takes tokens of one sequence
+constexpr int kLoTile = 128;      // shrink: tokens of a prompt CTA (32 a warp)
+constexpr int kLoTileOut = 64;    // expand: tokens of a prompt CTA (16 a warp)
+
 struct LoraParams {
-  const __nv_bfloat16* x;        // [M, K]
-  const __nv_bfloat16* a;        // [adapters, R, K]
-  const __nv_bfloat16* b;        // [adapters, N, R]
-  const float* scaling;          // [adapters]
-  const int* ids;                // [batch]
-  float* u;                      // [M, R]
-  float* out;                    // [M, N]
+  const __nv_bfloat16* x;  // [M, K]
+  const __nv_bfloat16* a;  // [adapters, R, K]
+  const __nv_bfloat16* b;  // [adapters, N, R]
+  const float* scaling;    // [adapters]
+  const int* ids;          // [batch]
+  float* u;                // [splits, M, R]
+  float* out;              // [M, N]
   int* err;
-  int q_len, K, N, R, adapters, accumulate;
+  int M, batch, q_len, K, N, R, adapters, accumulate;
+  int splits, k_chunk;     // shrink: k split s is [s k_chunk, (s + 1) k_chunk)
+  int n_block;             // expand: outputs of a CTA
 };
 
 // The adapter of sequence b, -1 for none; an id past the bank counts as none and is reported.
@@ -35,42 +58,273 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int b) {
   return id < 0 ? -1 : id;
 }
 
-__global__ void __launch_bounds__(256) lora_shrink_kernel(LoraParams p) {
-  grid_dep_wait();
-  grid_dep_launch();
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int id = lora_adapter(p, t / p.q_len);
-  if (id < 0) return;
-  const __nv_bfloat16* xr = p.x + (size_t)t * p.K;
-  for (int r = warp; r < p.R; r += 8) {
-    const __nv_bfloat16* ar = p.a + ((size_t)id * p.R + r) * p.K;
-    float acc = 0.f;
-    for (int v = lane; v < p.K / 8; v += 32) acc = dot8(ldg16(ar + v * 8), ldg16(xr + v * 8), acc);
-    acc = warp_sum(acc);
-    if (lane == 0) p.u[(size_t)t * p.R + r] = acc;
+// Short sequences: the sequences that the CTA of sequence b works for, in order: those
+// of its adapter in its window if it is the first of them, else none.  Returns their
+// number; `members` holds their indices.
+__device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, int* members) {
+  __shared__ int s_count[kLoWarps], s_first;
+  const int w0 = b / kLoWindow * kLoWindow, w1 = min(w0 + kLoWindow, p.batch);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) s_first = 1;
+  __syncthreads();
+  int n = 0;
+  for (int i0 = w0; i0 < w1; i0 += kLoThreads) {
+    const int i = i0 + threadIdx.x;
+    const bool same = i < w1 && p.ids[i] == id;
+    if (same && i < b) s_first = 0;
+    const uint32_t vote = __ballot_sync(0xffffffffu, same && i >= b);
+    if (lane == 0) s_count[warp] = __popc(vote);
+    __syncthreads();
+    int at = n;
+    for (int w = 0; w < kLoWarps; ++w) {
+      if (w < warp) at += s_count[w];
+      n += s_count[w];
+    }
+    if (vote >> lane & 1u) members[at + __popc(vote & ((1u << lane) - 1u))] = i;
+    __syncthreads();
+  }
+  return s_first ? n : 0;
+}
+
+__device__ __forceinline__ uint32_t lo_part(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// acc += x a^T over k in [k0, k1) in steps of `step` (each of 32 k): MT tiles of 16
+// tokens (rows g8 and g8 + 8 at xr; null: zeros), NT tiles of 8 ranks.
+template <int MT, int NT>
+__device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2], const __nv_bfloat16* a, int K, int R, int k0,
+                                         int k1, int step, float (&acc)[MT][NT][4]) {
+  const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+#pragma unroll 2
+  for (int k = k0; k < k1; k += step) {
+    const int kk = k + t4 * 8;  // k1 is a multiple of 8: a lane's 8 are there or not
+    const bool in = kk < k1;
+    uint4 xv[MT][2], av[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xv[i][h] = in && xr[i][h] ? ldg16(xr[i][h] + kk) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      av[j] = in && j * 8 + g8 < R ? ldg16(a + (size_t)(j * 8 + g8) * K + kk) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint32_t fa[4] = {lo_part(xv[i][0], 2 * s), lo_part(xv[i][1], 2 * s), lo_part(xv[i][0], 2 * s + 1),
+                                lo_part(xv[i][1], 2 * s + 1)};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma_bf16(acc[i][j], fa, lo_part(av[j], 2 * s), lo_part(av[j], 2 * s + 1));
+      }
   }
 }
 
-__global__ void __launch_bounds__(256) lora_expand_kernel(LoraParams p) {
+// Short sequences: the four warps share the CTA's k range; their sums meet in shared memory.
+template <int NT>
+__global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
+  __shared__ int members[kLoWindow];
+  __shared__ float red[kLoWarps][16][NT * 8 + 1];
   grid_dep_wait();
   grid_dep_launch();
-  const int t = blockIdx.x, n = blockIdx.y * 256 + threadIdx.x;
-  const int id = lora_adapter(p, t / p.q_len);
-  if (n >= p.N) return;
-  float acc = 0.f;
-  if (id >= 0) {
-    const __nv_bfloat16* br = p.b + ((size_t)id * p.N + n) * p.R;
-    const float* ur = p.u + (size_t)t * p.R;
-    for (int r = 0; r < p.R; r += 8) {
-      float f[8];
-      unpack8(ldg16(br + r), f);
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
+  const int id = lora_adapter(p, b);
+  if (id < 0) return;
+  const int tokens = lora_group(p, b, id, members) * p.q_len;
+  const int k0 = blockIdx.x * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
+  auto token = [&](int i) { return members[i / p.q_len] * p.q_len + i % p.q_len; };
+  for (int i0 = 0; i0 < tokens; i0 += 16) {
+    const __nv_bfloat16* xr[1][2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc = fmaf(ur[r + j], f[j], acc);
+    for (int h = 0; h < 2; ++h)
+      xr[0][h] = i0 + g8 + 8 * h < tokens ? p.x + (size_t)token(i0 + g8 + 8 * h) * p.K : nullptr;
+    float acc[1][NT][4] = {};
+    lora_dot<1, NT>(xr, p.a + (size_t)id * p.R * p.K, p.K, p.R, k0 + warp * 32, k1, 32 * kLoWarps, acc);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[warp][g8 + 8 * (e >> 1)][j * 8 + 2 * t4 + (e & 1)] = acc[0][j][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * p.R; i += kLoThreads) {
+      const int t = i / p.R, r = i - t * p.R;
+      if (i0 + t < tokens)
+        p.u[((size_t)blockIdx.x * p.M + token(i0 + t)) * p.R + r] =
+            (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
     }
-    acc *= p.scaling[id];
+    __syncthreads();
   }
-  float* o = p.out + (size_t)t * p.N + n;
-  *o = p.accumulate ? *o + acc : acc;
+}
+
+// Prompts: a warp takes 32 tokens over the whole k range of the CTA.
+template <int NT>
+__global__ void __launch_bounds__(kLoThreads) lora_shrink_prompt_kernel(LoraParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
+  const int id = lora_adapter(p, b);
+  if (id < 0) return;
+  const int i0 = blockIdx.y * kLoTile + warp * 32;
+  const int k0 = blockIdx.x * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
+  const __nv_bfloat16* xr[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = i0 + i * 16 + h * 8 + g8;
+      xr[i][h] = t < p.q_len ? p.x + ((size_t)b * p.q_len + t) * p.K : nullptr;
+    }
+  float acc[2][NT][4] = {};
+  lora_dot<2, NT>(xr, p.a + (size_t)id * p.R * p.K, p.K, p.R, k0, k1, 32, acc);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = i0 + i * 16 + h * 8 + g8;
+      if (t >= p.q_len) continue;
+      float* u = p.u + ((size_t)blockIdx.x * p.M + (size_t)b * p.q_len + t) * p.R;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        if (j * 8 < p.R)
+          *reinterpret_cast<float2*>(u + j * 8 + 2 * t4) = make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+    }
+}
+
+// u of 16 tokens as fragments of KS steps, each value a sum of three bf16.
+template <int KS>
+struct LoraU {
+  uint32_t f[KS][3][4];
+  __device__ __forceinline__ void load(const LoraParams& p, const int (&tok)[2]) {  // rows g8, g8 + 8 (< 0: zeros)
+    const int t4 = threadIdx.x & 3;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int k = s * 16 + t4 * 4;
+        if (tok[h] >= 0 && k < p.R) {
+          const float* u = p.u + (size_t)tok[h] * p.R + k;
+#pragma unroll 4
+          for (int i = 0; i < p.splits; ++i) {
+            const float4 w = __ldcg(reinterpret_cast<const float4*>(u + (size_t)i * p.M * p.R));
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+          }
+        }
+        float r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          float c[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            c[e] = round_bf16(r[e]);
+            r[e] = fabsf(c[e]) < INFINITY ? r[e] - c[e] : 0.f;  // (infinity and NaN are whole in the first part)
+          }
+          f[s][q][h] = pack_bf16(c[0], c[1]);
+          f[s][q][2 + h] = pack_bf16(c[2], c[3]);
+        }
+      }
+  }
+};
+
+// Outputs [n0, n1) of 16 tokens, 16 at a time, `step` apart; a lane's four are
+// neighbours: column 2 t4 + e of product j is output 4 t4 + 2 j + e.
+template <int KS>
+__device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS>& u, int id, const int (&tok)[2], int n0,
+                                             int n1, int step) {
+  const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+  const __nv_bfloat16* b = p.b + (size_t)id * p.N * p.R;
+  const float scale = p.scaling[id];
+#pragma unroll 4
+  for (int n = n0; n < n1; n += step) {
+    uint2 bv[2][KS];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = n + (g8 >> 1) * 4 + j * 2 + (g8 & 1);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int k = s * 16 + t4 * 4;
+        bv[j][s] = row < n1 && k < p.R ? *reinterpret_cast<const uint2*>(b + (size_t)row * p.R + k) : make_uint2(0u, 0u);
+      }
+    }
+    float acc[2][4] = {};
+#pragma unroll
+    for (int q = 2; q >= 0; --q)  // the small parts first
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma_bf16(acc[j], u.f[s][q], bv[j][s].x, bv[j][s].y);
+    if (n + t4 * 4 < n1) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (tok[h] < 0) continue;
+        float4* o = reinterpret_cast<float4*>(p.out + (size_t)tok[h] * p.N + n + t4 * 4);
+        float4 v = make_float4(acc[0][2 * h] * scale, acc[0][2 * h + 1] * scale, acc[1][2 * h] * scale,
+                               acc[1][2 * h + 1] * scale);
+        if (p.accumulate) {
+          const float4 w = *o;
+          v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
+        }
+        *o = v;
+      }
+    }
+  }
+}
+
+// Zeros into outputs [n0, n1) of `count` tokens from token t0 on.
+__device__ __forceinline__ void lora_zeros(const LoraParams& p, int t0, int count, int n0, int n1) {
+  const int w = (n1 - n0) / 4;
+  for (int i = threadIdx.x; i < count * w; i += kLoThreads)
+    *reinterpret_cast<float4*>(p.out + (size_t)(t0 + i / w) * p.N + n0 + i % w * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+template <int KS>
+__global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
+  __shared__ int members[kLoWindow];
+  // The ids and the grouping are the caller's and the same as in the kernel before.
+  grid_dep_wait();
+  grid_dep_launch();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2;
+  const int n0 = blockIdx.x * p.n_block, n1 = min(n0 + p.n_block, p.N);
+  const int id = lora_adapter(p, b);
+  if (id < 0) {
+    if (!p.accumulate) lora_zeros(p, b * p.q_len, p.q_len, n0, n1);
+    return;
+  }
+  const int tokens = lora_group(p, b, id, members) * p.q_len;
+  for (int i0 = 0; i0 < tokens; i0 += 16) {
+    int tok[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = i0 + g8 + 8 * h;
+      tok[h] = i < tokens ? members[i / p.q_len] * p.q_len + i % p.q_len : -1;
+    }
+    LoraU<KS> u;
+    u.load(p, tok);
+    lora_outputs<KS>(p, u, id, tok, n0 + warp * 16, n1, 16 * kLoWarps);
+  }
+}
+
+template <int KS>
+__global__ void __launch_bounds__(kLoThreads) lora_expand_prompt_kernel(LoraParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2;
+  const int n0 = blockIdx.x * p.n_block, n1 = min(n0 + p.n_block, p.N);
+  const int t0 = blockIdx.y * kLoTileOut;
+  const int id = lora_adapter(p, b);
+  if (id < 0) {
+    if (!p.accumulate) lora_zeros(p, b * p.q_len + t0, min(kLoTileOut, p.q_len - t0), n0, n1);
+    return;
+  }
+  int tok[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = t0 + warp * 16 + h * 8 + g8;
+    tok[h] = t < p.q_len ? b * p.q_len + t : -1;
+  }
+  if (t0 + warp * 16 >= p.q_len) return;
+  LoraU<KS> u;
+  u.load(p, tok);
+  lora_outputs<KS>(p, u, id, tok, n0, n1, 16);
 }
 
 }  // namespace lsb
@@ -78,13 +332,25 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraParams p) {
 namespace lsb_host {
 using namespace lsb;
 
-static int64_t lora_workspace(int64_t batch, int64_t q_len, int64_t rank) { return batch * q_len * rank * 4; }
+// k splits: with the sequences (or token tiles), about two CTAs an SM; at least 128
+// k's a CTA (32 a warp), at most 16 partials to add.
+static int64_t lora_splits(int64_t batch, int64_t q_len, int64_t k) {
+  const int64_t groups = q_len >= kLoPrompt ? batch * ((q_len + kLoTile - 1) / kLoTile) : batch;
+  int64_t s = 2 * (int64_t)sm_count() / groups;
+  const int64_t most = (k + 127) / 128;
+  if (s > most) s = most;
+  if (s > 16) s = 16;
+  return s < 1 ? 1 : s;
+}
 
-template <typename Kernel>
-static cudaError_t launch_lora_kernel(Kernel kernel, dim3 grid, const LoraParams& p, cudaStream_t stream) {
+static int64_t lora_workspace(int64_t batch, int64_t q_len, int64_t k, int64_t rank) {
+  return lora_splits(batch, q_len, k) * batch * q_len * rank * 4;
+}
+
+static cudaError_t launch_lora_kernel(void (*kernel)(LoraParams), dim3 grid, const LoraParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(kLoThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -94,10 +360,43 @@ static cudaError_t launch_lora_kernel(Kernel kernel, dim3 grid, const LoraParams
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-static int launch_lora(const LoraParams& p, int64_t batch, cudaStream_t stream) {
-  const unsigned m = (unsigned)(batch * p.q_len);
-  cudaError_t e = launch_lora_kernel(lora_shrink_kernel, dim3(m), p, stream);
-  if (e == cudaSuccess) e = launch_lora_kernel(lora_expand_kernel, dim3(m, (unsigned)((p.N + 255) / 256)), p, stream);
+static int launch_lora(LoraParams p, cudaStream_t stream) {
+  const bool prompt = p.q_len >= kLoPrompt;
+  p.splits = (int)lora_splits(p.batch, p.q_len, p.K);
+  p.k_chunk = ((p.K + p.splits - 1) / p.splits + 31) / 32 * 32;
+  const int nt = (p.R + 7) / 8, ks = (p.R + 15) / 16;
+  void (*shrink)(LoraParams);
+  void (*expand)(LoraParams);
+  if (prompt) {
+    shrink = nt <= 1   ? lora_shrink_prompt_kernel<1>
+             : nt <= 2 ? lora_shrink_prompt_kernel<2>
+             : nt <= 4 ? lora_shrink_prompt_kernel<4>
+             : nt <= 8 ? lora_shrink_prompt_kernel<8>
+                       : lora_shrink_prompt_kernel<16>;
+    expand = ks <= 1   ? lora_expand_prompt_kernel<1>
+             : ks <= 2 ? lora_expand_prompt_kernel<2>
+             : ks <= 4 ? lora_expand_prompt_kernel<4>
+                       : lora_expand_prompt_kernel<8>;
+  } else {
+    shrink = nt <= 1   ? lora_shrink_kernel<1>
+             : nt <= 2 ? lora_shrink_kernel<2>
+             : nt <= 4 ? lora_shrink_kernel<4>
+             : nt <= 8 ? lora_shrink_kernel<8>
+                       : lora_shrink_kernel<16>;
+    expand = ks <= 1 ? lora_expand_kernel<1> : ks <= 2 ? lora_expand_kernel<2> : ks <= 4 ? lora_expand_kernel<4> : lora_expand_kernel<8>;
+  }
+  // Outputs of a CTA: 64 (16 a warp) for few sequences, more as the grid grows
+  // beyond about 1200 CTAs; prompts 256.
+  const int64_t blocks = (int64_t)((p.N + 63) / 64) * p.batch;
+  const int64_t per = (blocks + 1199) / 1200;
+  p.n_block = prompt ? 256 : 64 * (int)(per < 1 ? 1 : per > 16 ? 16 : per);
+  const unsigned nb = (unsigned)((p.N + p.n_block - 1) / p.n_block);
+  auto tiles = [&](int tile) { return (unsigned)((p.q_len + tile - 1) / tile); };
+  const dim3 gs = prompt ? dim3((unsigned)p.splits, tiles(kLoTile), (unsigned)p.batch)
+                         : dim3((unsigned)p.splits, (unsigned)p.batch);
+  const dim3 ge = prompt ? dim3(nb, tiles(kLoTileOut), (unsigned)p.batch) : dim3(nb, (unsigned)p.batch);
+  cudaError_t e = launch_lora_kernel(shrink, gs, p, stream);
+  if (e == cudaSuccess) e = launch_lora_kernel(expand, ge, p, stream);
   return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "lora_delta launch: %s", cudaGetErrorString(e));
 }
 
@@ -116,7 +415,9 @@ int ls_lora_delta_workspace_bytes(int64_t batch, int64_t q_len, int64_t k, int64
              "ls_lora_delta: k=%lld, n=%lld and rank=%lld must be multiples of 8", (long long)k, (long long)n,
              (long long)rank);
   LS_REQUIRE(rank <= 128, LS_ERR_UNSUPPORTED_SHAPE, "ls_lora_delta: rank=%lld beyond 128", (long long)rank);
-  *bytes = lora_workspace(batch, q_len, rank);
+  LS_REQUIRE(batch <= 65535 && (q_len + 63) / 64 <= 65535, LS_ERR_UNSUPPORTED_SHAPE,
+             "ls_lora_delta: %lld sequences of %lld tokens exceed the grid", (long long)batch, (long long)q_len);
+  *bytes = lora_workspace(batch, q_len, k, rank);
   return LS_OK;
 }
 
@@ -141,13 +442,15 @@ int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const 
   p.u = static_cast<float*>(workspace);
   p.out = out;
   p.err = device_error_ptr();
+  p.M = (int)(batch * q_len);
+  p.batch = (int)batch;
   p.q_len = (int)q_len;
   p.K = (int)k;
   p.N = (int)n;
   p.R = (int)rank;
   p.adapters = (int)adapters;
   p.accumulate = accumulate ? 1 : 0;
-  return launch_lora(p, batch, (cudaStream_t)stream);
+  return launch_lora(p, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -639,8 +639,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     values in their first ``prefix_len`` rows; ``k_cache`` / ``v_cache``
     ``[batch, Hkv, max_seq, D]`` each sequence's own.  Token i of sequence b
     sees the whole prefix, then its own keys 0 .. ``cache_pos[b] + i``.
-    ``workspace``: zero-filled once, ``shared_prefix_attention_workspace_bytes``
-    long; calls on one stream may share it.
+    ``workspace``: ``shared_prefix_attention_workspace_bytes`` long, needs no
+    filling; calls on one stream may share it.
     """
     _check(q, "q")
     if q.numel() != batch * q_len * num_heads * head_dim:
@@ -661,7 +661,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         _check_on(q, out, "out", BF16, (m, num_heads * head_dim))
     if workspace is None:
         need = shared_prefix_attention_workspace_bytes(batch, q_len, num_heads, num_kv_heads, head_dim, prefix_len)
-        workspace = torch.zeros(max(need, 256), device=q.device, dtype=torch.uint8)
+        workspace = torch.empty(max(need, 256), device=q.device, dtype=torch.uint8)
     else:
         _check_on(q, workspace, "workspace", torch.uint8)
     _call_on(q, "ls_shared_prefix_attention", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), int(prefix_len),
@@ -687,7 +687,7 @@ def lora_delta(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch
     no adapter, zeros).  ``out`` fp32 ``[batch * q_len, n]`` has the layout of one
     split partial of :func:`gemm_tc_splits`, so the partials' consumer adds it to
     the shared projection before the one rounding; ``accumulate`` adds to ``out``
-    instead.  ``workspace``: zero-filled once; calls on one stream may share it.
+    instead.  ``workspace`` needs no filling; calls on one stream may share it.
     """
     _check(x, "x")
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
@@ -707,7 +707,7 @@ def lora_delta(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch
     else:
         _check_on(x, out, "out", torch.float32, (m, n))
     if workspace is None:
-        workspace = torch.zeros(lora_delta_workspace_bytes(m // q_len, q_len, k, n, rank), device=x.device,
+        workspace = torch.empty(lora_delta_workspace_bytes(m // q_len, q_len, k, n, rank), device=x.device,
                                 dtype=torch.uint8)
     else:
         _check_on(x, workspace, "workspace", torch.uint8)

@@ -86,6 +86,15 @@ def test_many_sequences_of_one_token_and_many_adapters():
     _assert_close(out, x, a, b, s, ids, 1)
 
 
+def test_a_window_of_sequences_and_prompts_at_the_edges():
+    """Sequences beyond the window that shares CTAs; the shortest prompts; token tiles that end inside."""
+    for batch, q_len in ((1030, 1), (2100, 2), (3, 15), (3, 16), (2, 127), (2, 128), (1, 129), (5, 65)):
+        ids = [(i * 3) % 5 - 1 for i in range(batch)]
+        x, a, b, s = _inputs(batch * q_len, 256, 72, 24, 4)
+        out = K.lora_delta(x, a, b, s, torch.tensor(ids, device=DEV, dtype=torch.int32), q_len)
+        _assert_close(out, x, a, b, s, ids, q_len)
+
+
 def test_an_unused_adapter_and_a_token_without_one_may_hold_anything():
     x, a, b, s = _inputs(3, 256, 256, 16, 4)
     a[1], b[1], s[1] = float("nan"), float("inf"), float("nan")
