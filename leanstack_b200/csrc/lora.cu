@@ -11,8 +11,9 @@
 // operands go from global memory straight into the fragments, since both sides may
 // take k in any order as long as it is the same one: a lane's 16 (8) bytes of a
 // row are its k's of two (one) MMA steps.
-//   * Shrink, u over k splits: fp32 partials in the workspace, added in split order
-//     by whoever reads them.
+//   * Shrink, u over up to 8 k splits: a cluster of CTAs whose partials meet in shared
+//     memory and are added in split order (left to the expand kernel, every one of
+//     its CTAs added them again: 20 us of 30 at rank 64 and 16 splits).
 //   * Expand: u keeps its 24 bits as a sum of three bf16 (8 bits each), three
 //     products per step; the outputs of a lane are four neighbours, one 16-byte
 //     store a row.
@@ -32,6 +33,8 @@ constexpr int kLoWarps = 4;
 constexpr int kLoWindow = 1024;   // sequences among which equal adapters share a CTA
 constexpr int kLoPrompt = 16;     // q_len from which a CTA takes tokens of one sequence
 constexpr int kLoTile = 128;      // shrink: tokens of a prompt CTA (32 a warp)
+constexpr int kLoRanks = 16;      // shrink: ranks of a CTA, at most (16 x 5 tokens at rank 64: 13.6 us; all 64: 14.7)
+constexpr int kLoRanksPrompt = 32;
 constexpr int kLoTileOut = 64;    // expand: tokens of a prompt CTA (16 a warp)
 
 struct LoraParams {
@@ -40,7 +43,7 @@ struct LoraParams {
   const __nv_bfloat16* b;  // [adapters, N, R]
   const float* scaling;    // [adapters]
   const int* ids;          // [batch]
-  float* u;                // [splits, M, R]
+  float* u;                // [M, R]
   float* out;              // [M, N]
   int* err;
   int M, batch, q_len, K, N, R, adapters, accumulate;
@@ -86,17 +89,23 @@ __device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, in
   return s_first ? n : 0;
 }
 
+// The lines of `bytes` bytes into L2, while the previous kernel is still at work.
+__device__ __forceinline__ void lora_prefetch(const void* base, int bytes) {
+  for (int i = threadIdx.x * 128; i < bytes; i += kLoThreads * 128)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(base) + i));
+}
+
 __device__ __forceinline__ uint32_t lo_part(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
 // acc += x a^T over k in [k0, k1) in steps of `step` (each of 32 k): MT tiles of 16
-// tokens (rows g8 and g8 + 8 at xr; null: zeros), NT tiles of 8 ranks.
+// tokens (rows g8 and g8 + 8 at xr; null: zeros), NT tiles of 8 of the R ranks at a.
 template <int MT, int NT>
 __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2], const __nv_bfloat16* a, int K, int R, int k0,
                                          int k1, int step, float (&acc)[MT][NT][4]) {
   const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-#pragma unroll 2
+#pragma unroll (MT * 2 + NT <= 4 ? 4 : 2)
   for (int k = k0; k < k1; k += step) {
     const int kk = k + t4 * 8;  // k1 is a multiple of 8: a lane's 8 are there or not
     const bool in = kk < k1;
@@ -120,11 +129,41 @@ __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2]
   }
 }
 
+// Elements [0, n) of the cluster's CTAs' partials, added in split order; CTA c of
+// them takes every ncta-th run of kLoThreads elements and hands its sums to store(i, v).
+template <typename Store>
+__device__ __forceinline__ void lora_join_splits(const float* part, int n, Store store) {
+  const int c = blockIdx.x, ncta = gridDim.x;  // the cluster is the grid's x extent
+  if (ncta > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+  for (int i = c * kLoThreads + threadIdx.x; i < n; i += ncta * kLoThreads) {
+    float v = 0.f;
+    if (ncta == 1) {
+      v = part[i];
+    } else {
+      float w[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part + i)), "r"(q < ncta ? q : 0));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w[q]) : "r"(at) : "memory");
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < ncta) v += w[q];
+    }
+    store(i, v);
+  }
+  // The partials are read by others: they stay until all are done.
+  if (ncta > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+}
+
 // Short sequences: the four warps share the CTA's k range; their sums meet in shared memory.
 template <int NT>
 __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
   __shared__ int members[kLoWindow];
-  __shared__ float red[kLoWarps][16][NT * 8 + 1];
+  __shared__ float red[kLoWarps][16][NT * 8 + 1], part[16 * NT * 8];
   grid_dep_wait();
   grid_dep_launch();
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
@@ -132,6 +171,7 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
   if (id < 0) return;
   const int tokens = lora_group(p, b, id, members) * p.q_len;
   const int k0 = blockIdx.x * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
+  const int r0 = blockIdx.z * kLoRanks, ranks = min(kLoRanks, p.R - r0);
   auto token = [&](int i) { return members[i / p.q_len] * p.q_len + i % p.q_len; };
   for (int i0 = 0; i0 < tokens; i0 += 16) {
     const __nv_bfloat16* xr[1][2];
@@ -139,31 +179,34 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
     for (int h = 0; h < 2; ++h)
       xr[0][h] = i0 + g8 + 8 * h < tokens ? p.x + (size_t)token(i0 + g8 + 8 * h) * p.K : nullptr;
     float acc[1][NT][4] = {};
-    lora_dot<1, NT>(xr, p.a + (size_t)id * p.R * p.K, p.K, p.R, k0 + warp * 32, k1, 32 * kLoWarps, acc);
+    lora_dot<1, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0 + warp * 32, k1, 32 * kLoWarps, acc);
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) red[warp][g8 + 8 * (e >> 1)][j * 8 + 2 * t4 + (e & 1)] = acc[0][j][e];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * p.R; i += kLoThreads) {
-      const int t = i / p.R, r = i - t * p.R;
-      if (i0 + t < tokens)
-        p.u[((size_t)blockIdx.x * p.M + token(i0 + t)) * p.R + r] =
-            (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
+    for (int i = threadIdx.x; i < 16 * NT * 8; i += kLoThreads) {
+      const int t = i / (NT * 8), r = i % (NT * 8);
+      part[i] = (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
     }
-    __syncthreads();
+    lora_join_splits(part, 16 * NT * 8, [&](int i, float v) {
+      const int t = i / (NT * 8), r = i % (NT * 8);
+      if (i0 + t < tokens && r < ranks) p.u[(size_t)token(i0 + t) * p.R + r0 + r] = v;
+    });
   }
 }
 
 // Prompts: a warp takes 32 tokens over the whole k range of the CTA.
 template <int NT>
 __global__ void __launch_bounds__(kLoThreads) lora_shrink_prompt_kernel(LoraParams p) {
+  __shared__ __align__(16) float part[kLoTile * NT * 8];
   grid_dep_wait();
   grid_dep_launch();
   const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
   const int id = lora_adapter(p, b);
   if (id < 0) return;
-  const int i0 = blockIdx.y * kLoTile + warp * 32;
+  const int groups = (p.R + kLoRanksPrompt - 1) / kLoRanksPrompt, t0 = blockIdx.y / groups * kLoTile, i0 = t0 + warp * 32;
+  const int r0 = blockIdx.y % groups * kLoRanksPrompt, ranks = min(kLoRanksPrompt, p.R - r0);
   const int k0 = blockIdx.x * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
   const __nv_bfloat16* xr[2][2];
 #pragma unroll
@@ -174,19 +217,19 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_prompt_kernel(LoraPara
       xr[i][h] = t < p.q_len ? p.x + ((size_t)b * p.q_len + t) * p.K : nullptr;
     }
   float acc[2][NT][4] = {};
-  lora_dot<2, NT>(xr, p.a + (size_t)id * p.R * p.K, p.K, p.R, k0, k1, 32, acc);
+  lora_dot<2, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0, k1, 32, acc);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = i0 + i * 16 + h * 8 + g8;
-      if (t >= p.q_len) continue;
-      float* u = p.u + ((size_t)blockIdx.x * p.M + (size_t)b * p.q_len + t) * p.R;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        if (j * 8 < p.R)
-          *reinterpret_cast<float2*>(u + j * 8 + 2 * t4) = make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
-    }
+        *reinterpret_cast<float2*>(part + (warp * 32 + i * 16 + h * 8 + g8) * (NT * 8) + j * 8 + 2 * t4) =
+            make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+  lora_join_splits(part, kLoTile * NT * 8, [&](int i, float v) {
+    const int t = t0 + i / (NT * 8), r = i % (NT * 8);
+    if (t < p.q_len && r < ranks) p.u[((size_t)b * p.q_len + t) * p.R + r0 + r] = v;
+  });
 }
 
 // u of 16 tokens as fragments of KS steps, each value a sum of three bf16.
@@ -202,12 +245,7 @@ struct LoraU {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         const int k = s * 16 + t4 * 4;
         if (tok[h] >= 0 && k < p.R) {
-          const float* u = p.u + (size_t)tok[h] * p.R + k;
-#pragma unroll 4
-          for (int i = 0; i < p.splits; ++i) {
-            const float4 w = __ldcg(reinterpret_cast<const float4*>(u + (size_t)i * p.M * p.R));
-            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-          }
+          v = __ldcg(reinterpret_cast<const float4*>(p.u + (size_t)tok[h] * p.R + k));
         }
         float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -242,7 +280,7 @@ __device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int k = s * 16 + t4 * 4;
-        bv[j][s] = row < n1 && k < p.R ? *reinterpret_cast<const uint2*>(b + (size_t)row * p.R + k) : make_uint2(0u, 0u);
+        bv[j][s] = row < n1 && k < p.R ? __ldg(reinterpret_cast<const uint2*>(b + (size_t)row * p.R + k)) : make_uint2(0u, 0u);
       }
     }
     float acc[2][4] = {};
@@ -279,17 +317,20 @@ __device__ __forceinline__ void lora_zeros(const LoraParams& p, int t0, int coun
 template <int KS>
 __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
   __shared__ int members[kLoWindow];
-  // The ids and the grouping are the caller's and the same as in the kernel before.
-  grid_dep_wait();
+  // The shrink kernel's CTAs let this one start only after every kernel before them
+  // is complete: ids, b and out may be used at once, u after the wait.
   grid_dep_launch();
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2;
   const int n0 = blockIdx.x * p.n_block, n1 = min(n0 + p.n_block, p.N);
   const int id = lora_adapter(p, b);
   if (id < 0) {
     if (!p.accumulate) lora_zeros(p, b * p.q_len, p.q_len, n0, n1);
+    grid_dep_wait();
     return;
   }
   const int tokens = lora_group(p, b, id, members) * p.q_len;
+  if (tokens > 0) lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
+  grid_dep_wait();
   for (int i0 = 0; i0 < tokens; i0 += 16) {
     int tok[2];
 #pragma unroll
@@ -305,7 +346,6 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
 
 template <int KS>
 __global__ void __launch_bounds__(kLoThreads) lora_expand_prompt_kernel(LoraParams p) {
-  grid_dep_wait();
   grid_dep_launch();
   const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2;
   const int n0 = blockIdx.x * p.n_block, n1 = min(n0 + p.n_block, p.N);
@@ -313,8 +353,11 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_prompt_kernel(LoraPara
   const int id = lora_adapter(p, b);
   if (id < 0) {
     if (!p.accumulate) lora_zeros(p, b * p.q_len + t0, min(kLoTileOut, p.q_len - t0), n0, n1);
+    grid_dep_wait();
     return;
   }
+  lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
+  grid_dep_wait();
   int tok[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -333,30 +376,36 @@ namespace lsb_host {
 using namespace lsb;
 
 // k splits: with the sequences (or token tiles), about two CTAs an SM; at least 128
-// k's a CTA (32 a warp), at most 16 partials to add.
+// k's a CTA (32 a warp), at most a cluster of 8.
 static int64_t lora_splits(int64_t batch, int64_t q_len, int64_t k) {
   const int64_t groups = q_len >= kLoPrompt ? batch * ((q_len + kLoTile - 1) / kLoTile) : batch;
   int64_t s = 2 * (int64_t)sm_count() / groups;
   const int64_t most = (k + 127) / 128;
   if (s > most) s = most;
-  if (s > 16) s = 16;
+  if (s > 8) s = 8;
   return s < 1 ? 1 : s;
 }
 
 static int64_t lora_workspace(int64_t batch, int64_t q_len, int64_t k, int64_t rank) {
-  return lora_splits(batch, q_len, k) * batch * q_len * rank * 4;
+  (void)k;
+  return batch * q_len * rank * 4;
 }
 
-static cudaError_t launch_lora_kernel(void (*kernel)(LoraParams), dim3 grid, const LoraParams& p, cudaStream_t stream) {
+static cudaError_t launch_lora_kernel(void (*kernel)(LoraParams), dim3 grid, unsigned cluster, const LoraParams& p,
+                                      cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kLoThreads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -364,39 +413,36 @@ static int launch_lora(LoraParams p, cudaStream_t stream) {
   const bool prompt = p.q_len >= kLoPrompt;
   p.splits = (int)lora_splits(p.batch, p.q_len, p.K);
   p.k_chunk = ((p.K + p.splits - 1) / p.splits + 31) / 32 * 32;
-  const int nt = (p.R + 7) / 8, ks = (p.R + 15) / 16;
+  const int most = prompt ? kLoRanksPrompt : kLoRanks;  // ranks of a shrink CTA
+  const int nt = (p.R < most ? p.R : most) / 8, ks = (p.R + 15) / 16;
+  const unsigned groups = (unsigned)((p.R + most - 1) / most);
   void (*shrink)(LoraParams);
   void (*expand)(LoraParams);
   if (prompt) {
-    shrink = nt <= 1   ? lora_shrink_prompt_kernel<1>
-             : nt <= 2 ? lora_shrink_prompt_kernel<2>
-             : nt <= 4 ? lora_shrink_prompt_kernel<4>
-             : nt <= 8 ? lora_shrink_prompt_kernel<8>
-                       : lora_shrink_prompt_kernel<16>;
+    shrink = nt <= 1 ? lora_shrink_prompt_kernel<1> : nt <= 2 ? lora_shrink_prompt_kernel<2> : lora_shrink_prompt_kernel<4>;
     expand = ks <= 1   ? lora_expand_prompt_kernel<1>
              : ks <= 2 ? lora_expand_prompt_kernel<2>
              : ks <= 4 ? lora_expand_prompt_kernel<4>
                        : lora_expand_prompt_kernel<8>;
   } else {
-    shrink = nt <= 1   ? lora_shrink_kernel<1>
-             : nt <= 2 ? lora_shrink_kernel<2>
-             : nt <= 4 ? lora_shrink_kernel<4>
-             : nt <= 8 ? lora_shrink_kernel<8>
-                       : lora_shrink_kernel<16>;
-    expand = ks <= 1 ? lora_expand_kernel<1> : ks <= 2 ? lora_expand_kernel<2> : ks <= 4 ? lora_expand_kernel<4> : lora_expand_kernel<8>;
+    shrink = nt <= 1 ? lora_shrink_kernel<1> : lora_shrink_kernel<2>;
+    expand = ks <= 1   ? lora_expand_kernel<1>
+             : ks <= 2 ? lora_expand_kernel<2>
+             : ks <= 4 ? lora_expand_kernel<4>
+                       : lora_expand_kernel<8>;
   }
   // Outputs of a CTA: 64 (16 a warp) for few sequences, more as the grid grows
-  // beyond about 1200 CTAs; prompts 256.
+  // beyond about 1200 CTAs; prompts 128 (64 / 256 / 512 were 4 / 7 / 20% slower).
   const int64_t blocks = (int64_t)((p.N + 63) / 64) * p.batch;
   const int64_t per = (blocks + 1199) / 1200;
-  p.n_block = prompt ? 256 : 64 * (int)(per < 1 ? 1 : per > 16 ? 16 : per);
+  p.n_block = prompt ? 128 : 64 * (int)(per < 1 ? 1 : per > 16 ? 16 : per);
   const unsigned nb = (unsigned)((p.N + p.n_block - 1) / p.n_block);
   auto tiles = [&](int tile) { return (unsigned)((p.q_len + tile - 1) / tile); };
-  const dim3 gs = prompt ? dim3((unsigned)p.splits, tiles(kLoTile), (unsigned)p.batch)
-                         : dim3((unsigned)p.splits, (unsigned)p.batch);
+  const dim3 gs = prompt ? dim3((unsigned)p.splits, tiles(kLoTile) * groups, (unsigned)p.batch)
+                         : dim3((unsigned)p.splits, (unsigned)p.batch, groups);
   const dim3 ge = prompt ? dim3(nb, tiles(kLoTileOut), (unsigned)p.batch) : dim3(nb, (unsigned)p.batch);
-  cudaError_t e = launch_lora_kernel(shrink, gs, p, stream);
-  if (e == cudaSuccess) e = launch_lora_kernel(expand, ge, p, stream);
+  cudaError_t e = launch_lora_kernel(shrink, gs, (unsigned)p.splits, p, stream);
+  if (e == cudaSuccess) e = launch_lora_kernel(expand, ge, 1, p, stream);
   return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "lora_delta launch: %s", cudaGetErrorString(e));
 }
 
@@ -415,7 +461,7 @@ int ls_lora_delta_workspace_bytes(int64_t batch, int64_t q_len, int64_t k, int64
              "ls_lora_delta: k=%lld, n=%lld and rank=%lld must be multiples of 8", (long long)k, (long long)n,
              (long long)rank);
   LS_REQUIRE(rank <= 128, LS_ERR_UNSUPPORTED_SHAPE, "ls_lora_delta: rank=%lld beyond 128", (long long)rank);
-  LS_REQUIRE(batch <= 65535 && (q_len + 63) / 64 <= 65535, LS_ERR_UNSUPPORTED_SHAPE,
+  LS_REQUIRE(batch <= 65535 && (q_len + 63) / 64 * 2 <= 65535, LS_ERR_UNSUPPORTED_SHAPE,
              "ls_lora_delta: %lld sequences of %lld tokens exceed the grid", (long long)batch, (long long)q_len);
   *bytes = lora_workspace(batch, q_len, k, rank);
   return LS_OK;
