@@ -17,6 +17,12 @@ Tensor parallelism (``tp`` given, world > 1): the runtime is this rank's shard
 one NCCL all-reduce sums before the residual-add kernel; the head reduces its
 vocab shard to int64 argmax keys and a MAX all-reduce picks the token.  The
 collectives are captured into the step's CUDA graph with the kernels.
+
+A batch of different requests (one GPU; ``requests.py``): ``prefix_capacity``
+makes room for a prompt prefix that all sequences share, held once
+(``prefill_prefix``); ``adapters`` is a bank of low-rank adapters, of which each
+sequence uses one or none (``set_adapters``); ``rules`` constrains each
+sequence's greedy pick.
 """
 
 from __future__ import annotations
@@ -26,6 +32,7 @@ import torch
 from . import kernels as K
 from .leanserve import allocate_arenas, build_resident_buffer_plan, runtime_weight_bytes
 from .qwen_explicit import QwenSemanticStackRuntime, build_qwen_position_cache
+from .requests import AdapterBank, SharedPrefix, TokenRules
 from .tp import TPComm, TPShard
 
 SMALL_M = 8      # largest token count of the CUDA-core linear kernels
@@ -56,12 +63,25 @@ class DecodeEngine:
     def __init__(self, runtime: QwenSemanticStackRuntime, batch_size: int, max_seq_len: int,
                  max_tokens_per_step: int | None = None, use_graph: bool = True, linear_backend: str = "auto",
                  tp: TPComm | None = None, shard: TPShard | None = None,
-                 tc_tiles: list[dict] | None = None):
+                 tc_tiles: list[dict] | None = None, prefix_capacity: int = 0, adapters: AdapterBank | None = None,
+                 rules: TokenRules | None = None):
         if runtime.final_norm_weight is None or runtime.lm_head_weight is None:
             raise ValueError("the engine needs the output head (include_output_head=True)")
         self.tp = tp if (tp is not None and tp.world > 1) else None
         if self.tp is not None and shard is None:
             raise ValueError("a tensor-parallel engine needs its TPShard")
+        if self.tp is not None and (prefix_capacity or adapters is not None or rules is not None):
+            raise ValueError("a shared prefix, adapters and token rules run on one GPU")
+        if adapters is not None:
+            if linear_backend == "cuda_core":
+                raise ValueError("adapters ride on the split partials of the tc linears")
+            if adapters.shapes["qkv"] != (runtime.config.hidden_size, runtime.config.qkv_dim) or \
+                    len(adapters.layers) != len(runtime.layers):
+                raise ValueError("the adapter bank is of another geometry")
+            linear_backend = "tc"
+        if rules is not None and (rules.batch, rules.vocab) != (batch_size, runtime.lm_head_weight.shape[0]):
+            raise ValueError(f"token rules for {rules.batch} rows of {rules.vocab} tokens, the engine has "
+                             f"{batch_size} of {runtime.lm_head_weight.shape[0]}")
         self.vocab_offset = shard.vocab_offset if self.tp is not None else 0
         self.vocab_rows = runtime.lm_head_weight.shape[0]
         self.backend = resolve_backend(linear_backend, batch_size, self.tp is not None)
@@ -80,9 +100,12 @@ class DecodeEngine:
         self.arenas = allocate_arenas(self.plan, g, runtime.device, runtime.dtype)
         self.kv = self.arenas.kv
         self.S = self.kv.layout.max_seq_len
-        self.cos, self.sin = build_qwen_position_cache(runtime.rope_inv_freq, runtime.attention_scaling, self.S,
-                                                       runtime.dtype)
+        self.cos, self.sin = build_qwen_position_cache(runtime.rope_inv_freq, runtime.attention_scaling,
+                                                       self.S + prefix_capacity, runtime.dtype)
         dev = runtime.device
+        self.prefix = SharedPrefix(g, prefix_capacity, dev, runtime.dtype) if prefix_capacity else None
+        self.prefix_epoch = 0  # moves when the prefix changes: steps captured before are stale
+        self.adapters, self.rules = adapters, rules
         ws = max(K.attention_workspace_bytes(batch_size, q, g.num_attention_heads, g.num_key_value_heads, g.head_dim,
                                              self.S) for q in range(1, self.T // batch_size + 1))
         self.attn_ws = torch.zeros(max(ws, 256), device=dev, dtype=torch.uint8)
@@ -117,10 +140,21 @@ class DecodeEngine:
                 shapes_.append((g.hidden_size, rt0.mlp.gate_up_proj_weight.shape[0]))
             part = max(K.gemm_splits(mm, k_, n_) * mm * n_
                        for mm in range(batch_size, T + 1, batch_size) for k_, n_ in shapes_)
+            if adapters is not None:  # the adapters' delta is one more partial of each linear
+                if not self.gu_plain and "gate_up" in adapters.targets:
+                    raise ValueError("gate_up adapters need an intermediate size that is a multiple of 128")
+                part = max((K.gemm_splits(mm, k_, n_) + 1) * mm * n_
+                           for mm in range(batch_size, T + 1, batch_size) for k_, n_ in shapes_)
+                self.adapter_ids = torch.full((batch_size,), -1, device=dev, dtype=torch.int32)
+                self.lora_ws = torch.empty(max(K.lora_delta_workspace_bytes(batch_size, q, k_, n_, adapters.rank)
+                                               for q in range(1, T // batch_size + 1) for k_, n_ in shapes_),
+                                           device=dev, dtype=torch.uint8)
             self.tc_part = torch.zeros(part, device=dev, dtype=torch.float32)
         else:
             self.lm_ws = torch.zeros(K.lmhead_workspace_bytes(self.T, self.vocab_rows), device=dev,
                                      dtype=torch.uint8)
+            if rules is not None:  # the rules work on logits, which the fused head does not keep
+                self.logits = torch.zeros(batch_size, self.vocab_rows, device=dev, dtype=runtime.dtype)
         if self.tp is not None:
             self.part = torch.zeros(self.T, g.hidden_size, device=dev, dtype=torch.float32)
             self.keys = torch.zeros(self.T, device=dev, dtype=torch.int64)
@@ -139,6 +173,82 @@ class DecodeEngine:
         self.graph: torch.cuda.CUDAGraph | None = None
 
     # ------------------------------------------------------------------
+    # a batch of different requests
+    # ------------------------------------------------------------------
+    @property
+    def prefix_len(self) -> int:
+        return 0 if self.prefix is None else self.prefix.length
+
+    def set_adapters(self, ids) -> None:
+        """The adapter of each sequence (-1: none) from the next step on; a captured step follows."""
+        if self.adapters is None:
+            raise ValueError("the engine has no adapter bank")
+        ids = [int(i) for i in ids]
+        if len(ids) != self.B or any(i >= self.adapters.adapters for i in ids):
+            raise ValueError(f"expected {self.B} adapter ids below {self.adapters.adapters}, got {ids}")
+        self.adapter_ids.copy_(torch.tensor(ids, dtype=torch.int32))
+
+    def prefill_prefix(self, prompt_ids: torch.Tensor, adapter: int = -1) -> None:
+        """Run ``prompt_ids [P]`` once and keep its keys and values as the prefix of every sequence.
+
+        The sequences' own tokens follow at positions P, P + 1, ...; their
+        caches must be empty.  ``adapter``: the adapter that the prefix is
+        computed with; a sequence that uses another one attends to the prefix as
+        this one left it.
+        """
+        if self.prefix is None:
+            raise ValueError("the engine has no room for a prefix (prefix_capacity)")
+        if prompt_ids.dim() != 1 or not 1 <= prompt_ids.shape[0] <= self.prefix.capacity:
+            raise ValueError(f"prefix must be [P] with 1 <= P <= {self.prefix.capacity}")
+        if any(self.kv.sequence_lens):
+            raise ValueError("the sequences already hold tokens: reset() first")
+        if adapter >= 0 and (self.adapters is None or adapter >= self.adapters.adapters):
+            raise ValueError(f"no adapter {adapter}")
+        ids = prompt_ids.to(self.rt.device, torch.int64).contiguous()
+        P = ids.shape[0]
+        adapter_ids = None
+        if self.adapters is not None:
+            adapter_ids = torch.full((1,), adapter, device=self.rt.device, dtype=torch.int32)
+        self.prefix.length = 0
+        self._prompt_pass(ids, 1, P, [k[None] for k in self.prefix.key], [v[None] for v in self.prefix.value],
+                          self.prefix.capacity, None, adapter_ids)
+        self.prefix.length = P
+        # Captured steps hold the old length and workspace.
+        self.graph = None
+        self.verify_graphs.clear()
+        self.prefix_epoch += 1
+        g = self.g
+        need = max(K.shared_prefix_attention_workspace_bytes(self.B, q, g.num_attention_heads, g.num_key_value_heads,
+                                                             g.head_dim, P) for q in range(1, self.T // self.B + 1))
+        if need > self.attn_ws.numel():
+            self.attn_ws = torch.zeros(need, device=self.rt.device, dtype=torch.uint8)
+        if self.rules is not None:
+            self.rules.note_prompt(ids.expand(self.B, P).contiguous())
+
+    def _lora(self, li: int, target: str, x: torch.Tensor, splits: int, q_len: int) -> int:
+        """The adapters' delta of a linear as one more partial behind its ``splits``; returns their number."""
+        if self.adapters is None or target not in self.adapters.targets:
+            return splits
+        a, b = self.adapters.layers[li][target]
+        m, n = x.shape[0], b.shape[1]
+        K.lora_delta(x, a, b, self.adapters.scaling, self.adapter_ids, q_len,
+                     out=self.tc_part[splits * m * n:(splits + 1) * m * n].view(m, n), workspace=self.lora_ws)
+        return splits + 1
+
+    def _attend(self, li: int, q: torch.Tensor, q_len: int, scale: float, out: torch.Tensor) -> None:
+        """Attention of the step's tokens over the sequences' caches, behind the shared prefix if there is one."""
+        g, kv = self.g, self.kv
+        if not self.prefix_len:
+            K.decode_attention(q, kv.key_cache[li], kv.value_cache[li], self.B, q_len, g.num_attention_heads,
+                               g.num_key_value_heads, g.head_dim, self.S, scale, cache_pos=kv.cache_pos, out=out,
+                               workspace=self.attn_ws)
+            return
+        K.shared_prefix_attention(q, self.prefix.key[li], self.prefix.value[li], kv.key_cache[li], kv.value_cache[li],
+                                  self.B, q_len, g.num_attention_heads, g.num_key_value_heads, g.head_dim,
+                                  self.prefix_len, self.S, scale, cache_pos=kv.cache_pos, out=out,
+                                  workspace=self.attn_ws)
+
+    # ------------------------------------------------------------------
     def _forward(self, q_len: int, head, advance: bool = True) -> None:
         """Enqueue one step of ``q_len`` tokens per sequence on the current stream.
 
@@ -154,6 +264,8 @@ class DecodeEngine:
         tc = self.backend == "tc"
         split = tc and self.tp is None  # one GPU: the residual linears' partials go to the residual consumer
         part = self.tc_part if tc else None
+        P = self.prefix_len
+        cos, sin = self.cos[P:], self.sin[P:]  # own token j of a sequence sits at position P + j
         s_down = 0
         K.embed_gather(a.ids[:m], rt.embed_tokens_weight, out=a.x[:m])
         for li, layer in enumerate(rt.layers):
@@ -167,27 +279,26 @@ class DecodeEngine:
                     K.residual_rmsnorm_splits(part, s_down, a.h[:m], out_residual=a.x[:m],
                                               norm_w=layer.input_layernorm_weight, eps=eps, out_norm=self.xn[:m])
                 s_qkv = K.gemm_tc_splits(self.xn[:m], att.qkv_proj_weight, part, tiled=tt.get("qkv"))
+                s_qkv = self._lora(li, "qkv", self.xn[:m], s_qkv, q_len)
                 K.qk_norm_rope_splits(part, s_qkv, B, q_len, g.num_attention_heads, g.num_key_value_heads,
-                                      g.head_dim, att.q_norm_weight, att.k_norm_weight, self.cos, self.sin, eps=eps,
+                                      g.head_dim, att.q_norm_weight, att.k_norm_weight, cos, sin, eps=eps,
                                       cache_pos=kv.cache_pos, k_cache=kv.key_cache[li], v_cache=kv.value_cache[li],
                                       max_seq=self.S, q_out=a.q[:m])
             else:
                 K.linear(a.x[:m], att.qkv_proj_weight, norm_w=layer.input_layernorm_weight, eps=eps,
                          out=a.qkv[:m])
-                if q_len == 1:  # q/k norm, RoPE, K/V append and attention in one launch
+                if q_len == 1 and not P:  # q/k norm, RoPE, K/V append and attention in one launch
                     K.decode_attention_qkv(a.qkv[:m], B, g.num_attention_heads, g.num_key_value_heads, g.head_dim,
                                            att.q_norm_weight, att.k_norm_weight, self.cos, self.sin,
                                            kv.key_cache[li], kv.value_cache[li], self.S, att.attention_scale,
                                            eps=eps, cache_pos=kv.cache_pos, out=a.attn[:m])
                 else:
                     K.qk_norm_rope(a.qkv[:m], B, q_len, g.num_attention_heads, g.num_key_value_heads, g.head_dim,
-                                   att.q_norm_weight, att.k_norm_weight, self.cos, self.sin, eps=eps,
+                                   att.q_norm_weight, att.k_norm_weight, cos, sin, eps=eps,
                                    cache_pos=kv.cache_pos, k_cache=kv.key_cache[li], v_cache=kv.value_cache[li],
                                    max_seq=self.S, q_out=a.q[:m])
-            if tc or q_len != 1:
-                K.decode_attention(a.q[:m], kv.key_cache[li], kv.value_cache[li], B, q_len, g.num_attention_heads,
-                                   g.num_key_value_heads, g.head_dim, self.S, att.attention_scale,
-                                   cache_pos=kv.cache_pos, out=a.attn[:m], workspace=self.attn_ws)
+            if tc or q_len != 1 or P:
+                self._attend(li, a.q[:m], q_len, att.attention_scale, a.attn[:m])
             if self.tp is not None:
                 self._row_split(a.attn[:m], att.o_proj_weight, a.x[:m], a.h[:m], tc, tt.get("o"))
                 if tc:
@@ -199,10 +310,12 @@ class DecodeEngine:
                 self._row_split(a.act[:m], mlp.down_proj_weight, a.h[:m], a.x[:m], tc, tt.get("down"))
             elif split:
                 s_o = K.gemm_tc_splits(a.attn[:m], att.o_proj_weight, part, tiled=tt.get("o"))
+                s_o = self._lora(li, "o", a.attn[:m], s_o, q_len)
                 K.residual_rmsnorm_splits(part, s_o, a.x[:m], out_residual=a.h[:m],
                                           norm_w=layer.post_attention_layernorm_weight, eps=eps, out_norm=self.xn[:m])
-                self._gate_up(self.xn[:m], mlp.gate_up_proj_weight, a.act[:m], tt.get("gu"))
+                self._gate_up(self.xn[:m], mlp.gate_up_proj_weight, a.act[:m], tt.get("gu"), li, q_len)
                 s_down = K.gemm_tc_splits(a.act[:m], mlp.down_proj_weight, part, tiled=tt.get("down"))
+                s_down = self._lora(li, "down", a.act[:m], s_down, q_len)
             else:
                 K.oproj_residual(a.attn[:m], att.o_proj_weight, a.x[:m], out=a.h[:m])
                 K.gateup_silu(a.h[:m], layer.post_attention_layernorm_weight, mlp.gate_up_proj_weight, eps,
@@ -222,12 +335,14 @@ class DecodeEngine:
             else:
                 a.head_rows.copy_(a.x[:m].view(B, q_len, -1)[:, -1])
                 rows, n, dest = a.head_rows, B, a.ids[:B]
-            self._head(rows, n, dest, tc, normed=normed)
+            self._head(rows, n, dest, tc, normed=normed, rules=self.rules if head != "all" else None)
         if advance:
             K.advance_cursors(kv.cache_pos, q_len)
 
-    def _head(self, rows: torch.Tensor, n: int, dest: torch.Tensor, tc: bool, normed: bool = False) -> None:
-        """Greedy head over ``rows [n, H]``: final norm, lm_head (this rank's vocab shard), argmax into ``dest``.
+    def _head(self, rows: torch.Tensor, n: int, dest: torch.Tensor, tc: bool, normed: bool = False,
+              rules: TokenRules | None = None) -> None:
+        """Greedy head over ``rows [n, H]``: final norm, lm_head (this rank's vocab shard), argmax into ``dest``
+        (under ``rules``: their pick).
         ``normed``: ``xn[:n]`` already holds the final norm of ``rows`` (tensor-core path)."""
         rt, eps = self.rt, self.g.rms_norm_eps
         self._head_rows = rows
@@ -246,7 +361,13 @@ class DecodeEngine:
             if not normed:
                 K.rmsnorm(rows, rt.final_norm_weight, eps, out=self.xn[:n])
             K.gemm_tc(self.xn[:n], rt.lm_head_weight, out=self.logits[:n], workspace=self.tc_ws)
-            K.argmax_rows(self.logits[:n], out_ids=dest, workspace=self.lm_ws)
+            if rules is not None:
+                rules.pick(self.logits[:n], dest)
+            else:
+                K.argmax_rows(self.logits[:n], out_ids=dest, workspace=self.lm_ws)
+        elif rules is not None:
+            K.linear(rows, rt.lm_head_weight, norm_w=rt.final_norm_weight, eps=eps, out=self.logits[:n])
+            rules.pick(self.logits[:n], dest)
         else:
             K.lmhead_argmax(rows, rt.final_norm_weight, rt.lm_head_weight, eps, out_ids=dest, workspace=self.lm_ws)
 
@@ -265,20 +386,55 @@ class DecodeEngine:
         B, P = prompt_ids.shape
         if len(set(self.kv.sequence_lens)) != 1 or self.kv.sequence_lens[0] + P > self.S:
             raise ValueError("prefill_full needs equal cursors and room for the prompt")
-        g, rt, a, kv = self.g, self.rt, self.arenas, self.kv
+        ids = prompt_ids.to(self.rt.device, torch.int64)
+        kv, a = self.kv, self.arenas
+        x = self._prompt_pass(ids.reshape(-1), B, P, kv.key_cache, kv.value_cache, self.S, kv.cache_pos,
+                              self.adapter_ids if self.adapters is not None else None)
+        if self.rules is not None:
+            self.rules.note_prompt(ids.contiguous())
+        a.head_rows.copy_(x.view(B, P, -1)[:, -1])
+        self._head(a.head_rows, B, a.ids[:B], self.backend == "tc", rules=self.rules)
+        K.advance_cursors(kv.cache_pos, P)
+        kv.note_advanced(P)
+        return a.ids[:B].clone()
+
+    def _prompt_pass(self, ids: torch.Tensor, B: int, P: int, key_cache, value_cache, max_seq: int,
+                     cache_pos: torch.Tensor | None, adapter_ids: torch.Tensor | None) -> torch.Tensor:
+        """``B * P`` prompt tokens through every layer at once, their K/V into the given caches (per layer ``[B,
+        Hkv, max_seq, D]``, from ``cache_pos`` on, or from 0); returns the last layer's hidden rows."""
+        g, rt = self.g, self.rt
         dev, dt, eps, m = rt.device, rt.dtype, g.rms_norm_eps, B * P
-        ids = prompt_ids.to(dev, torch.int64).reshape(-1)
+        pre = self.prefix_len
+        cos, sin = self.cos[pre:], self.sin[pre:]
         x = torch.empty(m, g.hidden_size, device=dev, dtype=dt)
         h = torch.empty_like(x)
         xn = torch.empty_like(x)
-        qkv = torch.empty(m, g.qkv_dim, device=dev, dtype=dt)
         q = torch.empty(m, g.num_attention_heads, g.head_dim, device=dev, dtype=dt)
         attn = torch.empty(m, g.q_dim, device=dev, dtype=dt)
         act = torch.empty(m, g.intermediate_size, device=dev, dtype=dt)
         part = torch.empty(m, g.hidden_size, device=dev, dtype=torch.float32) if self.tp is not None else None
+        qkv = None  # bf16; with adapters the wide linears go through one fp32 buffer instead
+        lora = self.adapters.targets if adapter_ids is not None else ()
+        wide = None
+        if lora:
+            wide = torch.empty(m * max(self.adapters.shapes[t][1] for t in lora), device=dev, dtype=torch.float32)
+            lora_ws = torch.empty(m * self.adapters.rank * 4, device=dev, dtype=torch.uint8)
+        if "qkv" not in lora:
+            qkv = torch.empty(m, g.qkv_dim, device=dev, dtype=dt)
 
-        def row_split(inp, w, res, out):
-            if self.tp is None:
+        def adapted(li, target, inp, w):
+            """The linear in fp32 with its adapter added, before its one rounding."""
+            out = wide[:m * w.shape[0]].view(m, w.shape[0])
+            K.gemm_big(inp, w, epilogue=K.EPI_STORE_F32, out=out)
+            a_, b_ = self.adapters.layers[li][target]
+            K.lora_delta(inp, a_, b_, self.adapters.scaling, adapter_ids, P, accumulate=True, out=out,
+                         workspace=lora_ws)
+            return out
+
+        def row_split(li, target, inp, w, res, out):
+            if target in lora:
+                K.residual_add_f32(res, adapted(li, target, inp, w), out=out)
+            elif self.tp is None:
                 K.gemm_big(inp, w, epilogue=K.EPI_RESIDUAL, residual=res, out=out)
             else:
                 K.gemm_big(inp, w, epilogue=K.EPI_STORE_F32, out=part)
@@ -288,31 +444,42 @@ class DecodeEngine:
         K.embed_gather(ids, rt.embed_tokens_weight, out=x)
         for li, layer in enumerate(rt.layers):
             att, mlp = layer.attention, layer.mlp
+            kc, vc = key_cache[li], value_cache[li]
+            rope = dict(eps=eps, cache_pos=cache_pos, k_cache=kc, v_cache=vc, max_seq=max_seq, q_out=q)
+            heads = (g.num_attention_heads, g.num_key_value_heads, g.head_dim, att.q_norm_weight, att.k_norm_weight,
+                     cos, sin)
             K.rmsnorm(x, layer.input_layernorm_weight, eps, out=xn)
-            K.gemm_big(xn, att.qkv_proj_weight, out=qkv)
-            K.qk_norm_rope(qkv, B, P, g.num_attention_heads, g.num_key_value_heads, g.head_dim, att.q_norm_weight,
-                           att.k_norm_weight, self.cos, self.sin, eps=eps, cache_pos=kv.cache_pos,
-                           k_cache=kv.key_cache[li], v_cache=kv.value_cache[li], max_seq=self.S, q_out=q)
-            K.decode_attention(q, kv.key_cache[li], kv.value_cache[li], B, P, g.num_attention_heads,
-                               g.num_key_value_heads, g.head_dim, self.S, att.attention_scale,
-                               cache_pos=kv.cache_pos, out=attn, workspace=self.attn_ws)
-            row_split(attn, att.o_proj_weight, x, h)
+            if "qkv" in lora:
+                K.qk_norm_rope_splits(adapted(li, "qkv", xn, att.qkv_proj_weight), 1, B, P, *heads, **rope)
+            else:
+                K.gemm_big(xn, att.qkv_proj_weight, out=qkv)
+                K.qk_norm_rope(qkv, B, P, *heads, **rope)
+            if pre:
+                K.shared_prefix_attention(q, self.prefix.key[li], self.prefix.value[li], kc, vc, B, P,
+                                          g.num_attention_heads, g.num_key_value_heads, g.head_dim, pre, max_seq,
+                                          att.attention_scale, cache_pos=cache_pos, out=attn)
+            else:
+                K.decode_attention(q, kc, vc, B, P, g.num_attention_heads, g.num_key_value_heads, g.head_dim, max_seq,
+                                   att.attention_scale, cache_pos=cache_pos, out=attn, workspace=self.attn_ws)
+            row_split(li, "o", attn, att.o_proj_weight, x, h)
             K.rmsnorm(h, layer.post_attention_layernorm_weight, eps, out=xn)
-            K.gemm_big(xn, mlp.gate_up_proj_weight, epilogue=K.EPI_SILU_MUL, out=act)
-            row_split(act, mlp.down_proj_weight, h, x)
-        a.head_rows.copy_(x.view(B, P, -1)[:, -1])
-        self._head(a.head_rows, B, a.ids[:B], self.backend == "tc")
-        K.advance_cursors(kv.cache_pos, P)
-        kv.note_advanced(P)
-        return a.ids[:B].clone()
+            if "gate_up" in lora:
+                K.silu_mul_splits(adapted(li, "gate_up", xn, mlp.gate_up_proj_weight), 1, m, g.intermediate_size,
+                                  out=act)
+            else:
+                K.gemm_big(xn, mlp.gate_up_proj_weight, epilogue=K.EPI_SILU_MUL, out=act)
+            row_split(li, "down", act, mlp.down_proj_weight, h, x)
+        return x
 
-    def _gate_up(self, xn: torch.Tensor, w: torch.Tensor, act: torch.Tensor, tiled: torch.Tensor | None) -> None:
+    def _gate_up(self, xn: torch.Tensor, w: torch.Tensor, act: torch.Tensor, tiled: torch.Tensor | None,
+                 li: int = 0, q_len: int = 1) -> None:
         """act = SiLU(gate) * up on the tensor cores: plain split-partial linear +
         combine (the paired tile image is the plain one when I % 128 == 0), or
         the paired SiLU epilogue."""
         m = xn.shape[0]
         if self.gu_plain:
             s_gu = K.gemm_tc_splits(xn, w, self.tc_part, tiled=tiled)
+            s_gu = self._lora(li, "gate_up", xn, s_gu, q_len)
             K.silu_mul_splits(self.tc_part, s_gu, m, w.shape[0] // 2, out=act)
         else:
             K.gemm_tc(xn, w, epilogue=K.EPI_SILU_MUL, out=act, workspace=self.tc_ws, tiled=tiled)
@@ -358,6 +525,8 @@ class DecodeEngine:
         start = self.kv.sequence_lens[0]
         if start + P > self.S:
             raise ValueError(f"prompt of {P} tokens does not fit: cursor {start}, max_seq {self.S}")
+        if self.rules is not None:
+            self.rules.note_prompt(ids.contiguous())
         chunk = max(1, self.T // self.B)
         for c0 in range(0, P, chunk):
             c1 = min(P, c0 + chunk)
@@ -378,10 +547,14 @@ class DecodeEngine:
         a = self.arenas
         saved_pos = self.kv.cache_pos.clone()
         saved_ids = a.ids[:self.B].clone()
+        saved_rules = (self.rules.counts.clone(), self.rules.seen.clone()) if self.rules is not None else None
         self._decode_once()  # eager warm-up: sets kernel attributes, resolves symbols
         torch.cuda.synchronize()
         self.kv.cache_pos.copy_(saved_pos)
         a.ids[:self.B].copy_(saved_ids)
+        if saved_rules is not None:
+            self.rules.counts.copy_(saved_rules[0])
+            self.rules.seen.copy_(saved_rules[1])
         graph = torch.cuda.CUDAGraph()
         stream = torch.cuda.Stream()
         stream.wait_stream(torch.cuda.current_stream())
@@ -416,6 +589,8 @@ class DecodeEngine:
         The host's cursor mirror is not updated (that would need a sync); call
         :meth:`sync_cursors` to refresh it.
         """
+        if self.rules is not None:
+            raise ValueError("a verify pass takes the plain greedy token of every position: no token rules")
         if self.B * (k + 1) > self.T:
             raise ValueError(f"verify of {self.B} x {k + 1} tokens exceeds the {self.T}-token step")
         if max(self.kv.sequence_lens) + k + 1 > self.S:
@@ -483,6 +658,12 @@ class DecodeEngine:
         """Kernels one decode step launches (embedding, layers, head, cursor advance)."""
         per_layer = (9 if self.gu_plain else 8) if self.backend == "tc" else 5  # CUDA cores: attention takes the q/k norm
         head = 3 if self.backend == "tc" else 1
+        if self.prefix_len:  # prefix, strips and join instead of one attention (after a q/k norm of its own)
+            per_layer += 2 if self.backend == "tc" else 3
+        if self.adapters is not None:  # shrink and expand beside each linear
+            per_layer += 2 * len(self.adapters.targets)
+        if self.rules is not None:  # rules and pick instead of the argmax (after an lm_head of its own)
+            head += 1 if self.backend == "tc" else 2
         if self.tp is not None:  # + all-reduce / residual-add kernels after each row-split linear, + keys-to-ids
             if self.tp.p2p is None or self.backend == "tc":
                 per_layer += 2

@@ -32,6 +32,8 @@ class SpeculativeDecoder:
             raise ValueError("draft and target engines must hold the same batch")
         if proposal_len < 1:
             raise ValueError("proposal_len must be positive")
+        if draft.rules is not None or target.rules is not None:
+            raise ValueError("proposals and verdicts are plain greedy tokens: no token rules")
         if target.B * (proposal_len + 1) > target.T:
             raise ValueError(f"verify of {target.B} x {proposal_len + 1} tokens exceeds the target's "
                              f"{target.T}-token step")
@@ -43,7 +45,7 @@ class SpeculativeDecoder:
         self.out = torch.zeros(self.B, max_new_tokens, device=dev, dtype=torch.int64)
         self.out_len = torch.zeros(self.B, device=dev, dtype=torch.int32)
         self.use_graph = use_graph
-        self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
+        self.graphs: dict[tuple, torch.cuda.CUDAGraph] = {}
 
     def prefill(self, prompt_ids: torch.Tensor) -> torch.Tensor:
         """Prefill both models; returns the target's first greedy token per sequence (the first current)."""
@@ -63,6 +65,10 @@ class SpeculativeDecoder:
             ids[:, i + 1].copy_(d.arenas.ids[:self.B])
         t._verify_once(k, draft_cache_pos=d.kv.cache_pos, out_tokens=self.out, out_len=self.out_len)
 
+    def _graph_key(self, k: int) -> tuple:
+        """A captured cycle is good for its proposal length and the engines' present prefixes."""
+        return k, self.draft.prefix_epoch, self.target.prefix_epoch
+
     def _capture(self, k: int) -> None:
         d, t = self.draft, self.target
         saved = [x.clone() for x in (d.kv.cache_pos, t.kv.cache_pos, d.arenas.ids, t.arenas.ids, t.next_ids,
@@ -79,7 +85,7 @@ class SpeculativeDecoder:
             self._cycle(k)
         torch.cuda.current_stream().wait_stream(stream)
         torch.cuda.synchronize()
-        self.graphs[k] = graph
+        self.graphs[self._graph_key(k)] = graph
 
     def cycle(self, k: int | None = None) -> None:
         """Enqueue one draft-propose / target-verify / accept cycle (no host sync)."""
@@ -88,9 +94,10 @@ class SpeculativeDecoder:
             if max(eng.kv.sequence_lens) + k + 1 > eng.S:
                 raise ValueError("KV cache is full")
         if self.use_graph:
-            if k not in self.graphs:
+            key = self._graph_key(k)
+            if key not in self.graphs:
                 self._capture(k)
-            self.graphs[k].replay()
+            self.graphs[key].replay()
         else:
             self._cycle(k)
         # conservative host bounds until sync_cursors()
