@@ -331,19 +331,20 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
           }
         }
         const float neg_m = m_run == -INFINITY ? 0.f : -m_run;  // a row without keys so far: exp2(-inf) = 0
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), neg2 = make_float2(neg_m, neg_m);
+        float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[kSpKeys / 2];
 #pragma unroll
         for (int e = 0; e < kSpKeys / 2; ++e) {
-          const float x0 = ex2_approx(fmaf(__uint_as_float(sv[2 * e]), p.scale_log2, neg_m));
-          const float x1 = ex2_approx(fmaf(__uint_as_float(sv[2 * e + 1]), p.scale_log2, neg_m));
-          ls[(2 * e) & 3] += x0;
-          ls[(2 * e + 1) & 3] += x1;
-          const __nv_bfloat162 v2 = __floats2bfloat162_rn(x0, x1);
+          float2 x = fma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale2, neg2);
+          x.x = ex2_approx(x.x);
+          x.y = ex2_approx(x.y);
+          ls[e & 1] = add2(ls[e & 1], x);
+          const __nv_bfloat162 v2 = __floats2bfloat162_rn(x.x, x.y);
           pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
         }
         tmem_st32(tS, pk);
-        l_run = l_run * corr + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+        l_run = l_run * corr + ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y));
         tmem_st_wait();
       }
       if (nk < kSpKeys) {
