@@ -11,6 +11,7 @@ import ctypes
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libleanb200.so"
+FRONT_PATH = LIB_PATH.parent / "_torch_front.so"
 
 LS_OK = 0
 STATUS_NAMES = {
@@ -125,6 +126,7 @@ PROFILING_SIGNATURES: dict[str, list] = {
 }
 
 _LIB: ctypes.CDLL | None = None
+_FRONT = None
 
 
 def load() -> ctypes.CDLL:
@@ -151,6 +153,30 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+def front():
+    """The C++ front end of the multi-request calls (csrc/torch_front.cpp), loaded once."""
+    global _FRONT
+    if _FRONT is not None:
+        return _FRONT
+    load()
+    if not FRONT_PATH.exists():
+        raise NativeLibraryMissing(f"{FRONT_PATH} is missing: build it with `python -m leanstack_b200.build`")
+    import importlib.machinery
+    import importlib.util
+
+    import torch
+
+    spec = importlib.util.spec_from_loader(
+        "_torch_front", importlib.machinery.ExtensionFileLoader("_torch_front", str(FRONT_PATH)))
+    mod = importlib.util.module_from_spec(spec)
+    if torch.__version__.split("+")[0] != mod.torch_version:
+        raise NativeLibraryMissing(f"{FRONT_PATH} was built for PyTorch {mod.torch_version}, this is "
+                                   f"{torch.__version__}: rebuild it with `python -m leanstack_b200.build --force`")
+    spec.loader.exec_module(mod)
+    _FRONT = mod
+    return mod
+
+
 def last_error() -> str:
     msg = load().ls_last_error()
     return msg.decode("utf-8", "replace") if msg else ""
@@ -160,6 +186,13 @@ def call(name: str, *args) -> None:
     rc = getattr(load(), name)(*args)
     if rc != LS_OK:
         raise LeanB200Error(name, rc, last_error())
+
+
+def finished(name: str, done):
+    """What a front-end call of ``name`` returned: its output tensor, or a status to raise."""
+    if type(done) is int:
+        raise LeanB200Error(name, done, last_error())
+    return done
 
 
 def exported_symbols() -> list[str]:

@@ -1,4 +1,4 @@
-"""Build libleanb200.so in-tree with nvcc for sm_100a.
+"""Build libleanb200.so (nvcc, sm_100a) and the front end _torch_front.so (host C++) in-tree.
 
 ``python -m leanstack_b200.build [--force] [--verbose] [--profiling]`` compiles
 every ``csrc/*.cu`` into ``leanstack_b200/_lib/libleanb200.so``.
@@ -7,7 +7,9 @@ hooks (per-CTA timestamp buffers, the NVLink ping-pong probe) to the library;
 the default build has none of them.  The library links
 the shared CUDA runtime (``libcudart.so.12``), so inside a PyTorch process it
 binds to the runtime PyTorch already loaded and sees the same current device
-and streams.  No GPU is needed to build.
+and streams.  ``csrc/torch_front.cpp`` becomes ``_lib/_torch_front.so``, a Python
+module on the installed PyTorch's headers that calls the library.  No GPU is
+needed to build.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -26,6 +29,8 @@ INCLUDE = PKG.parent / "include"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libleanb200.so"
 OBJ_DIR = PKG / "_build"
+FRONT_SRC = CSRC / "torch_front.cpp"
+FRONT = OUT_DIR / "_torch_front.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
@@ -68,6 +73,33 @@ def _compile(src: Path, verbose: bool, ptxas_verbose: bool, defines: list[str]) 
     return obj, res.stderr
 
 
+def needs_front() -> bool:
+    if not FRONT.exists():
+        return True
+    return any(p.stat().st_mtime > FRONT.stat().st_mtime for p in [FRONT_SRC, *INCLUDE.glob("*.h"), Path(__file__)])
+
+
+def build_front(verbose: bool = False) -> Path:
+    """Compile the front end against the installed PyTorch and link it to libleanb200.so beside it."""
+    import torch
+
+    home = Path(torch.__file__).parent
+    tmp = FRONT.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(home / "include"),
+           "-I", str(home / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda_home() / "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", str(INCLUDE), str(FRONT_SRC), "-o", str(tmp),
+           "-L", str(home / "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+           "-L", str(OUT_DIR), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"the front end failed to build:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, FRONT)
+    return FRONT
+
+
 def needs_build(defines: list[str] | None = None) -> bool:
     if not LIB.exists():
         return True
@@ -80,6 +112,8 @@ def needs_build(defines: list[str] | None = None) -> bool:
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False, profiling: bool = False) -> Path:
     defines = ["-DLEANB200_PROFILING"] if profiling else []
     if not force and not needs_build(defines):
+        if needs_front():
+            build_front(verbose)
         return LIB
     OUT_DIR.mkdir(parents=True, exist_ok=True)
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
@@ -104,6 +138,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
     STAMP.write_text(" ".join(defines) + "\n")
+    build_front(verbose)
     return LIB
 
 

@@ -645,6 +645,11 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     ``workspace``: ``shared_prefix_attention_workspace_bytes`` long, needs no
     filling; calls on one stream may share it.
     """
+    done = (nat._FRONT or nat.front()).shared_prefix_attention(
+        q, k_prefix, v_prefix, k_cache, v_cache, batch, q_len, num_heads, num_kv_heads, head_dim, prefix_len, max_seq,
+        scale, cache_pos, uniform_past, out, workspace)
+    if done is not None:
+        return nat.finished("ls_shared_prefix_attention", done)
     _check(q, "q")
     if q.numel() != batch * q_len * num_heads * head_dim:
         raise ValueError(f"q holds {q.numel()} elements, expected {batch} x {q_len} x {num_heads} x {head_dim}")
@@ -692,6 +697,9 @@ def lora_delta(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch
     the shared projection before the one rounding; ``accumulate`` adds to ``out``
     instead.  ``workspace`` needs no filling; calls on one stream may share it.
     """
+    done = (nat._FRONT or nat.front()).lora_delta(x, a, b, scaling, adapter_ids, q_len, accumulate, out, workspace)
+    if done is not None:
+        return nat.finished("ls_lora_delta", done)
     _check(x, "x")
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError("lora_delta takes x [m, k], a [adapters, rank, k] and b [adapters, n, rank]")
@@ -746,6 +754,11 @@ def constrained_argmax(logits: torch.Tensor, *, counts: torch.Tensor | None = No
     processed logits (-inf where not allowed).  ``workspace`` needs no filling;
     calls on one stream may share it.
     """
+    done = (nat._FRONT or nat.front()).constrained_argmax(
+        logits, counts, seen, repetition, frequency, presence, bias_ids, bias_values, allowed, record, out_ids,
+        out_logits, workspace)
+    if done is not None:
+        return nat.finished("ls_constrained_argmax", done)
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (BF16, torch.float32):
         raise TypeError("logits must be a bf16 or fp32 tensor")
     _check(logits, "logits", logits.dtype)
