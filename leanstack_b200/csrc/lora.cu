@@ -7,7 +7,7 @@
 // so the kernel that adds the partials adds the adapter too and the projection
 // plus its adapter round once.
 //
-// Two launches, both on mma.sync m16n8k16 (16 tokens x 8 ranks or outputs); the
+// Two halves, both on mma.sync m16n8k16 (16 tokens x 8 ranks or outputs); the
 // operands go from global memory straight into the fragments, since both sides may
 // take k in any order as long as it is the same one: a lane's 16 (8) bytes of a
 // row are its k's of two (one) MMA steps.
@@ -17,19 +17,22 @@
 //   * Expand: u keeps its 24 bits as a sum of three bf16 (8 bits each), three
 //     products per step; the outputs of a lane are four neighbours, one 16-byte
 //     store a row.
-// Short sequences (decode, verify): the CTA of a sequence works for every sequence
-// with the same adapter if it is the first of them (within a window of 1024), so an
-// adapter is read once for all its tokens; long ones (prompts, q_len >= 16): a CTA
-// takes tokens of one sequence.
+// Two launches, or one in which a cluster does both halves of a tile (lora_one_launch).
+// Short sequences (decode, verify): the tokens of one adapter (within a window of 1024
+// sequences) make tiles of 16, and the CTA of a tile's first sequence works for all of
+// it, so an adapter is read once for every 16 of its tokens; one CTA for all of them
+// walked its tiles one by one (64 tokens of one adapter, 2560 -> 6144: 23 us, in tiles
+// at once 7.4).  Long ones (prompts, q_len >= 16): a CTA takes tokens of one sequence.
 // What bounds it: memory -- A and B of the adapters in use for short sequences
-// (where two dependent launches of a few MB are latency), x and the fp32 output for
-// prompts.  Tensor cores of the tcgen05 kind would wait: 2 r flops per byte of x.
+// (where a few MB are latency), x and the fp32 output for prompts.  Tensor cores of
+// the tcgen05 kind would wait: 2 r flops per byte of x.
 #include "mma_sync.cuh"
 
 namespace lsb {
 
 constexpr int kLoThreads = 128;
 constexpr int kLoWarps = 4;
+constexpr int kLoOneRanks = 64;   // of the one-launch kernel (its sums: 16 tokens x ranks of every warp)
 constexpr int kLoWindow = 1024;   // sequences among which equal adapters share a CTA
 constexpr int kLoPrompt = 16;     // q_len from which a CTA takes tokens of one sequence
 constexpr int kLoTile = 128;      // shrink: tokens of a prompt CTA (32 a warp)
@@ -61,37 +64,41 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int b) {
   return id < 0 ? -1 : id;
 }
 
-// Short sequences: the sequences that the CTA of sequence b works for, in order: those
-// of its adapter in its window if it is the first of them, else none.  Returns their
-// number; `members` holds their indices.
-__device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, int* members) {
-  __shared__ int s_count[kLoWarps], s_first;
-  const int w0 = b / kLoWindow * kLoWindow, w1 = min(w0 + kLoWindow, p.batch);
+// Short sequences: the sequences that the CTA of sequence b works for, a tile of at most
+// 16 tokens: those of its adapter in its window are counted through, and the first of
+// every 16 / q_len works for itself and those up to the next such.  Returns their number
+// (0: b is not such a first); `members` holds their indices, in order.
+template <int WARPS = kLoWarps>
+__device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, int (&members)[16]) {
+  __shared__ int s_before[WARPS], s_from[WARPS];
+  const int w0 = b / kLoWindow * kLoWindow, w1 = min(w0 + kLoWindow, p.batch), most = 16 / p.q_len;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) s_first = 1;
-  __syncthreads();
-  int n = 0;
-  for (int i0 = w0; i0 < w1; i0 += kLoThreads) {
+  int before = 0, n = 0;
+  for (int i0 = w0; i0 < w1; i0 += WARPS * 32) {
     const int i = i0 + threadIdx.x;
     const bool same = i < w1 && p.ids[i] == id;
-    if (same && i < b) s_first = 0;
-    const uint32_t vote = __ballot_sync(0xffffffffu, same && i >= b);
-    if (lane == 0) s_count[warp] = __popc(vote);
-    __syncthreads();
-    int at = n;
-    for (int w = 0; w < kLoWarps; ++w) {
-      if (w < warp) at += s_count[w];
-      n += s_count[w];
+    const uint32_t vote = __ballot_sync(0xffffffffu, same && i < b), from = __ballot_sync(0xffffffffu, same && i >= b);
+    if (lane == 0) {
+      s_before[warp] = __popc(vote);
+      s_from[warp] = __popc(from);
     }
-    if (vote >> lane & 1u) members[at + __popc(vote & ((1u << lane) - 1u))] = i;
+    __syncthreads();
+    int at = n + __popc(from & ((1u << lane) - 1u));
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) at += s_from[w];
+      n += s_from[w];
+      before += s_before[w];
+    }
+    if ((from >> lane & 1u) && at < most) members[at] = i;
     __syncthreads();
   }
-  return s_first ? n : 0;
+  return before % most ? 0 : min(n, most);
 }
 
 // The lines of `bytes` bytes into L2, while the previous kernel is still at work.
 __device__ __forceinline__ void lora_prefetch(const void* base, int bytes) {
-  for (int i = threadIdx.x * 128; i < bytes; i += kLoThreads * 128)
+  for (int i = threadIdx.x * 128; i < bytes; i += blockDim.x * 128)
     asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(base) + i));
 }
 
@@ -100,23 +107,17 @@ __device__ __forceinline__ uint32_t lo_part(const uint4& v, int i) {
 }
 
 // acc += x a^T over k in [k0, k1) in steps of `step` (each of 32 k): MT tiles of 16
-// tokens (rows g8 and g8 + 8 at xr; null: zeros), NT tiles of 8 of the R ranks at a.
+// tokens (rows g8 and g8 + 8 at xr), NT tiles of 8 of the R ranks at a.  Every xr is a row
+// of x, a missing token's any other's, and so are the rows of a past R: rows and columns
+// of the products are independent, and those are not used.  Only k's past k1 are zeros.
 template <int MT, int NT>
 __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2], const __nv_bfloat16* a, int K, int R, int k0,
                                          int k1, int step, float (&acc)[MT][NT][4]) {
   const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-#pragma unroll (MT * 2 + NT <= 4 ? 4 : 2)
-  for (int k = k0; k < k1; k += step) {
-    const int kk = k + t4 * 8;  // k1 is a multiple of 8: a lane's 8 are there or not
-    const bool in = kk < k1;
-    uint4 xv[MT][2], av[NT];
+  const __nv_bfloat16* ar[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) xv[i][h] = in && xr[i][h] ? ldg16(xr[i][h] + kk) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-      av[j] = in && j * 8 + g8 < R ? ldg16(a + (size_t)(j * 8 + g8) * K + kk) : make_uint4(0, 0, 0, 0);
+  for (int j = 0; j < NT; ++j) ar[j] = a + (size_t)(j * 8 + g8 < R ? j * 8 + g8 : 0) * K;
+  auto products = [&](const uint4 (&xv)[MT][2], const uint4 (&av)[NT]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -126,7 +127,50 @@ __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2]
 #pragma unroll
         for (int j = 0; j < NT; ++j) mma_bf16(acc[i][j], fa, lo_part(av[j], 2 * s), lo_part(av[j], 2 * s + 1));
       }
+  };
+  int k = k0;
+#pragma unroll (MT * 2 + NT <= 4 ? 4 : 2)
+  for (; k + 32 <= k1; k += step) {
+    const int kk = k + t4 * 8;
+    uint4 xv[MT][2], av[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xv[i][h] = ldg16(xr[i][h] + kk);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) av[j] = ldg16(ar[j] + kk);
+    products(xv, av);
   }
+  if (k < k1) {  // k1 is a multiple of 8: a lane's 8 are there or not
+    const int kk = k + t4 * 8;
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    uint4 xv[MT][2], av[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xv[i][h] = kk < k1 ? ldg16(xr[i][h] + kk) : none;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) av[j] = kk < k1 ? ldg16(ar[j] + kk) : none;
+    products(xv, av);
+  }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// An fp32 at the same place as `local` in CTA `cta` of the cluster.
+__device__ __forceinline__ float ld_cluster(const float* local, int cta) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(cta));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_cluster(float* local, int cta, float v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(cta));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
 // Elements [0, n) of the cluster's CTAs' partials, added in split order; CTA c of
@@ -134,7 +178,7 @@ __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2]
 template <typename Store>
 __device__ __forceinline__ void lora_join_splits(const float* part, int n, Store store) {
   const int c = blockIdx.x, ncta = gridDim.x;  // the cluster is the grid's x extent
-  if (ncta > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (ncta > 1) cluster_sync();
   else __syncthreads();
   for (int i = c * kLoThreads + threadIdx.x; i < n; i += ncta * kLoThreads) {
     float v = 0.f;
@@ -143,11 +187,7 @@ __device__ __forceinline__ void lora_join_splits(const float* part, int n, Store
     } else {
       float w[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part + i)), "r"(q < ncta ? q : 0));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w[q]) : "r"(at) : "memory");
-      }
+      for (int q = 0; q < 8; ++q) w[q] = ld_cluster(part + i, q < ncta ? q : 0);
 #pragma unroll
       for (int q = 0; q < 8; ++q)
         if (q < ncta) v += w[q];
@@ -155,14 +195,14 @@ __device__ __forceinline__ void lora_join_splits(const float* part, int n, Store
     store(i, v);
   }
   // The partials are read by others: they stay until all are done.
-  if (ncta > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (ncta > 1) cluster_sync();
   else __syncthreads();
 }
 
 // Short sequences: the four warps share the CTA's k range; their sums meet in shared memory.
 template <int NT>
 __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
-  __shared__ int members[kLoWindow];
+  __shared__ int members[16];
   __shared__ float red[kLoWarps][16][NT * 8 + 1], part[16 * NT * 8];
   grid_dep_wait();
   grid_dep_launch();
@@ -170,30 +210,28 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
   const int id = lora_adapter(p, b);
   if (id < 0) return;
   const int tokens = lora_group(p, b, id, members) * p.q_len;
+  if (!tokens) return;  // the whole cluster
   const int k0 = blockIdx.x * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
   const int r0 = blockIdx.z * kLoRanks, ranks = min(kLoRanks, p.R - r0);
   auto token = [&](int i) { return members[i / p.q_len] * p.q_len + i % p.q_len; };
-  for (int i0 = 0; i0 < tokens; i0 += 16) {
-    const __nv_bfloat16* xr[1][2];
+  const __nv_bfloat16* xr[1][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      xr[0][h] = i0 + g8 + 8 * h < tokens ? p.x + (size_t)token(i0 + g8 + 8 * h) * p.K : nullptr;
-    float acc[1][NT][4] = {};
-    lora_dot<1, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0 + warp * 32, k1, 32 * kLoWarps, acc);
+  for (int h = 0; h < 2; ++h) xr[0][h] = p.x + (size_t)token(g8 + 8 * h < tokens ? g8 + 8 * h : 0) * p.K;
+  float acc[1][NT][4] = {};
+  lora_dot<1, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0 + warp * 32, k1, 32 * kLoWarps, acc);
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][g8 + 8 * (e >> 1)][j * 8 + 2 * t4 + (e & 1)] = acc[0][j][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * NT * 8; i += kLoThreads) {
-      const int t = i / (NT * 8), r = i % (NT * 8);
-      part[i] = (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
-    }
-    lora_join_splits(part, 16 * NT * 8, [&](int i, float v) {
-      const int t = i / (NT * 8), r = i % (NT * 8);
-      if (i0 + t < tokens && r < ranks) p.u[(size_t)token(i0 + t) * p.R + r0 + r] = v;
-    });
+    for (int e = 0; e < 4; ++e) red[warp][g8 + 8 * (e >> 1)][j * 8 + 2 * t4 + (e & 1)] = acc[0][j][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * NT * 8; i += kLoThreads) {
+    const int t = i / (NT * 8), r = i % (NT * 8);
+    part[i] = (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
   }
+  lora_join_splits(part, 16 * NT * 8, [&](int i, float v) {
+    const int t = i / (NT * 8), r = i % (NT * 8);
+    if (t < tokens && r < ranks) p.u[(size_t)token(t) * p.R + r0 + r] = v;
+  });
 }
 
 // Prompts: a warp takes 32 tokens over the whole k range of the CTA.
@@ -214,7 +252,7 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_prompt_kernel(LoraPara
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int t = i0 + i * 16 + h * 8 + g8;
-      xr[i][h] = t < p.q_len ? p.x + ((size_t)b * p.q_len + t) * p.K : nullptr;
+      xr[i][h] = p.x + ((size_t)b * p.q_len + min(t, p.q_len - 1)) * p.K;
     }
   float acc[2][NT][4] = {};
   lora_dot<2, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0, k1, 32, acc);
@@ -237,16 +275,21 @@ template <int KS>
 struct LoraU {
   uint32_t f[KS][3][4];
   __device__ __forceinline__ void load(const LoraParams& p, const int (&tok)[2]) {  // rows g8, g8 + 8 (< 0: zeros)
+    split(p.R, [&](int h, int k) {
+      return tok[h] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : __ldcg(reinterpret_cast<const float4*>(p.u + (size_t)tok[h] * p.R + k));
+    });
+  }
+  // value(h, k): u of rank k .. k + 3 of row g8 + 8 h
+  template <typename Value>
+  __device__ __forceinline__ void split(int R, Value value) {
     const int t4 = threadIdx.x & 3;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         const int k = s * 16 + t4 * 4;
-        if (tok[h] >= 0 && k < p.R) {
-          v = __ldcg(reinterpret_cast<const float4*>(p.u + (size_t)tok[h] * p.R + k));
-        }
+        const float4 v = k < R ? value(h, k) : make_float4(0.f, 0.f, 0.f, 0.f);
         float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
@@ -271,7 +314,7 @@ __device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS
   const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
   const __nv_bfloat16* b = p.b + (size_t)id * p.N * p.R;
   const float scale = p.scaling[id];
-#pragma unroll 4
+#pragma unroll (KS == 1 ? 8 : 4)
   for (int n = n0; n < n1; n += step) {
     uint2 bv[2][KS];
 #pragma unroll
@@ -310,13 +353,13 @@ __device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS
 // Zeros into outputs [n0, n1) of `count` tokens from token t0 on.
 __device__ __forceinline__ void lora_zeros(const LoraParams& p, int t0, int count, int n0, int n1) {
   const int w = (n1 - n0) / 4;
-  for (int i = threadIdx.x; i < count * w; i += kLoThreads)
+  for (int i = threadIdx.x; i < count * w; i += blockDim.x)
     *reinterpret_cast<float4*>(p.out + (size_t)(t0 + i / w) * p.N + n0 + i % w * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 template <int KS>
 __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
-  __shared__ int members[kLoWindow];
+  __shared__ int members[16];
   // The shrink kernel's CTAs let this one start only after every kernel before them
   // is complete: ids, b and out may be used at once, u after the wait.
   grid_dep_launch();
@@ -331,17 +374,16 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
   const int tokens = lora_group(p, b, id, members) * p.q_len;
   if (tokens > 0) lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
   grid_dep_wait();
-  for (int i0 = 0; i0 < tokens; i0 += 16) {
-    int tok[2];
+  if (!tokens) return;
+  int tok[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = i0 + g8 + 8 * h;
-      tok[h] = i < tokens ? members[i / p.q_len] * p.q_len + i % p.q_len : -1;
-    }
-    LoraU<KS> u;
-    u.load(p, tok);
-    lora_outputs<KS>(p, u, id, tok, n0 + warp * 16, n1, 16 * kLoWarps);
+  for (int h = 0; h < 2; ++h) {
+    const int i = g8 + 8 * h;
+    tok[h] = i < tokens ? members[i / p.q_len] * p.q_len + i % p.q_len : -1;
   }
+  LoraU<KS> u;
+  u.load(p, tok);
+  lora_outputs<KS>(p, u, id, tok, n0 + warp * 16, n1, 16 * kLoWarps);
 }
 
 template <int KS>
@@ -370,6 +412,76 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_prompt_kernel(LoraPara
   lora_outputs<KS>(p, u, id, tok, n0, n1, 16);
 }
 
+// Short sequences, both halves in one launch: a cluster of 8 CTAs per sequence.  CTA c
+// takes k split c for every rank; its partials meet those of the others in shared memory
+// (each CTA adds an eighth of them, in split order, and hands its sums to all), then it
+// takes outputs [c n_block, (c + 1) n_block).
+template <int KS, int THREADS>
+__global__ void __launch_bounds__(THREADS) lora_one_kernel(LoraParams p) {
+  constexpr int NT = KS * 2, RP = KS * 16, WARPS = THREADS / 32;
+  __shared__ int members[16];
+  __shared__ float red[WARPS / 2][16][RP + 1], part[16 * RP];
+  __shared__ __align__(16) float sum[16][RP];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int b = blockIdx.y, c = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
+  const int n0 = min(c * p.n_block, p.N), n1 = min(n0 + p.n_block, p.N);
+  const int id = lora_adapter(p, b);
+  if (id < 0) {  // the whole cluster
+    if (!p.accumulate) lora_zeros(p, b * p.q_len, p.q_len, n0, n1);
+    return;
+  }
+  const int tokens = lora_group<WARPS>(p, b, id, members) * p.q_len;
+  if (!tokens) return;
+  lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
+  const int k0 = c * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
+  const __nv_bfloat16* xr[1][2];
+  int tok[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = g8 + 8 * h;
+    tok[h] = i < tokens ? members[i / p.q_len] * p.q_len + i % p.q_len : -1;
+    xr[0][h] = p.x + (size_t)(tok[h] >= 0 ? tok[h] : members[0] * p.q_len) * p.K;
+  }
+  float acc[1][NT][4] = {};
+  lora_dot<1, NT>(xr, p.a + (size_t)id * p.R * p.K, p.K, p.R, k0 + warp * 32, k1, 32 * WARPS, acc);
+  // Two warps share a place of the sums: the upper one stores, then the lower one adds.
+#pragma unroll
+  for (int half = 1; half >= 0; --half) {
+    if (warp / (WARPS / 2) == half) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float& to = red[warp % (WARPS / 2)][g8 + 8 * (e >> 1)][j * 8 + 2 * t4 + (e & 1)];
+          to = half ? acc[0][j][e] : to + acc[0][j][e];
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 16 * RP; i += THREADS) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS / 2; ++w) v += red[w][i / RP][i % RP];
+    part[i] = v;
+  }
+  cluster_sync();
+  for (int i = c * (2 * RP) + threadIdx.x; i < (c + 1) * (2 * RP); i += THREADS) {
+    float w[8], v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) w[q] = ld_cluster(part + i, q);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += w[q];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) st_cluster(&sum[0][0] + i, q, v);
+  }
+  cluster_sync();  // (and no CTA reads or writes another's memory any more)
+  LoraU<KS> u;
+  u.split(p.R, [&](int h, int k) { return *reinterpret_cast<const float4*>(&sum[g8 + 8 * h][k]); });
+  lora_outputs<KS>(p, u, id, tok, n0 + warp * 16, n1, 16 * WARPS);
+}
+
 }  // namespace lsb
 
 namespace lsb_host {
@@ -386,16 +498,29 @@ static int64_t lora_splits(int64_t batch, int64_t q_len, int64_t k) {
   return s < 1 ? 1 : s;
 }
 
+// Short sequences of rank <= 64, one launch or two.  One saves a launch (about 2 us of
+// host time) and, for many sequences, the CTAs of those that another works for; but eight
+// CTAs a tile are few for wide outputs, and rank 64 wants more of them.  us one / two:
+// rank 16, 6144 outputs: 5.6 / 5.5 (1 sequence; 5.7 / 8.9 with the host's), 7.4 / 8.7
+// (32), 9.0 / 10.8 (100); 19456 outputs: 8.1 / 5.7, 11.7 / 12.3, 14.8 / 18.7; rank 64,
+// 6144 outputs: 9.6 / 6.7, 15.3 / 16.4, 16.4 / 23.0.
+// Threads: 512 halve a CTA's steps, 256 let more CTAs stay: rank 16, 6144 outputs,
+// 256 / 512: 6.1 / 5.6 (1 sequence), 7.4 / 8.1 (32); 19456 outputs: 16.5 / 14.8 (100);
+// rank 64: 15.3 / 22.9 (32).
+static bool lora_one_launch(int64_t batch, int64_t n, int64_t rank) {
+  return batch >= 32 || (rank <= 32 && n <= 8192);
+}
+
 static int64_t lora_workspace(int64_t batch, int64_t q_len, int64_t k, int64_t rank) {
   (void)k;
   return batch * q_len * rank * 4;
 }
 
 static cudaError_t launch_lora_kernel(void (*kernel)(LoraParams), dim3 grid, unsigned cluster, const LoraParams& p,
-                                      cudaStream_t stream) {
+                                      cudaStream_t stream, int threads = kLoThreads) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kLoThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -411,6 +536,16 @@ static cudaError_t launch_lora_kernel(void (*kernel)(LoraParams), dim3 grid, uns
 
 static int launch_lora(LoraParams p, cudaStream_t stream) {
   const bool prompt = p.q_len >= kLoPrompt;
+  if (!prompt && p.R <= kLoOneRanks && lora_one_launch(p.batch, p.N, p.R)) {
+    p.k_chunk = ((p.K + 7) / 8 + 31) / 32 * 32;
+    p.n_block = ((p.N + 7) / 8 + 15) / 16 * 16;
+    const bool wide = p.R <= 32 && (p.batch < 16 || p.N > 8192);
+    void (*one)(LoraParams) = p.R <= 16   ? (wide ? lora_one_kernel<1, 512> : lora_one_kernel<1, 256>)
+                              : p.R <= 32 ? (wide ? lora_one_kernel<2, 512> : lora_one_kernel<2, 256>)
+                                          : lora_one_kernel<4, 256>;
+    const cudaError_t e = launch_lora_kernel(one, dim3(8, (unsigned)p.batch), 8, p, stream, wide ? 512 : 256);
+    return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "lora_delta launch: %s", cudaGetErrorString(e));
+  }
   p.splits = (int)lora_splits(p.batch, p.q_len, p.K);
   p.k_chunk = ((p.K + p.splits - 1) / p.splits + 31) / 32 * 32;
   const int most = prompt ? kLoRanksPrompt : kLoRanks;  // ranks of a shrink CTA

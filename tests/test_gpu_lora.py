@@ -95,6 +95,41 @@ def test_a_window_of_sequences_and_prompts_at_the_edges():
         _assert_close(out, x, a, b, s, ids, q_len)
 
 
+@pytest.mark.parametrize("batch", [1, 3, 15, 16, 40])
+@pytest.mark.parametrize("n", [8, 120, 8192, 8200])
+@pytest.mark.parametrize("rank", [8, 24, 64, 72])
+def test_one_launch_and_two(batch, n, rank):
+    """Few and many sequences, narrow and wide outputs, low and high ranks: every kernel and thread count."""
+    k, adapters = 1064, 4
+    ids = [(i * 3) % 5 - 1 if batch > 1 else 2 for i in range(batch)]
+    x, a, b, s = _inputs(batch, k, n, rank, adapters)
+    t = torch.tensor(ids, device=DEV, dtype=torch.int32)
+    out = torch.full((batch, n), float("nan"), device=DEV)
+    K.lora_delta(x, a, b, s, t, 1, out=out)
+    _assert_close(out, x, a, b, s, ids, 1)
+    base = torch.randn_like(out)
+    acc = base.clone()
+    K.lora_delta(x, a, b, s, t, 1, accumulate=True, out=acc)
+    _assert_close(acc, x, a, b, s, ids, 1, base)
+
+
+@pytest.mark.parametrize("rank", [16, 72])
+@pytest.mark.parametrize("batch,q_len", [(80, 1), (35, 2), (30, 3), (14, 5), (11, 6), (9, 8), (7, 9), (5, 15)])
+def test_tiles_of_one_adapter(batch, q_len, rank):
+    """More tokens of one adapter than a tile holds, sequences that do not divide it, others in between."""
+    k, n = 272, 136
+    for ids in ([0] * batch, [0 if i % 3 else 1 - i % 2 * 2 for i in range(batch)]):
+        x, a, b, s = _inputs(batch * q_len, k, n, rank, 2)
+        x[0] = float("inf")  # stays with its token
+        x[0, 1:] = 1.0
+        out = K.lora_delta(x, a, b, s, torch.tensor(ids, device=DEV, dtype=torch.int32), q_len)
+        x[0] = 0
+        keep = out.clone()
+        keep[0] = K.lora_delta(x, a, b, s, torch.tensor(ids, device=DEV, dtype=torch.int32), q_len)[0]
+        _assert_close(keep, x, a, b, s, ids, q_len)
+        assert ids[0] < 0 or not torch.isfinite(out[0]).any()
+
+
 def test_an_unused_adapter_and_a_token_without_one_may_hold_anything():
     x, a, b, s = _inputs(3, 256, 256, 16, 4)
     a[1], b[1], s[1] = float("nan"), float("inf"), float("nan")
