@@ -34,7 +34,7 @@
 //     two 128-row tiles and share every K/V tile.  Keys (kKeys, at most 128
 //     rows): they hold the same rows and take alternate K/V tiles; their results
 //     join in the epilogue, and 114 KB of shared memory and 128 registers leave
-//     room for three strip CTAs on the same SM.
+//     room for five strip CTAs on the same SM.
 //   * P is rounded to bf16 (2^-8 of each probability, independent from key to
 //     key, against one more 2^-8 when the output is rounded), the row sum is
 //     taken before that rounding in fp32.  The maximum in use moves only when a
@@ -42,6 +42,8 @@
 //   * kFull: a prompt's rows.  A CTA owns 256 rows of one (sequence, kv head)
 //     and walks the prefix tiles, then the sequence's own tiles with the causal
 //     mask, and writes the finished rows: no partials, no join.
+#include <algorithm>
+
 #include "mma_sync.cuh"
 #include "tcgen05.cuh"
 
@@ -57,7 +59,7 @@ constexpr int kSpKvHalf = kSpKeys * 128;           // 64 dims of 64 keys: 8 KB
 constexpr int kSpSlot = 2 * kSpKvHalf;             // one K or V tile: 16 KB
 constexpr int kSpSoft = 256;
 constexpr float kSpRescaleLog2 = 8.f;
-enum SpMode { kKeys = 0, kRows = 1, kFull = 2 };
+enum SpMode { kKeys = 0, kRows = 1, kFull = 2, kFew = 3 };  // (kFew: without prefix_tc_kernel)
 constexpr int sp_threads(int mode) { return mode == kKeys ? 320 : 352; }
 constexpr int sp_slots(int mode) { return mode == kKeys ? 5 : 8; }
 constexpr int sp_ahead(int mode) { return mode == kKeys ? 4 : 2; }  // tiles whose S is issued before the first PV
@@ -452,11 +454,12 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
 }
 
 // Groups of a sequence's own strip: one warp per (sequence, kv head, 16 query
-// rows, key chunk), mma.sync m16n8k16 on 16-key tiles from a 3-stage cp.async
+// rows, key chunk), mma.sync m16n8k16 on 16-key tiles from a 2-stage cp.async
 // ring, online softmax in registers, P rounded to bf16 as in prefix_tc_kernel.
 // A chunk is a row's share of its sequence's keys, at least kStMinBlocks tiles; a
 // chunk behind the end leaves a group without weight.  Single warps: nothing to
-// merge, and the SM's scheduler evens out strips of different lengths.
+// merge, and the SM's scheduler evens out strips of different lengths.  kFew: a short
+// prefix of at most 16 rows in all is taken as one more sequence, whose rows see all of it.
 constexpr int kStMinBlocks = 4;
 constexpr int kStStages = 2;
 constexpr int kStTile = 16 * kTaHeadDim * 2;  // 16 keys of K or V: 4 KB
@@ -470,7 +473,11 @@ struct StParams {
   float* part_o;    // groups n_pre .. n_part - 1 are written here
   float2* part_ml;
   int* err;
+  const __nv_bfloat16* k_prefix;  // kFew: the prefix is sequence `batch`, its rows those of all (16 at most)
+  const __nv_bfloat16* v_prefix;
+  int batch, P, prefix_cap, own;  // own: groups of a sequence's strip
   int q_len, Hq, Hkv, G, R, RG, max_seq, n_pre, n_part;
+  int behind;       // prefix_tc_kernel was launched before
   float scale_log2;
 };
 
@@ -479,23 +486,31 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
   // Behind a prefix: that kernel's CTAs let this one start only after every kernel
   // before is complete, so what is read here is there, and one CTA waits for it at
   // the end, so that whoever waits for this kernel has both.
-  if (p.n_pre == 0) grid_dep_wait();
+  if (!p.behind) grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x, g8 = lane >> 2, t4 = lane & 3;
-  const int b = blockIdx.z, hkv = blockIdx.y / p.RG, r0 = (blockIdx.y - hkv * p.RG) * 16;
-  const int nrows = min(16, p.R - r0);
-  int cp = p.cache_pos ? __ldcg(p.cache_pos + b) : p.uniform_past;
-  if ((cp < 0 || cp > p.max_seq - p.q_len) && lane == 0) raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
-  cp = min(cp, p.max_seq);
-  const int L = min(max(cp + p.q_len, 0), p.max_seq);
+  const bool pre = (int)blockIdx.z == p.batch;
+  const int hkv = blockIdx.y / p.RG, r0 = (blockIdx.y - hkv * p.RG) * 16;
+  const int b = pre ? 0 : blockIdx.z, R = pre ? p.batch * p.R : p.R, groups = pre ? p.n_pre : p.own;
+  if ((int)blockIdx.x >= groups) return;  // (only where `pre` makes the grid wider)
+  const int nrows = min(16, R - r0);
+  int L = p.P, cp = 0;  // the first L keys; row r sees those up to cp + r / G, of the prefix all
+  if (!pre) {
+    cp = p.cache_pos ? __ldcg(p.cache_pos + b) : p.uniform_past;
+    if ((cp < 0 || cp > p.max_seq - p.q_len) && lane == 0) raise_device_error(p.err, LS_ERR_KV_OVERFLOW);
+    cp = min(cp, p.max_seq);
+    L = min(max(cp + p.q_len, 0), p.max_seq);
+  }
   const int blocks = (L + 15) / 16;
-  const int per = max((blocks + (int)gridDim.x - 1) / (int)gridDim.x, kStMinBlocks);
+  const int per = max((blocks + groups - 1) / groups, kStMinBlocks);
   const int blk0 = min((int)blockIdx.x * per, blocks), nb = min(per, blocks - blk0);
-  const size_t at = (((size_t)hkv * gridDim.z + b) * p.R + r0) * p.n_part + p.n_pre + blockIdx.x;  // row r: + r n_part
+  // row r: + r n_part
+  const size_t at = (((size_t)hkv * p.batch + b) * p.R + r0) * p.n_part + (pre ? 0 : p.n_pre) + blockIdx.x;
   if (nb <= 0) {
     if (lane < nrows) p.part_ml[at + (size_t)lane * p.n_part] = make_float2(-INFINITY, 0.f);
   } else {
-    const size_t base = ((size_t)b * p.Hkv + hkv) * p.max_seq * kTaHeadDim;
+    const size_t base = pre ? (size_t)hkv * p.prefix_cap * kTaHeadDim : ((size_t)b * p.Hkv + hkv) * p.max_seq * kTaHeadDim;
+    const __nv_bfloat16 *keys = pre ? p.k_prefix : p.k_cache, *values = pre ? p.v_prefix : p.v_cache;
     const uint32_t ring = smem_u32(sm), sq = ring + kStStages * 2 * kStTile;
 #pragma unroll
     for (int it = 0; it < 8; ++it) {  // the query rows, zeros behind the end; with the first tiles' copies
@@ -512,8 +527,8 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
         const int r = (lane >> 4) + 2 * it, j = (blk0 + n) * 16 + r;
         const bool ok = j < L;
         const size_t off = base + (size_t)(ok ? j : 0) * kTaHeadDim + (lane & 15) * 8;
-        cp_async16(st + ta_swz(r, lane & 15), p.k_cache + off, ok ? 16u : 0u);
-        cp_async16(st + kStTile + ta_swz(r, lane & 15), p.v_cache + off, ok ? 16u : 0u);
+        cp_async16(st + ta_swz(r, lane & 15), keys + off, ok ? 16u : 0u);
+        cp_async16(st + kStTile + ta_swz(r, lane & 15), values + off, ok ? 16u : 0u);
       }
     };
 #pragma unroll
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
     }
     int lim[2];  // last key the rows g8 and g8 + 8 see
 #pragma unroll
-    for (int hr = 0; hr < 2; ++hr) lim[hr] = g8 + 8 * hr < nrows ? cp + (r0 + g8 + 8 * hr) / p.G : -1;
+    for (int hr = 0; hr < 2; ++hr) lim[hr] = g8 + 8 * hr >= nrows ? -1 : pre ? L - 1 : cp + (r0 + g8 + 8 * hr) / p.G;
     uint32_t qa[8][4];
     float o[16][4];
 #pragma unroll
@@ -615,7 +630,7 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
             make_float2(o[nt][2 * hr], o[nt][2 * hr + 1]);
     }
   }
-  if (p.n_pre > 0 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+  if (p.behind && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
     grid_dep_wait();
 }
 
@@ -675,6 +690,7 @@ struct SpPlan {
 };
 
 constexpr int kSpMaxChunks = 32;
+constexpr int64_t kSpFewKeys = 2048;
 // kFull when the prompt rows alone give three quarters of the SMs a CTA (one
 // launch, nothing written in between); else the prefix is split over the SMs.
 static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int64_t prefix_len, int64_t max_seq) {
@@ -692,6 +708,12 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   // heads and 8192 shared keys, kKeys / kRows: 192 rows 34 / 37 us, 384 rows 53 / 56,
   // 768 rows 52 / 49.
   pl.mode = rows <= 512 ? kKeys : kRows;
+  // One row tile and a short prefix: its keys go to the strips' kernel, a launch less.
+  // us without / with, and with the host's time, 1 - 4 sequences of 4 rows: 64 keys
+  // 7.2 / 6.7 and 9.4 / 7.5, 300 keys 7.9 / 7.2 and 9.4 / 7.5, 2000 keys 9.6 / 8.6 and
+  // 9.9 / 9.3, 8192 keys 14.6 / 21.4.  8 sequences (two row tiles): 300 keys 8.2 / 9.1.
+  const bool few = rows <= 16 && prefix_len <= kSpFewKeys;
+  if (few) pl.mode = kFew;
   const int64_t per = pl.mode == kKeys ? kSpRows : 2 * kSpRows;
   pl.row_blocks = (int)((rows + per - 1) / per);
   // As many splits as fill the SMs once, of at least 128 keys each.
@@ -700,6 +722,8 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   if (splits < 1) splits = 1;
   if (splits > most) splits = most;
   pl.splits = prefix_len > 0 ? (int)splits : 0;
+  const int64_t few_splits = (std::min<int64_t>(prefix_len, kSpFewKeys) + 16 * kStMinBlocks - 1) / (16 * kStMinBlocks);
+  if (few) pl.splits = (int)few_splits;
   // Strip chunks: about 2048 warps in all (14 an SM, of which 7 fit at once).
   const int64_t strips = batch * hkv * ((q_len * g + 15) / 16);
   int64_t chunks = 2048 / strips;
@@ -707,7 +731,8 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   if (chunks > longest) chunks = longest;
   if (chunks > kSpMaxChunks) chunks = kSpMaxChunks;
   pl.chunks = chunks < 1 ? 1 : (int)chunks;
-  const int64_t groups = pl.splits + pl.chunks;
+  // (A longer prefix never needs less, although it may leave kFew.)
+  const int64_t groups = (rows <= 16 ? std::max<int64_t>(pl.splits, few_splits) : pl.splits) + pl.chunks;
   pl.ml_bytes = (hkv * rows * groups * 8 + 255) / 256 * 256;
   pl.bytes = pl.ml_bytes + hkv * rows * groups * kSpHeadDim * 4;
   return pl;
@@ -774,7 +799,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   p.scale_log2 = scale * 1.4426950408889634f;
   CUtensorMap kp, vp, kc, vc;
   int rc = LS_OK;
-  if (prefix_len > 0) {
+  if (prefix_len > 0 && pl.mode != kFew) {
     rc = make_map(&kp, k_prefix, hkv * prefix_cap, kSpHeadDim, kSpBox);
     if (!rc) rc = make_map(&vp, v_prefix, hkv * prefix_cap, kSpHeadDim, kSpBox);
   }
@@ -787,7 +812,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
                                    stream);
   }
   if (rc) return rc;
-  if (prefix_len > 0) {
+  if (prefix_len > 0 && pl.mode != kFew) {
     const dim3 grid((unsigned)pl.splits, (unsigned)pl.row_blocks, (unsigned)hkv);
     rc = pl.mode == kKeys ? launch_prefix_tc<kKeys>(kp, vp, kp, vp, p, grid, stream)
                           : launch_prefix_tc<kRows>(kp, vp, kp, vp, p, grid, stream);
@@ -807,13 +832,22 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   st.Hkv = p.Hkv;
   st.G = p.G;
   st.R = p.q_len * p.G;
+  const bool few = pl.mode == kFew && prefix_len > 0;
   st.RG = (st.R + 15) / 16;
+  st.k_prefix = static_cast<const __nv_bfloat16*>(k_prefix);
+  st.v_prefix = static_cast<const __nv_bfloat16*>(v_prefix);
+  st.batch = (int)batch;
+  st.P = p.P;
+  st.prefix_cap = p.prefix_cap;
+  st.own = pl.chunks;
+  st.behind = prefix_len > 0 && !few;
   st.max_seq = p.max_seq;
   st.n_pre = pl.splits;
   st.n_part = p.n_part;
   st.scale_log2 = p.scale_log2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)pl.chunks, (unsigned)(hkv * st.RG), (unsigned)batch);
+  cfg.gridDim = dim3((unsigned)(few && pl.splits > pl.chunks ? pl.splits : pl.chunks), (unsigned)(hkv * st.RG),
+                     (unsigned)(few ? batch + 1 : batch));
   cfg.blockDim = dim3(32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

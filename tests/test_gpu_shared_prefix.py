@@ -107,6 +107,22 @@ def test_wide_batches_and_prompts(batch, q_len, hq, hkv, prefix, slots):
     _check(batch, q_len, hq, hkv, prefix, lens, slots, cap=prefix + 13)
 
 
+@pytest.mark.parametrize("batch,q_len,hq,hkv", [(1, 1, 8, 8), (4, 1, 32, 8), (1, 4, 8, 2), (2, 2, 8, 2), (16, 1, 2, 2),
+                                                (5, 1, 6, 2), (17, 1, 2, 2)])
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 2047, 2048, 2049])
+def test_few_rows(batch, q_len, hq, hkv, prefix):
+    """Around the sizes at which the prefix goes to the strips' kernel; own strips shorter and longer than it."""
+    _check(batch, q_len, hq, hkv, prefix, [(37 * i) % (300 - q_len) for i in range(batch)], 300)
+    _check(batch, q_len, hq, hkv, prefix, [0] * batch, q_len)
+
+
+def test_workspace_grows_with_the_prefix():
+    for batch, q_len, hq, hkv in ((1, 1, 8, 8), (4, 1, 32, 8), (16, 1, 2, 2), (17, 1, 2, 2), (3, 5, 32, 8)):
+        need = [K.shared_prefix_attention_workspace_bytes(batch, q_len, hq, hkv, 128, p)
+                for p in (0, 1, 100, 500, 1000, 2047, 2048, 2049, 2100, 3000, 9000, 30000)]
+        assert need == sorted(need), (batch, q_len, need)
+
+
 def test_long_prefix():
     _check(4, 1, 16, 8, 70001, [3, 0, 50, 17], 64, cap=70003)
 
