@@ -15,19 +15,26 @@
 // bans outright are not read at all.  Where the vocabulary is no multiple of 8 the
 // groups are aligned in the flattened [m, vocab] array, not in the row, so that
 // these sizes take 16-byte accesses too, and a group's bits are cut from two
-// words.  The CTAs of a row leave one key each and a second, tiny kernel picks the
-// row's token and enters it into its state: no counters to zero, no order of
+// words.  The CTAs of a row leave one key each, of a value and the group of 8 that holds
+// it, and a second, small kernel finds the token in that group, meets it with the biased
+// ones and enters it into the row's state: no counters to zero, no order of
 // arrival, nothing that two captured graphs share.  (With a row as a cluster of
 // CTAs whose winners met in shared memory, 64 rows of 151936 took 17 us instead of
 // 10: clusters are placed slowly and wait for one another.)  What bounds it: for
 // few rows the chain bits -> logits, counts -> pick of dependent latencies; for
-// many, instruction issue, so a group is kept short: bits as bytes, one maximum
-// per group, seen and biased tokens one at a time.
+// many, instruction issue beside the loads, so a group is kept short: bits as bytes,
+// masks by byte permutes, a packed maximum and no index (161 -> 70 instructions a
+// group of 8 bf16 tokens), seen tokens one at a time.
+// Measured: 1 row of 151936 bf16 5.0 us (launch and latency), 32 rows of it under a
+// grammar of 300 tokens 7.3, 128 rows with everything and written logits 34 (3.5 TB/s).
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace lsb {
 
 constexpr int kTrThreads = 256;
+constexpr int kTrPickThreads = 128;
 
 constexpr int64_t kTrNoKey = INT64_MIN;  // below every argmax_key: a CTA without a candidate
 
@@ -46,37 +53,82 @@ struct TrParams {
   int V, W, bias_cap;
 };
 
-// 8 consecutive logits as loaded, and as fp32.
+// 8 consecutive logits as loaded; kept(): with -inf in place of the tokens whose bit is
+// clear, from which their maximum (NaN drops out) and their fp32 are taken.
 template <typename T>
 struct TrRaw {};
 template <>
 struct TrRaw<__nv_bfloat16> {
-  uint4 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ldg16(p); }  // 16-byte aligned
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {  // 16-byte aligned
+    const uint4 v = ldg16(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
   __device__ __forceinline__ void load(const __nv_bfloat16* p, int lo, int hi) {  // elements lo .. hi - 1 only
     uint32_t h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = j >= lo && j < hi ? (uint32_t)__bfloat16_as_ushort(p[j]) : 0u;
-    v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | h[2 * i + 1] << 16;
   }
-  __device__ __forceinline__ void get(float f[8]) const { unpack8(v, f); }
+  __device__ __forceinline__ float value(int j) const {
+    const uint32_t x = j & 4 ? (j & 2 ? w[3] : w[2]) : (j & 2 ? w[1] : w[0]);
+    return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
+  }
+  // Four bits become the sign bits of four bytes, and two byte permutes that repeat
+  // signs make 16-bit masks of them.
+  __device__ __forceinline__ TrRaw kept(uint32_t bits) const {
+    TrRaw r = *this;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t sign = ((bits >> 4 * i & 15u) * 0x10204080u) & 0x80808080u;
+      uint32_t m0, m1;
+      asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m0) : "r"(sign));
+      asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m1) : "r"(sign));
+      r.w[2 * i] = (w[2 * i] & m0) | (0xff80ff80u & ~m0);
+      r.w[2 * i + 1] = (w[2 * i + 1] & m1) | (0xff80ff80u & ~m1);
+    }
+    return r;
+  }
+  __device__ __forceinline__ float top() const {
+    __nv_bfloat162 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+    const float2 t = __bfloat1622float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+    return fmaxf(t.x, t.y);
+  }
+  __device__ __forceinline__ void get(float f[8]) const { unpack8(make_uint4(w[0], w[1], w[2], w[3]), f); }
 };
 template <>
 struct TrRaw<float> {
-  float4 a, b;
+  float f[8];
   __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const float4*>(p);
-    b = *reinterpret_cast<const float4*>(p + 4);
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
   }
   __device__ __forceinline__ void load(const float* p, int lo, int hi) {
-    float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = j >= lo && j < hi ? p[j] : 0.f;
-    a = make_float4(f[0], f[1], f[2], f[3]);
-    b = make_float4(f[4], f[5], f[6], f[7]);
   }
-  __device__ __forceinline__ void get(float f[8]) const {
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  __device__ __forceinline__ float value(int j) const {
+    float x = f[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e)
+      if (e == j) x = f[e];
+    return x;
+  }
+  __device__ __forceinline__ TrRaw kept(uint32_t bits) const {
+    TrRaw r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.f[j] = bits >> j & 1u ? f[j] : -INFINITY;
+    return r;
+  }
+  __device__ __forceinline__ float top() const {
+    return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  }
+  __device__ __forceinline__ void get(float o[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = f[j];
   }
 };
 
@@ -153,6 +205,7 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
     for (int u = 0; u < U; ++u) {
       const int g = gb + u * stride;
       sb[u] &= ab[u];
+      raw[u] = {};  // (a value in any case: what no bit keeps is masked, not unknown)
       if (ab[u] == 0u) continue;
       if (!VEC && row == (int)gridDim.y - 1 && g * 8 - a + 8 > p.V) raw[u].load(logits + g * 8, 0, p.V - (g * 8 - a));
       else raw[u].load(logits + g * 8);  // (the array does not end inside the group)
@@ -179,34 +232,21 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
     __syncthreads();
   }
   float best = -INFINITY;
-  int besti = 0x7fffffff, at = 0;  // at: where this thread's group of the batch's first tile has its bias bits
+  int bestg = 0x7fffffff, at = 0;  // at: where this thread's group of the batch's first tile has its bias bits
 #pragma unroll 1
   for (; gb < ngroups; at += U << lg) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int g = gb + u * stride;
       if (g >= ngroups) break;
-      float f[8];
-      raw[u].get(f);
-      // Few tokens are seen or biased: one at a time, not eight predicated divisions.
-#pragma unroll 1
-      for (uint32_t m = sb[u]; m; m &= m - 1u) {
-        const int j = __ffs(m) - 1, n = m == sb[u] ? n0[u] : counts[g * 8 + j];
-        float x = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e == j) x = f[e];
-        x = tr_penalise(x, rep, n, freq, pres);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e == j) f[e] = x;
-      }
-      if (ab[u] != 0xffu) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!(ab[u] >> j & 1u)) f[j] = -INFINITY;
-      }
+      // Seen tokens are few: one at a time beside the group's maximum, not eight
+      // predicated divisions.  Biased ones are the pick's.
+      const uint32_t bb = p.bias_cap ? bias_bits[at + (u << lg)] : 0u, keep = ab[u] & ~(sb[u] | bb);
+      TrRaw<T> kept = raw[u];
+      if (keep != 0xffu) kept = raw[u].kept(keep);
       if (out) {
+        float f[8];
+        kept.get(f);
         float* o = out + g * 8;
         if (VEC || (g * 8 >= a && g * 8 - a + 8 <= p.V)) {
           *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
@@ -217,24 +257,15 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
             if (g * 8 + j >= a && g * 8 - a + j < p.V) o[j] = f[j];
         }
       }
-      if (p.bias_cap) {  // biased tokens are left to the pick
-        const uint32_t bb = bias_bits[at + (u << lg)];
-        ab[u] &= ~bb;
-        if (bb) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (bb >> j & 1u) f[j] = -INFINITY;
-        }
+      float top = kept.top();
+#pragma unroll 1
+      for (uint32_t m = sb[u]; m; m &= m - 1u) {
+        const int j = __ffs(m) - 1;
+        const float x = tr_penalise(raw[u].value(j), rep, m == sb[u] ? n0[u] : counts[g * 8 + j], freq, pres);
+        if (out) out[g * 8 + j] = x;
+        if (!(bb >> j & 1u)) top = fmaxf(top, x);
       }
-      // The group's maximum (NaN drops out); a thread meets its tokens in order, so
-      // a later equal one does not win.  -inf counts while there is nothing else.
-      const float top = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-      if (top > best || (besti == 0x7fffffff && top == -INFINITY)) {
-        best = top;
-#pragma unroll
-        for (int j = 7; j >= 0; --j)
-          if (f[j] == top && (ab[u] >> j & 1u)) besti = g * 8 - a + j;
-      }
+      if (top > best) best = top, bestg = g;  // a thread meets its groups in order: the first of equals stays
     }
     gb += U * stride;
     if (gb >= ngroups) break;
@@ -244,67 +275,158 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, besti, o);
-    if (tr_better(ov, oi, best, besti)) best = ov, besti = oi;
+    const int og = __shfl_xor_sync(0xffffffffu, bestg, o);
+    if (tr_better(ov, og, best, bestg)) best = ov, bestg = og;
   }
-  if ((threadIdx.x & 31) == 0) bv[threadIdx.x >> 5] = best, bi[threadIdx.x >> 5] = besti;
+  if ((threadIdx.x & 31) == 0) bv[threadIdx.x >> 5] = best, bi[threadIdx.x >> 5] = bestg;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < nt / 32; ++w)
-      if (tr_better(bv[w], bi[w], best, besti)) best = bv[w], besti = bi[w];
-    p.keys[(size_t)row * ncta + c] = besti != 0x7fffffff ? argmax_key(best, besti) : kTrNoKey;
+      if (tr_better(bv[w], bi[w], best, bestg)) best = bv[w], bestg = bi[w];
+    p.keys[(size_t)row * ncta + c] = bestg != 0x7fffffff ? argmax_key(best, bestg) : kTrNoKey;
   }
 }
 
-// The row's token, one warp per row: its CTAs' keys against its biased tokens, which
-// are worked out here, one lane each, at their first place in the list (once a row
-// instead of once a CTA: 60 biases on 128 rows cost 13 us there).  record: into the
-// row's state.
-template <typename T>
-__global__ void __launch_bounds__(32) constrained_pick_kernel(TrParams p, int ncta, int record, int64_t* out_ids) {
-  grid_dep_wait();
-  grid_dep_launch();
-  const int row = blockIdx.x, lane = threadIdx.x;
-  int64_t key = kTrNoKey;
-  for (int i = lane; i < ncta; i += 32)
-    key = max(key, (int64_t)__ldcg(reinterpret_cast<const long long*>(p.keys) + (size_t)row * ncta + i));
-  if (p.bias_cap) {
-    const int* ids = p.bias_ids + (size_t)row * p.bias_cap;
-    const float* values = p.bias_values + (size_t)row * p.bias_cap;
-    const float rep = p.repetition ? p.repetition[row] : 1.f;
-    const float freq = p.frequency ? p.frequency[row] : 0.f;
-    const float pres = p.presence ? p.presence[row] : 0.f;
-    for (int k = lane; k < p.bias_cap; k += 32) {
-      const int v = ids[k];
-      if (v < 0 || v >= p.V) continue;
-      const size_t word = (size_t)row * p.W + (v >> 5), at = (size_t)row * p.V + v;
-      const bool free = !p.allowed || (p.allowed[word] >> (v & 31) & 1u);
-      const bool was = p.seen && (p.seen[word] >> (v & 31) & 1u);
-      float x = tr_value(static_cast<const T*>(p.logits)[at]);
-      const int n = was ? p.counts[at] : 0;
-      bool first = true;
-      float add = 0.f;  // its biases in list order
-#pragma unroll 4
-      for (int q = 0; q < p.bias_cap; ++q)
-        if (ids[q] == v) {
-          first = first && q >= k;
-          add = __fadd_rn(add, values[q]);
-        }
-      if (!free || !first) continue;
-      if (was) x = tr_penalise(x, rep, n, freq, pres);
-      x = __fadd_rn(x, add);
-      if (p.out_logits) p.out_logits[at] = x;
-      if (x == x) key = max(key, argmax_key(x, v));
-    }
-  }
+__device__ __forceinline__ int64_t tr_block_max(int64_t key, int64_t* warps) {  // of all kTrPickThreads threads
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) key = max(key, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)key, o));
-  if (lane != 0) return;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = key;
+  __syncthreads();
+  for (int w = 0; w < kTrPickThreads / 32; ++w) key = max(key, warps[w]);
+  return key;
+}
+
+// The row's token.  Its CTAs' keys name a value and the group of 8 that holds it; the
+// group's tokens are worked out again here and the best of them, lowest id first, meets
+// the biased tokens.  Those are worked out here, a thread each at their first place in
+// the list, the first 128 before the wait: they need nothing of the kernel before, and a
+// list of 60 took 8 us behind it.  Where no token is above -inf, one that is -inf itself
+// is looked for.  record: the pick into the row's state.
+template <typename T>
+__global__ void __launch_bounds__(kTrPickThreads) constrained_pick_kernel(TrParams p, int ncta, int record, int64_t* out_ids) {
+  constexpr int kStage = 512;
+  __shared__ __align__(16) int ids[kStage];
+  __shared__ float values[kStage];
+  __shared__ int64_t warps[kTrPickThreads / 32];
+  __shared__ int s_first;
+  __shared__ uint32_t s_biased;  // tokens of the winning group that have a bias
+  // The kernel before lets this one start only after every kernel before it is
+  // complete: logits, state and rules may be used at once, its keys after the wait.
+  grid_dep_launch();
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const size_t row_v = (size_t)row * p.V, row_w = (size_t)row * p.W;
+  const T* logits = static_cast<const T*>(p.logits) + row_v;
+  const int* bias_ids = p.bias_ids + (size_t)row * p.bias_cap;
+  const float* bias_values = p.bias_values + (size_t)row * p.bias_cap;
+  const float rep = p.repetition ? p.repetition[row] : 1.f;
+  const float freq = p.frequency ? p.frequency[row] : 0.f;
+  const float pres = p.presence ? p.presence[row] : 0.f;
+  // Token v without its biases, and whether it is allowed; all it needs is loaded at once.
+  auto token = [&](int v, bool& free) {
+    const uint32_t aw = p.allowed ? p.allowed[row_w + (v >> 5)] : 0xffffffffu, sw = p.seen ? p.seen[row_w + (v >> 5)] : 0u;
+    const int n = p.seen ? p.counts[row_v + v] : 0;
+    const float x = tr_value(logits[v]);
+    free = aw >> (v & 31) & 1u;
+    return sw >> (v & 31) & 1u ? tr_penalise(x, rep, n, freq, pres) : x;
+  };
+  auto unbiased = [&](int v) {
+    for (int k = 0; k < p.bias_cap; ++k)
+      if (bias_ids[k] == v) return false;
+    return true;
+  };
+  // Place k of the list: its token if this is the token's first place and it is allowed, else -1.
+  auto biased = [&](int k, float& x) {
+    int v = k < p.bias_cap ? bias_ids[k] : -1;
+    if (v >= p.V) v = -1;
+    bool free = false, first = true;
+    x = v >= 0 ? token(v, free) : 0.f;
+    float add = 0.f;  // its biases in list order
+    for (int q0 = 0; q0 < p.bias_cap; q0 += kStage) {
+      const int n = min(kStage, p.bias_cap - q0);
+      __syncthreads();
+      for (int q = tid; q < ((n + 3) & ~3); q += kTrPickThreads) {
+        ids[q] = q < n ? bias_ids[q0 + q] : -1;
+        values[q] = q < n ? bias_values[q0 + q] : 0.f;
+      }
+      __syncthreads();
+      for (int q = 0; q < n; q += 4) {
+        const int4 four = *reinterpret_cast<const int4*>(ids + q);
+        const int id[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (id[e] == v) {
+            first = first && q0 + q + e >= k;
+            add = __fadd_rn(add, values[q + e]);
+          }
+      }
+    }
+    x = __fadd_rn(x, add);
+    return free && first ? v : -1;
+  };
+  int64_t key = kTrNoKey;
+  float x = 0.f;
+  int v = p.bias_cap ? biased(tid, x) : -1;
+  grid_dep_wait();
+  for (int k = tid;;) {  // (with the block: biased() has barriers)
+    if (v >= 0) {
+      if (p.out_logits) p.out_logits[row_v + v] = x;
+      if (x == x) key = max(key, argmax_key(x, v));
+    }
+    k += kTrPickThreads;
+    if (k - tid >= p.bias_cap) break;
+    v = biased(k, x);
+  }
+  int64_t top = kTrNoKey;
+  for (int i = tid; i < ncta; i += kTrPickThreads)
+    top = max(top, (int64_t)__ldcg(reinterpret_cast<const long long*>(p.keys) + (size_t)row * ncta + i));
+  if (tid == 0) s_biased = 0u;
+  top = tr_block_max(top, warps);
+  if (top != kTrNoKey) {
+    const int a = p.V % 8 ? (int)(row_v & 7) : 0;
+    const int v0 = (int)argmax_key_id(top) * 8 - a;
+    for (int k = tid; k < p.bias_cap; k += kTrPickThreads) {
+      const unsigned d = (unsigned)(bias_ids[k] - v0);
+      if (d < 8u) atomicOr(&s_biased, 1u << d);
+    }
+    bool free = false;
+    v = v0 + tid;
+    if (tid < 8 && v >= 0 && v < p.V) x = token(v, free);
+    __syncthreads();
+    if (free && x == x && !(s_biased >> tid & 1u)) key = max(key, argmax_key(x, v));
+    key = tr_block_max(key, warps);
+  } else {
+    key = tr_block_max(key, warps);
+    // Nothing above -inf without a bias.  Unless a biased token is, a word of tokens a
+    // thread, until a block of words holds one that is allowed, not biased and -inf.
+    for (int w0 = 0; w0 < p.W && key <= argmax_key(-INFINITY, 0); w0 += kTrPickThreads) {
+      if (tid == 0) s_first = p.V;
+      __syncthreads();
+      const int w = w0 + tid;
+      uint32_t free = w >= p.W ? 0u : p.allowed ? p.allowed[row_w + w] : 0xffffffffu;
+      for (; free; free &= free - 1u) {
+        const int t = w * 32 + __ffs(free) - 1;
+        if (t >= p.V) break;
+        bool is_free;
+        if (token(t, is_free) == -INFINITY && unbiased(t)) {
+          atomicMin(&s_first, t);
+          break;
+        }
+      }
+      __syncthreads();
+      if (s_first < p.V) {
+        key = max(key, argmax_key(-INFINITY, s_first));
+        break;
+      }
+      __syncthreads();
+    }
+  }
+  if (tid != 0) return;
   const int64_t id = key == kTrNoKey ? -1 : argmax_key_id(key);
   out_ids[row] = id;
   if (record && id >= 0) {  // atomics only so that nothing waits for the old value
-    atomicAdd(p.counts + (size_t)row * p.V + id, 1);
-    atomicOr(p.seen + (size_t)row * p.W + id / 32, 1u << (id & 31));
+    atomicAdd(p.counts + row_v + id, 1);
+    atomicOr(p.seen + row_w + id / 32, 1u << (id & 31));
   }
 }
 
@@ -332,11 +454,20 @@ __global__ void __launch_bounds__(kTrThreads) token_stats_add_kernel(const int64
 namespace lsb_host {
 using namespace lsb;
 
-// CTAs of a row: a group per thread while that does not fill the GPU several times,
-// else four (those that a thread has in flight).
+// CTAs of a row: a group per thread while that does not fill the GPU several times;
+// then four groups (those a thread has in flight); from 16 groups a thread for one wave
+// of CTAs (four an SM) on, that wave: 128 rows of 151936 bf16 with penalties, biases and
+// masks, logits written, four groups / one wave: 37.8 / 33.9 us, 64 rows (which make 8)
+// 14.2 / 15.7.  At most 64 tiles a CTA: their bias bits are 16 KB.
 static int64_t tr_ctas(int64_t m, int64_t vocab) {
-  const int64_t tiles = (vocab + 14) / 8 / kTrThreads + 1;
-  return m * tiles <= 8 * (int64_t)sm_count() ? tiles : (tiles + 3) / 4;
+  const int64_t tiles = (vocab + 14) / 8 / kTrThreads + 1, sms = sm_count();
+  if (m * tiles <= 8 * sms) return tiles;
+  int64_t per = 4;
+  if (m * tiles >= 16 * 4 * sms) {
+    const int64_t ctas = std::max<int64_t>(4 * sms / m, 1);
+    per = std::min<int64_t>((tiles + ctas - 1) / ctas, 64);
+  }
+  return (tiles + per - 1) / per;
 }
 constexpr int64_t kTrMaxVocab = 1 << 20;
 
@@ -356,7 +487,7 @@ static int launch_constrained_argmax(const TrParams& p, int64_t m, int record, i
   cudaError_t e = cudaLaunchKernelEx(&cfg, constrained_argmax_kernel<T, VEC>, p);
   if (e == cudaSuccess) {
     cfg.gridDim = dim3((unsigned)m);
-    cfg.blockDim = dim3(32);
+    cfg.blockDim = dim3(kTrPickThreads);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, constrained_pick_kernel<T>, p, (int)ncta, record, out_ids);
   }

@@ -148,6 +148,80 @@ def test_a_far_minus_infinity_behind_nan():
         assert K.constrained_argmax(logits).tolist() == [8500, 4000, -1]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [40, 9000, 9003])
+def test_rows_without_a_finite_candidate(dtype, vocab):
+    """Only -inf left: the lowest token that is allowed and -inf, biased or not; a biased one above -inf wins."""
+    inf, nan = float("inf"), float("nan")
+    m = 8
+    logits = torch.full((m, vocab), nan, device=DEV, dtype=dtype)
+    allowed = torch.ones(m, vocab, dtype=torch.bool, device=DEV)
+    ids = torch.full((m, 2), -1, device=DEV, dtype=torch.int32)
+    vals = torch.zeros(m, 2, device=DEV)
+    want = []
+    logits[0, vocab - 2] = -inf  # behind NaN
+    want.append(vocab - 2)
+    logits[1] = -inf  # the lowest is banned
+    allowed[1, :7] = False
+    want.append(7)
+    logits[2] = 5.0  # nothing allowed
+    allowed[2] = False
+    want.append(-1)
+    logits[3] = 1.0  # biased to -inf, the only one allowed
+    allowed[3] = False
+    allowed[3, 33] = True
+    ids[3, 0], vals[3, 0] = 33, -inf
+    want.append(33)
+    logits[4] = -inf  # the lowest one is biased, which leaves it -inf
+    ids[4, 0], vals[4, 0] = 0, 3.0
+    want.append(0)
+    logits[5] = -inf  # one of them is forced above
+    ids[5, 1], vals[5, 1] = 38, inf  # -inf + inf: NaN, no candidate
+    ids[5, 0], vals[5, 0] = 0, inf
+    want.append(1)
+    logits[6] = -inf
+    logits[6, 20] = -3.0  # finite, but biased away
+    ids[6, 0], vals[6, 0] = 20, -inf
+    want.append(0)
+    logits[7] = 2.0  # every token of the largest group but one is biased down
+    logits[7, 8:16] = 4.0
+    ids7 = torch.tensor([8, 9], device=DEV, dtype=torch.int32)
+    ids[7], vals[7] = ids7, torch.tensor([-1.0, -3.0], device=DEV)
+    want.append(10)
+    out = torch.empty(m, vocab, device=DEV)
+    got = K.constrained_argmax(logits, allowed=pack(allowed), bias_ids=ids, bias_values=vals, out_logits=out)
+    assert got.tolist() == want
+    ref = logits.float()
+    for r in range(m):
+        for k in range(2):
+            if ids[r, k] >= 0:
+                ref[r, ids[r, k].item()] += vals[r, k]
+    ref[~allowed] = -inf
+    assert torch.equal(torch.nan_to_num(out, nan=7e4), torch.nan_to_num(ref, nan=7e4))
+
+
+@pytest.mark.parametrize("cap", [1, 127, 128, 129, 512, 513, 1100])
+@pytest.mark.parametrize("vocab", [700, 5003])
+def test_long_bias_lists(cap, vocab):
+    """Lists longer than a stage and than the pick's threads, with repeated tokens far apart."""
+    g = torch.Generator(device=DEV).manual_seed(cap)
+    m = 3
+    logits = torch.randn(m, vocab, generator=g, device=DEV)
+    ids = torch.randint(-3, vocab + 3, (m, cap), generator=g, device=DEV, dtype=torch.int32)
+    if cap > 2:
+        ids[:, cap - 1] = ids[:, 0]
+        ids[1] = 5  # one token only
+    vals = torch.randint(-8, 9, (m, cap), generator=g, device=DEV).float() / 4  # (sums of quarters: exact)
+    out = torch.empty(m, vocab, device=DEV)
+    got = K.constrained_argmax(logits, bias_ids=ids, bias_values=vals, out_logits=out)
+    steps = torch.zeros(m, vocab, device=DEV)
+    inside = (ids >= 0) & (ids < vocab)
+    steps.scatter_add_(1, ids.clamp(0, vocab - 1).long(), vals * inside)
+    want = logits + steps
+    assert torch.equal(out, want)
+    assert torch.equal(got, torch.stack([(r == r.max()).nonzero()[0, 0] for r in want]))
+
+
 def test_a_bias_of_minus_infinity_bans_and_plus_infinity_forces():
     logits = torch.arange(100, device=DEV, dtype=torch.float32).expand(2, 100).contiguous()
     ids = torch.tensor([[99, 98], [3, 99]], device=DEV, dtype=torch.int32)
