@@ -458,7 +458,8 @@ int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const 
  *   bias_ids, bias_values  [m, bias_cap]; ids outside the vocabulary are skipped
  *   allowed   uint32 [m, ceil(vocab / 32)] or NULL (every token)
  *   record    count the picked token and mark it seen
- * NaN logits are never picked; vocab <= 2^20; the workspace needs no filling.
+ * NaN logits are never picked (-1 where nothing else is allowed); vocab <= 2^20,
+ * bias_cap <= 2^14; the workspace needs no filling.
  * ls_token_stats_add enters ids [batch, len]
  * (negative: padding) into seen and, unless counts is NULL (a prompt), counts;
  * an id past the vocabulary raises LS_ERR_INVALID_ARGUMENT in the device error

@@ -470,6 +470,7 @@ static int64_t tr_ctas(int64_t m, int64_t vocab) {
   return (tiles + per - 1) / per;
 }
 constexpr int64_t kTrMaxVocab = 1 << 20;
+constexpr int64_t kTrMaxBiases = 1 << 14;  // the pick compares each with each: about 10 ms there, and four times that for twice as many
 
 template <typename T, bool VEC>
 static int launch_constrained_argmax(const TrParams& p, int64_t m, int record, int64_t* out_ids, cudaStream_t stream) {
@@ -525,6 +526,8 @@ int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t
   LS_REQUIRE((bias_ids == nullptr) == (bias_values == nullptr) && (bias_ids != nullptr) == (bias_cap > 0) &&
                  bias_cap >= 0 && bias_cap < (1ll << 31),
              LS_ERR_INVALID_ARGUMENT, "ls_constrained_argmax: bias_ids, bias_values and bias_cap come together");
+  LS_REQUIRE(bias_cap <= kTrMaxBiases, LS_ERR_UNSUPPORTED_SHAPE, "ls_constrained_argmax: %lld biases a row, beyond %lld",
+             (long long)bias_cap, (long long)kTrMaxBiases);
   LS_REQUIRE(aligned16(logits) && aligned16(out_logits), LS_ERR_MISALIGNED,
              "ls_constrained_argmax: logits must be 16-byte aligned");
   LS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, LS_ERR_WORKSPACE,

@@ -68,6 +68,12 @@ def test_constrained_argmax(lib):
         _refused(fn, args, changes, code)
 
 
+def test_constrained_argmax_bounds_its_bias_lists(lib):
+    """Every bias meets every other of its row: a list that would keep the GPU for long is refused."""
+    args = [P, 0, 4, 151936, None, None, None, None, None, P, P, (1 << 14) + 1, None, 0, P, None, P, 1 << 40, None]
+    assert lib.ls_constrained_argmax(*args) == 2, nat.last_error()
+
+
 def test_front_end_refuses_cpu_tensors():
     x = torch.zeros(2, 256, dtype=torch.bfloat16)
     kv = torch.zeros(2, 16, 128, dtype=torch.bfloat16)
