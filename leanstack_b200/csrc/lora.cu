@@ -129,7 +129,7 @@ __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2]
       }
   };
   int k = k0;
-#pragma unroll (MT * 2 + NT <= 4 ? 4 : 2)
+#pragma unroll 4
   for (; k + 32 <= k1; k += step) {
     const int kk = k + t4 * 8;
     uint4 xv[MT][2], av[NT];
