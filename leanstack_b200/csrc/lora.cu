@@ -26,6 +26,10 @@
 // What bounds it: memory -- A and B of the adapters in use for short sequences
 // (where a few MB are latency), x and the fp32 output for prompts.  Tensor cores of
 // the tcgen05 kind would wait: 2 r flops per byte of x.
+// Measured: 1 token 2560 -> 6144 at rank 16 5.6 us (launch, three dependent loads, a
+// cluster's exchange), 32 tokens with an adapter each 2560 -> 19456 11.4 us (1.5 TB/s),
+// 7 prompts of 701 tokens 2560 -> 6144 at rank 32 39.9 us (3.6 TB/s: 13 of it shrink
+// at 1.9, the rest writes the output).
 #include "mma_sync.cuh"
 
 namespace lsb {
@@ -35,7 +39,8 @@ constexpr int kLoWarps = 4;
 constexpr int kLoOneRanks = 64;   // of the one-launch kernel (its sums: 16 tokens x ranks of every warp)
 constexpr int kLoWindow = 1024;   // sequences among which equal adapters share a CTA
 constexpr int kLoPrompt = 16;     // q_len from which a CTA takes tokens of one sequence
-constexpr int kLoTile = 128;      // shrink: tokens of a prompt CTA (32 a warp)
+constexpr int kLoTile = 128;      // shrink: tokens of a prompt CTA (32 a pair of warps)
+constexpr int kLoPromptThreads = 256;
 constexpr int kLoRanks = 16;      // shrink: ranks of a CTA, at most (16 x 5 tokens at rank 64: 13.6 us; all 64: 14.7)
 constexpr int kLoRanksPrompt = 32;
 constexpr int kLoTileOut = 64;    // expand: tokens of a prompt CTA (16 a warp)
@@ -174,13 +179,13 @@ __device__ __forceinline__ void st_cluster(float* local, int cta, float v) {
 }
 
 // Elements [0, n) of the cluster's CTAs' partials, added in split order; CTA c of
-// them takes every ncta-th run of kLoThreads elements and hands its sums to store(i, v).
-template <typename Store>
+// them takes every ncta-th run of THREADS elements and hands its sums to store(i, v).
+template <int THREADS, typename Store>
 __device__ __forceinline__ void lora_join_splits(const float* part, int n, Store store) {
   const int c = blockIdx.x, ncta = gridDim.x;  // the cluster is the grid's x extent
   if (ncta > 1) cluster_sync();
   else __syncthreads();
-  for (int i = c * kLoThreads + threadIdx.x; i < n; i += ncta * kLoThreads) {
+  for (int i = c * THREADS + threadIdx.x; i < n; i += ncta * THREADS) {
     float v = 0.f;
     if (ncta == 1) {
       v = part[i];
@@ -228,19 +233,20 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
     const int t = i / (NT * 8), r = i % (NT * 8);
     part[i] = (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
   }
-  lora_join_splits(part, 16 * NT * 8, [&](int i, float v) {
+  lora_join_splits<kLoThreads>(part, 16 * NT * 8, [&](int i, float v) {
     const int t = i / (NT * 8), r = i % (NT * 8);
     if (t < tokens && r < ranks) p.u[(size_t)token(t) * p.R + r0 + r] = v;
   });
 }
 
-// Prompts: a warp takes 32 tokens over the whole k range of the CTA.
+// Prompts: two warps take 32 tokens, each every other step of the CTA's k range.
 template <int NT>
-__global__ void __launch_bounds__(kLoThreads) lora_shrink_prompt_kernel(LoraParams p) {
+__global__ void __launch_bounds__(kLoPromptThreads) lora_shrink_prompt_kernel(LoraParams p) {
   __shared__ __align__(16) float part[kLoTile * NT * 8];
   grid_dep_wait();
   grid_dep_launch();
-  const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
+  const int b = blockIdx.z, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+  const int warp = threadIdx.x >> 5 & 3, odd = threadIdx.x >> 7;
   const int id = lora_adapter(p, b);
   if (id < 0) return;
   const int groups = (p.R + kLoRanksPrompt - 1) / kLoRanksPrompt, t0 = blockIdx.y / groups * kLoTile, i0 = t0 + warp * 32;
@@ -255,16 +261,23 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_prompt_kernel(LoraPara
       xr[i][h] = p.x + ((size_t)b * p.q_len + min(t, p.q_len - 1)) * p.K;
     }
   float acc[2][NT][4] = {};
-  lora_dot<2, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0, k1, 32, acc);
+  lora_dot<2, NT>(xr, p.a + ((size_t)id * p.R + r0) * p.K, p.K, ranks, k0 + odd * 32, k1, 64, acc);
+  for (int half = 1; half >= 0; --half) {  // the odd steps' warp stores its sums, the other adds its own
+    if (odd == half) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        *reinterpret_cast<float2*>(part + (warp * 32 + i * 16 + h * 8 + g8) * (NT * 8) + j * 8 + 2 * t4) =
-            make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
-  lora_join_splits(part, kLoTile * NT * 8, [&](int i, float v) {
+          for (int j = 0; j < NT; ++j) {
+            float2* to = reinterpret_cast<float2*>(part + (warp * 32 + i * 16 + h * 8 + g8) * (NT * 8) + j * 8 + 2 * t4);
+            const float2 had = half ? make_float2(0.f, 0.f) : *to;
+            *to = make_float2(had.x + acc[i][j][2 * h], had.y + acc[i][j][2 * h + 1]);
+          }
+    }
+    __syncthreads();
+  }
+  lora_join_splits<kLoPromptThreads>(part, kLoTile * NT * 8, [&](int i, float v) {
     const int t = t0 + i / (NT * 8), r = i % (NT * 8);
     if (t < p.q_len && r < ranks) p.u[((size_t)b * p.q_len + t) * p.R + r0 + r] = v;
   });
@@ -576,7 +589,7 @@ static int launch_lora(LoraParams p, cudaStream_t stream) {
   const dim3 gs = prompt ? dim3((unsigned)p.splits, tiles(kLoTile) * groups, (unsigned)p.batch)
                          : dim3((unsigned)p.splits, (unsigned)p.batch, groups);
   const dim3 ge = prompt ? dim3(nb, tiles(kLoTileOut), (unsigned)p.batch) : dim3(nb, (unsigned)p.batch);
-  cudaError_t e = launch_lora_kernel(shrink, gs, (unsigned)p.splits, p, stream);
+  cudaError_t e = launch_lora_kernel(shrink, gs, (unsigned)p.splits, p, stream, prompt ? kLoPromptThreads : kLoThreads);
   if (e == cudaSuccess) e = launch_lora_kernel(expand, ge, 1, p, stream);
   return e == cudaSuccess ? LS_OK : set_error(LS_ERR_CUDA, "lora_delta launch: %s", cudaGetErrorString(e));
 }
