@@ -74,14 +74,14 @@ __device__ __forceinline__ int lora_adapter(const LoraParams& p, int b) {
 // every 16 / q_len works for itself and those up to the next such.  Returns their number
 // (0: b is not such a first); `members` holds their indices, in order.
 template <int WARPS = kLoWarps>
-__device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, int (&members)[16]) {
+__device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, int first, int (&members)[16]) {
   __shared__ int s_before[WARPS], s_from[WARPS];
   const int w0 = b / kLoWindow * kLoWindow, w1 = min(w0 + kLoWindow, p.batch), most = 16 / p.q_len;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int before = 0, n = 0;
   for (int i0 = w0; i0 < w1; i0 += WARPS * 32) {
     const int i = i0 + threadIdx.x;
-    const bool same = i < w1 && p.ids[i] == id;
+    const bool same = i < w1 && (i0 == w0 ? first : p.ids[i]) == id;
     const uint32_t vote = __ballot_sync(0xffffffffu, same && i < b), from = __ballot_sync(0xffffffffu, same && i >= b);
     if (lane == 0) {
       s_before[warp] = __popc(vote);
@@ -99,6 +99,12 @@ __device__ __forceinline__ int lora_group(const LoraParams& p, int b, int id, in
     __syncthreads();
   }
   return before % most ? 0 : min(n, most);
+}
+
+// What lora_group compares first, loaded beside the id that it compares with.
+__device__ __forceinline__ int lora_first(const LoraParams& p, int b) {
+  const int i = b / kLoWindow * kLoWindow + threadIdx.x;
+  return i < p.batch ? p.ids[i] : -1;
 }
 
 // The lines of `bytes` bytes into L2, while the previous kernel is still at work.
@@ -134,7 +140,7 @@ __device__ __forceinline__ void lora_dot(const __nv_bfloat16* const (&xr)[MT][2]
       }
   };
   int k = k0;
-#pragma unroll 4
+#pragma unroll (NT <= 4 ? 4 : 2)  // (64 ranks: 140 registers with 4 leave an SM one CTA, 32 sequences 23 us instead of 15)
   for (; k + 32 <= k1; k += step) {
     const int kk = k + t4 * 8;
     uint4 xv[MT][2], av[NT];
@@ -212,9 +218,9 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraParams p) {
   grid_dep_wait();
   grid_dep_launch();
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
-  const int id = lora_adapter(p, b);
+  const int first = lora_first(p, b), id = lora_adapter(p, b);
   if (id < 0) return;
-  const int tokens = lora_group(p, b, id, members) * p.q_len;
+  const int tokens = lora_group(p, b, id, first, members) * p.q_len;
   if (!tokens) return;  // the whole cluster
   const int k0 = blockIdx.x * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
   const int r0 = blockIdx.z * kLoRanks, ranks = min(kLoRanks, p.R - r0);
@@ -319,47 +325,63 @@ struct LoraU {
   }
 };
 
-// Outputs [n0, n1) of 16 tokens, 16 at a time, `step` apart; a lane's four are
-// neighbours: column 2 t4 + e of product j is output 4 t4 + 2 j + e.
+// The rows of b of outputs n .. n + 15 as two fragments a step; a lane's four outputs
+// are neighbours: column 2 t4 + e of product j is output 4 t4 + 2 j + e.
 template <int KS>
-__device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS>& u, int id, const int (&tok)[2], int n0,
-                                             int n1, int step) {
-  const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-  const __nv_bfloat16* b = p.b + (size_t)id * p.N * p.R;
-  const float scale = p.scaling[id];
-#pragma unroll (KS == 1 ? 8 : 4)
-  for (int n = n0; n < n1; n += step) {
-    uint2 bv[2][KS];
+struct LoraB {
+  uint2 v[2][KS];
+  __device__ __forceinline__ void load(const __nv_bfloat16* b, int n, int n1, int R) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = n + (g8 >> 1) * 4 + j * 2 + (g8 & 1);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int k = s * 16 + t4 * 4;
-        bv[j][s] = row < n1 && k < p.R ? __ldg(reinterpret_cast<const uint2*>(b + (size_t)row * p.R + k)) : make_uint2(0u, 0u);
+        v[j][s] = row < n1 && k < R ? __ldg(reinterpret_cast<const uint2*>(b + (size_t)row * R + k)) : make_uint2(0u, 0u);
       }
     }
-    float acc[2][4] = {};
+  }
+};
+
+// Outputs n .. n + 15 of 16 tokens.
+template <int KS>
+__device__ __forceinline__ void lora_store(const LoraParams& p, const LoraU<KS>& u, const LoraB<KS>& b, float scale,
+                                           const int (&tok)[2], int n, int n1) {
+  const int t4 = threadIdx.x & 3;
+  float acc[2][4] = {};
 #pragma unroll
-    for (int q = 2; q >= 0; --q)  // the small parts first
+  for (int q = 2; q >= 0; --q)  // the small parts first
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mma_bf16(acc[j], u.f[s][q], bv[j][s].x, bv[j][s].y);
-    if (n + t4 * 4 < n1) {
+      for (int j = 0; j < 2; ++j) mma_bf16(acc[j], u.f[s][q], b.v[j][s].x, b.v[j][s].y);
+  if (n + t4 * 4 >= n1) return;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (tok[h] < 0) continue;
-        float4* o = reinterpret_cast<float4*>(p.out + (size_t)tok[h] * p.N + n + t4 * 4);
-        float4 v = make_float4(acc[0][2 * h] * scale, acc[0][2 * h + 1] * scale, acc[1][2 * h] * scale,
-                               acc[1][2 * h + 1] * scale);
-        if (p.accumulate) {
-          const float4 w = *o;
-          v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
-        }
-        *o = v;
-      }
+  for (int h = 0; h < 2; ++h) {
+    if (tok[h] < 0) continue;
+    float4* o = reinterpret_cast<float4*>(p.out + (size_t)tok[h] * p.N + n + t4 * 4);
+    float4 v = make_float4(acc[0][2 * h] * scale, acc[0][2 * h + 1] * scale, acc[1][2 * h] * scale,
+                           acc[1][2 * h + 1] * scale);
+    if (p.accumulate) {
+      const float4 w = *o;
+      v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
     }
+    *o = v;
+  }
+}
+
+// Outputs [n0, n1) of 16 tokens, 16 at a time, `step` apart.
+template <int KS>
+__device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS>& u, int id, const int (&tok)[2], int n0,
+                                             int n1, int step) {
+  const __nv_bfloat16* b = p.b + (size_t)id * p.N * p.R;
+  const float scale = p.scaling[id];
+#pragma unroll (KS == 1 ? 8 : 4)
+  for (int n = n0; n < n1; n += step) {
+    LoraB<KS> f;
+    f.load(b, n, n1, p.R);
+    lora_store<KS>(p, u, f, scale, tok, n, n1);
   }
 }
 
@@ -384,7 +406,7 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
     grid_dep_wait();
     return;
   }
-  const int tokens = lora_group(p, b, id, members) * p.q_len;
+  const int tokens = lora_group(p, b, id, lora_first(p, b), members) * p.q_len;
   if (tokens > 0) lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
   grid_dep_wait();
   if (!tokens) return;
@@ -440,14 +462,15 @@ __global__ void __launch_bounds__(THREADS) lora_one_kernel(LoraParams p) {
   const int b = blockIdx.y, c = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
   const int n0 = min(c * p.n_block, p.N), n1 = min(n0 + p.n_block, p.N);
-  const int id = lora_adapter(p, b);
+  const int first = lora_first(p, b), id = lora_adapter(p, b);
   if (id < 0) {  // the whole cluster
     if (!p.accumulate) lora_zeros(p, b * p.q_len, p.q_len, n0, n1);
     return;
   }
-  const int tokens = lora_group<WARPS>(p, b, id, members) * p.q_len;
+  const int tokens = lora_group<WARPS>(p, b, id, first, members) * p.q_len;
   if (!tokens) return;
-  lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
+  const __nv_bfloat16* pb = p.b + (size_t)id * p.N * p.R;
+  lora_prefetch(pb + (size_t)n0 * p.R, (n1 - n0) * p.R * 2);
   const int k0 = c * p.k_chunk, k1 = min(k0 + p.k_chunk, p.K);
   const __nv_bfloat16* xr[1][2];
   int tok[2];
@@ -479,6 +502,13 @@ __global__ void __launch_bounds__(THREADS) lora_one_kernel(LoraParams p) {
     for (int w = 0; w < WARPS / 2; ++w) v += red[w][i / RP][i % RP];
     part[i] = v;
   }
+  // The first outputs' rows of b, while the CTAs exchange their sums.
+  constexpr int kPre = KS == 1 ? 2 : 1;
+  const int nw = n0 + warp * 16;
+  LoraB<KS> pre[kPre];
+#pragma unroll
+  for (int q = 0; q < kPre; ++q) pre[q].load(pb, nw + q * 16 * WARPS, n1, p.R);
+  const float scale = p.scaling[id];
   cluster_sync();
   for (int i = c * (2 * RP) + threadIdx.x; i < (c + 1) * (2 * RP); i += THREADS) {
     float w[8], v = 0.f;
@@ -492,7 +522,9 @@ __global__ void __launch_bounds__(THREADS) lora_one_kernel(LoraParams p) {
   cluster_sync();  // (and no CTA reads or writes another's memory any more)
   LoraU<KS> u;
   u.split(p.R, [&](int h, int k) { return *reinterpret_cast<const float4*>(&sum[g8 + 8 * h][k]); });
-  lora_outputs<KS>(p, u, id, tok, n0 + warp * 16, n1, 16 * WARPS);
+#pragma unroll
+  for (int q = 0; q < kPre; ++q) lora_store<KS>(p, u, pre[q], scale, tok, nw + q * 16 * WARPS, n1);
+  lora_outputs<KS>(p, u, id, tok, nw + kPre * 16 * WARPS, n1, 16 * WARPS);
 }
 
 }  // namespace lsb
