@@ -42,6 +42,12 @@
 //   * kFull: a prompt's rows.  A CTA owns 256 rows of one (sequence, kv head)
 //     and walks the prefix tiles, then the sequence's own tiles with the causal
 //     mask, and writes the finished rows: no partials, no join.
+//
+// Measured with 32 / 8 heads, all kernels together: 32 sequences behind 8192 keys, 372
+// own ones each, 26.6 us (83 MB, 3.1 TB/s: from release to first tile 2.4 us, tiles 5.7,
+// epilogue 2, then the last strips and the join); 13 x 5 rows (16 / 8 heads) behind 5003
+// keys 23.4 us; 6 prompts of 384 behind 8192 keys 293 us (1088 TFLOP/s: scores of 64 keys
+// keep the tensor pipe waiting for shared memory); 2 sequences behind 300 keys 6.0 us.
 #include <algorithm>
 
 #include "mma_sync.cuh"
@@ -636,7 +642,8 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
 
 // Join of a row's key groups: one warp per row (kv head, token, group member) and
 // half of its dims, a lane two of them.  The groups' weights e^(m_g - M) sit in
-// the lanes, their O is read 32 groups at a time.
+// the lanes, their O is read 32 groups at a time.  14 MB of partials in 3 us beside
+// the launch: latency.
 constexpr int kSpJoinWarps = 4;
 __global__ void __launch_bounds__(kSpJoinWarps * 32) prefix_join_kernel(const float* part_o, const float2* part_ml,
                                                                         int n_part, int rows, int G, int Hq,

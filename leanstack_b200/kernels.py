@@ -4,6 +4,9 @@ Each function takes CUDA tensors, checks dtype / device / layout, and enqueues
 the kernel on torch's current stream.  Outputs are written into caller tensors
 when given (the engine passes its resident arenas) and allocated otherwise (the
 reference-style dispatch helpers return fresh tensors, as the reference does).
+The calls on up to sixteen tensors ask the C++ front end first
+(``csrc/torch_front.cpp``), which takes those whose operands are plainly right;
+the checks here see the others.
 """
 
 from __future__ import annotations
