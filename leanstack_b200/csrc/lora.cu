@@ -15,8 +15,9 @@
 //     memory and are added in split order (left to the expand kernel, every one of
 //     its CTAs added them again: 20 us of 30 at rank 64 and 16 splits).
 //   * Expand: u keeps its 24 bits as a sum of three bf16 (8 bits each), three
-//     products per step; the outputs of a lane are four neighbours, one 16-byte
-//     store a row.
+//     products per step.  Up to 8 tokens in a tile: outputs are the rows, tokens the
+//     columns, half the products of the other way round (32 tokens with an adapter each
+//     to 19456 outputs: 10.8 us instead of 11.7).  A lane's outputs are neighbours.
 // Two launches, or one in which a cluster does both halves of a tile (lora_one_launch).
 // Short sequences (decode, verify): the tokens of one adapter (within a window of 1024
 // sequences) make tiles of 16, and the CTA of a tile's first sequence works for all of
@@ -26,10 +27,12 @@
 // What bounds it: memory -- A and B of the adapters in use for short sequences
 // (where a few MB are latency), x and the fp32 output for prompts.  Tensor cores of
 // the tcgen05 kind would wait: 2 r flops per byte of x.
-// Measured: 1 token 2560 -> 6144 at rank 16 5.6 us (launch, three dependent loads, a
-// cluster's exchange), 32 tokens with an adapter each 2560 -> 19456 11.4 us (1.5 TB/s),
-// 7 prompts of 701 tokens 2560 -> 6144 at rank 32 39.9 us (3.6 TB/s: 13 of it shrink
+// Measured: 1 token 2560 -> 6144 at rank 16 5.2 us (launch, three dependent loads, a
+// cluster's exchange), 32 tokens with an adapter each 2560 -> 19456 10.8 us (1.5 TB/s),
+// 7 prompts of 701 tokens 2560 -> 6144 at rank 32 39.5 us (3.7 TB/s: 13 of it shrink
 // at 1.9, the rest writes the output).
+#include <type_traits>
+
 #include "mma_sync.cuh"
 
 namespace lsb {
@@ -289,52 +292,64 @@ __global__ void __launch_bounds__(kLoPromptThreads) lora_shrink_prompt_kernel(Lo
   });
 }
 
-// u of 16 tokens as fragments of KS steps, each value a sum of three bf16.
-template <int KS>
-struct LoraU {
-  uint32_t f[KS][3][4];
-  __device__ __forceinline__ void load(const LoraParams& p, const int (&tok)[2]) {  // rows g8, g8 + 8 (< 0: zeros)
-    split(p.R, [&](int h, int k) {
-      return tok[h] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                        : __ldcg(reinterpret_cast<const float4*>(p.u + (size_t)tok[h] * p.R + k));
-    });
+// Four values as sums of three bf16, each part as two pairs.
+__device__ __forceinline__ void lora_three(const float4& v, uint32_t (&lo)[3], uint32_t (&hi)[3]) {
+  float r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    float c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c[e] = round_bf16(r[e]);
+      r[e] = fabsf(c[e]) < INFINITY ? r[e] - c[e] : 0.f;  // (infinity and NaN are whole in the first part)
+    }
+    lo[q] = pack_bf16(c[0], c[1]);
+    hi[q] = pack_bf16(c[2], c[3]);
   }
-  // value(h, k): u of rank k .. k + 3 of row g8 + 8 h
+}
+
+// u of a tile's tokens as fragments of KS steps, each value a sum of three bf16: TOK = 16
+// as the MMA's rows (a lane's are g8 and g8 + 8), TOK = 8 as its columns (a lane's is g8).
+template <int KS, int TOK>
+struct LoraU {
+  static constexpr int H = TOK / 8;
+  uint32_t f[KS][3][2 * H];
+  // value(h, k): u of rank k .. k + 3 of token g8 + 8 h
   template <typename Value>
   __device__ __forceinline__ void split(int R, Value value) {
     const int t4 = threadIdx.x & 3;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < H; ++h) {
         const int k = s * 16 + t4 * 4;
-        const float4 v = k < R ? value(h, k) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float r[4] = {v.x, v.y, v.z, v.w};
+        uint32_t lo[3], hi[3];
+        lora_three(k < R ? value(h, k) : make_float4(0.f, 0.f, 0.f, 0.f), lo, hi);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-          float c[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            c[e] = round_bf16(r[e]);
-            r[e] = fabsf(c[e]) < INFINITY ? r[e] - c[e] : 0.f;  // (infinity and NaN are whole in the first part)
-          }
-          f[s][q][h] = pack_bf16(c[0], c[1]);
-          f[s][q][2 + h] = pack_bf16(c[2], c[3]);
-        }
+        for (int q = 0; q < 3; ++q) f[s][q][h] = lo[q], f[s][q][H + h] = hi[q];
       }
+  }
+  // From the workspace; tok: the tokens, < 0: zeros.
+  __device__ __forceinline__ void load(const LoraParams& p, const int (&tok)[H]) {
+    split(p.R, [&](int h, int k) {
+      return tok[h] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : __ldcg(reinterpret_cast<const float4*>(p.u + (size_t)tok[h] * p.R + k));
+    });
   }
 };
 
-// The rows of b of outputs n .. n + 15 as two fragments a step; a lane's four outputs
-// are neighbours: column 2 t4 + e of product j is output 4 t4 + 2 j + e.
-template <int KS>
+// The rows of b of outputs n .. n + 15 as fragments of KS steps.  TOK = 16: columns of two
+// products, column 2 t4 + e of product j is output 4 t4 + 2 j + e, so that a lane's four
+// outputs of a token are neighbours; TOK = 8: rows of one, rows g8 and g8 + 8 are outputs
+// 2 g8 and 2 g8 + 1, so that a lane's two of a token are.
+template <int KS, int TOK>
 struct LoraB {
   uint2 v[2][KS];
   __device__ __forceinline__ void load(const __nv_bfloat16* b, int n, int n1, int R) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int row = n + (g8 >> 1) * 4 + j * 2 + (g8 & 1);
+      const int row = n + (TOK == 8 ? 2 * g8 + j : (g8 >> 1) * 4 + j * 2 + (g8 & 1));
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int k = s * 16 + t4 * 4;
@@ -344,45 +359,74 @@ struct LoraB {
   }
 };
 
-// Outputs n .. n + 15 of 16 tokens.
-template <int KS>
-__device__ __forceinline__ void lora_store(const LoraParams& p, const LoraU<KS>& u, const LoraB<KS>& b, float scale,
-                                           const int (&tok)[2], int n, int n1) {
-  const int t4 = threadIdx.x & 3;
-  float acc[2][4] = {};
+// Outputs n .. n + 15 of a tile.  tok: the tokens that this lane stores, g8 and g8 + 8
+// (TOK = 16) or 2 t4 and 2 t4 + 1 (TOK = 8); < 0: none.
+template <int KS, int TOK>
+__device__ __forceinline__ void lora_store(const LoraParams& p, const LoraU<KS, TOK>& u, const LoraB<KS, TOK>& b,
+                                           float scale, const int (&tok)[2], int n, int n1) {
+  const int g8 = (threadIdx.x & 31) >> 2, t4 = threadIdx.x & 3;
+  if constexpr (TOK == 8) {
+    float acc[4] = {};
 #pragma unroll
-  for (int q = 2; q >= 0; --q)  // the small parts first
+    for (int q = 2; q >= 0; --q)  // the small parts first
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KS; ++s) {
+        const uint32_t fa[4] = {b.v[0][s].x, b.v[1][s].x, b.v[0][s].y, b.v[1][s].y};
+        mma_bf16(acc, fa, u.f[s][q][0], u.f[s][q][1]);
+      }
+    if (n + 2 * g8 >= n1) return;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) mma_bf16(acc[j], u.f[s][q], b.v[j][s].x, b.v[j][s].y);
-  if (n + t4 * 4 >= n1) return;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (tok[h] < 0) continue;
-    float4* o = reinterpret_cast<float4*>(p.out + (size_t)tok[h] * p.N + n + t4 * 4);
-    float4 v = make_float4(acc[0][2 * h] * scale, acc[0][2 * h + 1] * scale, acc[1][2 * h] * scale,
-                           acc[1][2 * h + 1] * scale);
-    if (p.accumulate) {
-      const float4 w = *o;
-      v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
+    for (int h = 0; h < 2; ++h) {
+      if (tok[h] < 0) continue;
+      float2* o = reinterpret_cast<float2*>(p.out + (size_t)tok[h] * p.N + n + 2 * g8);
+      float2 v = make_float2(acc[h] * scale, acc[2 + h] * scale);
+      if (p.accumulate) {
+        const float2 w = *o;
+        v = make_float2(w.x + v.x, w.y + v.y);
+      }
+      *o = v;
     }
-    *o = v;
+  } else {
+    float acc[2][4] = {};
+#pragma unroll
+    for (int q = 2; q >= 0; --q)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma_bf16(acc[j], u.f[s][q], b.v[j][s].x, b.v[j][s].y);
+    if (n + t4 * 4 >= n1) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (tok[h] < 0) continue;
+      float4* o = reinterpret_cast<float4*>(p.out + (size_t)tok[h] * p.N + n + t4 * 4);
+      float4 v = make_float4(acc[0][2 * h] * scale, acc[0][2 * h + 1] * scale, acc[1][2 * h] * scale,
+                             acc[1][2 * h + 1] * scale);
+      if (p.accumulate) {
+        const float4 w = *o;
+        v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
+      }
+      *o = v;
+    }
   }
 }
 
-// Outputs [n0, n1) of 16 tokens, 16 at a time, `step` apart.
-template <int KS>
-__device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS>& u, int id, const int (&tok)[2], int n0,
-                                             int n1, int step) {
+// Outputs [n0, n1) of a tile, 16 at a time, `step` apart.
+template <int KS, int TOK>
+__device__ __forceinline__ void lora_outputs(const LoraParams& p, const LoraU<KS, TOK>& u, int id, const int (&tok)[2],
+                                             int n0, int n1, int step) {
   const __nv_bfloat16* b = p.b + (size_t)id * p.N * p.R;
   const float scale = p.scaling[id];
 #pragma unroll (KS == 1 ? 8 : 4)
   for (int n = n0; n < n1; n += step) {
-    LoraB<KS> f;
+    LoraB<KS, TOK> f;
     f.load(b, n, n1, p.R);
-    lora_store<KS>(p, u, f, scale, tok, n, n1);
+    lora_store<KS, TOK>(p, u, f, scale, tok, n, n1);
   }
+}
+
+// Token i of a tile of short sequences, -1 behind its last.
+__device__ __forceinline__ int lora_token(const LoraParams& p, const int (&members)[16], int tokens, int i) {
+  return i < tokens ? members[i / p.q_len] * p.q_len + i % p.q_len : -1;
 }
 
 // Zeros into outputs [n0, n1) of `count` tokens from token t0 on.
@@ -393,7 +437,7 @@ __device__ __forceinline__ void lora_zeros(const LoraParams& p, int t0, int coun
 }
 
 template <int KS>
-__global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
+__global__ void __launch_bounds__(kLoThreads, KS == 1 ? 10 : KS <= 4 ? 4 : 3) lora_expand_kernel(LoraParams p) {
   __shared__ int members[16];
   // The shrink kernel's CTAs let this one start only after every kernel before them
   // is complete: ids, b and out may be used at once, u after the wait.
@@ -410,15 +454,19 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraParams p) {
   if (tokens > 0) lora_prefetch(p.b + ((size_t)id * p.N + n0) * p.R, (n1 - n0) * p.R * 2);
   grid_dep_wait();
   if (!tokens) return;
-  int tok[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = g8 + 8 * h;
-    tok[h] = i < tokens ? members[i / p.q_len] * p.q_len + i % p.q_len : -1;
+  const int t4 = lane & 3;
+  if (tokens <= 8) {
+    const int of[1] = {lora_token(p, members, tokens, g8)};
+    const int tok[2] = {lora_token(p, members, tokens, 2 * t4), lora_token(p, members, tokens, 2 * t4 + 1)};
+    LoraU<KS, 8> u;
+    u.load(p, of);
+    lora_outputs<KS, 8>(p, u, id, tok, n0 + warp * 16, n1, 16 * kLoWarps);
+  } else {
+    const int tok[2] = {lora_token(p, members, tokens, g8), lora_token(p, members, tokens, g8 + 8)};
+    LoraU<KS, 16> u;
+    u.load(p, tok);
+    lora_outputs<KS, 16>(p, u, id, tok, n0 + warp * 16, n1, 16 * kLoWarps);
   }
-  LoraU<KS> u;
-  u.load(p, tok);
-  lora_outputs<KS>(p, u, id, tok, n0 + warp * 16, n1, 16 * kLoWarps);
 }
 
 template <int KS>
@@ -442,9 +490,9 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_prompt_kernel(LoraPara
     tok[h] = t < p.q_len ? b * p.q_len + t : -1;
   }
   if (t0 + warp * 16 >= p.q_len) return;
-  LoraU<KS> u;
+  LoraU<KS, 16> u;
   u.load(p, tok);
-  lora_outputs<KS>(p, u, id, tok, n0, n1, 16);
+  lora_outputs<KS, 16>(p, u, id, tok, n0, n1, 16);
 }
 
 // Short sequences, both halves in one launch: a cluster of 8 CTAs per sequence.  CTA c
@@ -452,7 +500,7 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_prompt_kernel(LoraPara
 // (each CTA adds an eighth of them, in split order, and hands its sums to all), then it
 // takes outputs [c n_block, (c + 1) n_block).
 template <int KS, int THREADS>
-__global__ void __launch_bounds__(THREADS) lora_one_kernel(LoraParams p) {
+__global__ void __launch_bounds__(THREADS, KS == 1 ? 1024 / THREADS : 512 / THREADS) lora_one_kernel(LoraParams p) {  // registers for 1024 threads an SM at rank 16, else for 512
   constexpr int NT = KS * 2, RP = KS * 16, WARPS = THREADS / 32;
   __shared__ int members[16];
   __shared__ float red[WARPS / 2][16][RP + 1], part[16 * RP];
@@ -502,29 +550,40 @@ __global__ void __launch_bounds__(THREADS) lora_one_kernel(LoraParams p) {
     for (int w = 0; w < WARPS / 2; ++w) v += red[w][i / RP][i % RP];
     part[i] = v;
   }
-  // The first outputs' rows of b, while the CTAs exchange their sums.
-  constexpr int kPre = KS == 1 ? 2 : 1;
-  const int nw = n0 + warp * 16;
-  LoraB<KS> pre[kPre];
+  auto exchange = [&]() {
+    cluster_sync();
+    for (int i = c * (2 * RP) + threadIdx.x; i < (c + 1) * (2 * RP); i += THREADS) {
+      float w[8], v = 0.f;
 #pragma unroll
-  for (int q = 0; q < kPre; ++q) pre[q].load(pb, nw + q * 16 * WARPS, n1, p.R);
+      for (int q = 0; q < 8; ++q) w[q] = ld_cluster(part + i, q);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += w[q];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) st_cluster(&sum[0][0] + i, q, v);
+    }
+    cluster_sync();  // (and no CTA reads or writes another's memory any more)
+  };
   const float scale = p.scaling[id];
-  cluster_sync();
-  for (int i = c * (2 * RP) + threadIdx.x; i < (c + 1) * (2 * RP); i += THREADS) {
-    float w[8], v = 0.f;
+  // The rows of b of the warp's first outputs are loaded while the CTAs exchange their sums.
+  auto expand = [&](auto tile, const int (&to)[2]) {
+    constexpr int TOK = decltype(tile)::value, kPre = KS == 1 ? 2 : 1;
+    const int nw = n0 + warp * 16;
+    LoraB<KS, TOK> pre[kPre];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) w[q] = ld_cluster(part + i, q);
+    for (int q = 0; q < kPre; ++q) pre[q].load(pb, nw + q * 16 * WARPS, n1, p.R);
+    exchange();
+    LoraU<KS, TOK> u;
+    u.split(p.R, [&](int h, int k) { return *reinterpret_cast<const float4*>(&sum[g8 + 8 * h][k]); });
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v += w[q];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) st_cluster(&sum[0][0] + i, q, v);
+    for (int q = 0; q < kPre; ++q) lora_store<KS, TOK>(p, u, pre[q], scale, to, nw + q * 16 * WARPS, n1);
+    lora_outputs<KS, TOK>(p, u, id, to, nw + kPre * 16 * WARPS, n1, 16 * WARPS);
+  };
+  if (tokens <= 8) {  // (for the whole cluster)
+    const int to[2] = {lora_token(p, members, tokens, 2 * t4), lora_token(p, members, tokens, 2 * t4 + 1)};
+    expand(std::integral_constant<int, 8>(), to);
+  } else {
+    expand(std::integral_constant<int, 16>(), tok);
   }
-  cluster_sync();  // (and no CTA reads or writes another's memory any more)
-  LoraU<KS> u;
-  u.split(p.R, [&](int h, int k) { return *reinterpret_cast<const float4*>(&sum[g8 + 8 * h][k]); });
-#pragma unroll
-  for (int q = 0; q < kPre; ++q) lora_store<KS>(p, u, pre[q], scale, tok, nw + q * 16 * WARPS, n1);
-  lora_outputs<KS>(p, u, id, tok, nw + kPre * 16 * WARPS, n1, 16 * WARPS);
 }
 
 }  // namespace lsb
