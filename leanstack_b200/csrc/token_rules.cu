@@ -25,8 +25,8 @@
 // many, instruction issue beside the loads, so a group is kept short: bits as bytes,
 // masks by byte permutes, a packed maximum and no index (161 -> 70 instructions a
 // group of 8 bf16 tokens), seen tokens one at a time.
-// Measured: 1 row of 151936 bf16 5.0 us (launch and latency), 32 rows of it under a
-// grammar of 300 tokens 7.3, 128 rows with everything and written logits 34 (3.5 TB/s).
+// Measured: 1 row of 151936 bf16 4.8 us (launch and latency), 32 rows of it under a
+// grammar of 300 tokens 7.1, 128 rows with everything and written logits 34 (3.5 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -287,9 +287,13 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
   }
 }
 
-__device__ __forceinline__ int64_t tr_block_max(int64_t key, int64_t* warps) {  // of all kTrPickThreads threads
+__device__ __forceinline__ int64_t tr_warp_max(int64_t key) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) key = max(key, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)key, o));
+  return key;
+}
+__device__ __forceinline__ int64_t tr_block_max(int64_t key, int64_t* warps) {  // of all kTrPickThreads threads
+  key = tr_warp_max(key);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = key;
   __syncthreads();
@@ -310,7 +314,6 @@ __global__ void __launch_bounds__(kTrPickThreads) constrained_pick_kernel(TrPara
   __shared__ float values[kStage];
   __shared__ int64_t warps[kTrPickThreads / 32];
   __shared__ int s_first;
-  __shared__ uint32_t s_biased;  // tokens of the winning group that have a bias
   // The kernel before lets this one start only after every kernel before it is
   // complete: logits, state and rules may be used at once, its keys after the wait.
   grid_dep_launch();
@@ -364,39 +367,46 @@ __global__ void __launch_bounds__(kTrPickThreads) constrained_pick_kernel(TrPara
     x = __fadd_rn(x, add);
     return free && first ? v : -1;
   };
-  int64_t key = kTrNoKey;
+  int64_t key = kTrNoKey;  // of the biased tokens; the same in every thread
   float x = 0.f;
-  int v = p.bias_cap ? biased(tid, x) : -1;
-  grid_dep_wait();
-  for (int k = tid;;) {  // (with the block: biased() has barriers)
-    if (v >= 0) {
-      if (p.out_logits) p.out_logits[row_v + v] = x;
-      if (x == x) key = max(key, argmax_key(x, v));
-    }
-    k += kTrPickThreads;
-    if (k - tid >= p.bias_cap) break;
-    v = biased(k, x);
+  int v = -1;
+  if (p.bias_cap) {
+    v = biased(tid, x);
+    key = tr_block_max(v >= 0 && x == x ? argmax_key(x, v) : kTrNoKey, warps);
   }
+  grid_dep_wait();
+  for (int k0 = 0;; v = biased(k0 + tid, x)) {  // (with the block: biased() has barriers)
+    if (v >= 0 && p.out_logits) p.out_logits[row_v + v] = x;
+    if (k0 > 0) key = max(key, tr_block_max(v >= 0 && x == x ? argmax_key(x, v) : kTrNoKey, warps));
+    k0 += kTrPickThreads;
+    if (k0 >= p.bias_cap) break;
+  }
+  // Every warp finds the winning key, the first one the token: no barrier on this way.
   int64_t top = kTrNoKey;
-  for (int i = tid; i < ncta; i += kTrPickThreads)
-    top = max(top, (int64_t)__ldcg(reinterpret_cast<const long long*>(p.keys) + (size_t)row * ncta + i));
-  if (tid == 0) s_biased = 0u;
-  top = tr_block_max(top, warps);
-  if (top != kTrNoKey) {
-    const int a = p.V % 8 ? (int)(row_v & 7) : 0;
-    const int v0 = (int)argmax_key_id(top) * 8 - a;
-    for (int k = tid; k < p.bias_cap; k += kTrPickThreads) {
-      const unsigned d = (unsigned)(bias_ids[k] - v0);
-      if (d < 8u) atomicOr(&s_biased, 1u << d);
+  for (int i0 = tid & 31; i0 < ncta; i0 += 128) {
+    int64_t k[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 32 * u;
+      k[u] = i < ncta ? (int64_t)__ldcg(reinterpret_cast<const long long*>(p.keys) + (size_t)row * ncta + i) : kTrNoKey;
     }
+    top = max(top, max(max(k[0], k[1]), max(k[2], k[3])));
+  }
+  top = tr_warp_max(top);
+  if (top != kTrNoKey) {
+    if (tid >= 32) return;
+    const int a = p.V % 8 ? (int)(row_v & 7) : 0, v0 = (int)argmax_key_id(top) * 8 - a;
     bool free = false;
     v = v0 + tid;
     if (tid < 8 && v >= 0 && v < p.V) x = token(v, free);
-    __syncthreads();
-    if (free && x == x && !(s_biased >> tid & 1u)) key = max(key, argmax_key(x, v));
-    key = tr_block_max(key, warps);
+    uint32_t hit = 0u;  // tokens of the group that have a bias
+    for (int k = tid; k < p.bias_cap; k += 32) {
+      const unsigned d = (unsigned)(bias_ids[k] - v0);
+      if (d < 8u) hit |= 1u << d;
+    }
+    hit = __reduce_or_sync(0xffffffffu, hit);
+    key = max(key, tr_warp_max(free && x == x && !(hit >> tid & 1u) ? argmax_key(x, v) : kTrNoKey));
   } else {
-    key = tr_block_max(key, warps);
     // Nothing above -inf without a bias.  Unless a biased token is, a word of tokens a
     // thread, until a block of words holds one that is allowed, not biased and -inf.
     for (int w0 = 0; w0 < p.W && key <= argmax_key(-INFINITY, 0); w0 += kTrPickThreads) {
