@@ -25,8 +25,8 @@
 // many, instruction issue beside the loads, so a group is kept short: bits as bytes,
 // masks by byte permutes, a packed maximum and no index (161 -> 70 instructions a
 // group of 8 bf16 tokens), seen tokens one at a time.
-// Measured: 1 row of 151936 bf16 4.8 us (launch and latency), 32 rows of it under a
-// grammar of 300 tokens 7.1, 128 rows with everything and written logits 34 (3.5 TB/s).
+// Measured: 1 row of 151936 bf16 4.6 us (launch and latency), 32 rows of it under a
+// grammar of 300 tokens 7.0, 128 rows with everything and written logits 34 (3.5 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -153,15 +153,14 @@ __device__ __forceinline__ float tr_penalise(float x, float rep, int n, float fr
 __device__ __forceinline__ float tr_value(__nv_bfloat16 v) { return bf16_to_f(v); }
 __device__ __forceinline__ float tr_value(float v) { return v; }
 
-// VEC: the vocabulary is a multiple of 8.
-template <typename T, bool VEC>
+// VEC: the vocabulary is a multiple of 8.  U: groups in flight per thread.
+template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrParams p) {
   extern __shared__ uint32_t tr_bias[];  // bias lists only: 8 bits for each group of this CTA's tiles
   __shared__ float bv[kTrThreads / 32];
   __shared__ int bi[kTrThreads / 32];
   grid_dep_wait();
   grid_dep_launch();
-  constexpr int U = sizeof(T) == 2 ? 4 : 2;  // groups in flight per thread
   constexpr int nt = kTrThreads, lg = 8;
   const int row = blockIdx.y, c = blockIdx.x, ncta = gridDim.x;
   // Groups of 8 flattened indices; the row's first and last group may reach into
@@ -280,10 +279,15 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
   }
   if ((threadIdx.x & 31) == 0) bv[threadIdx.x >> 5] = best, bi[threadIdx.x >> 5] = bestg;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < nt / 32; ++w)
-      if (tr_better(bv[w], bi[w], best, bestg)) best = bv[w], bestg = bi[w];
-    p.keys[(size_t)row * ncta + c] = bestg != 0x7fffffff ? argmax_key(best, bestg) : kTrNoKey;
+  if (threadIdx.x < nt / 32) {
+    best = bv[threadIdx.x], bestg = bi[threadIdx.x];
+#pragma unroll
+    for (int o = nt / 64; o > 0; o >>= 1) {
+      const float ov = __shfl_xor_sync((1u << nt / 32) - 1u, best, o);
+      const int og = __shfl_xor_sync((1u << nt / 32) - 1u, bestg, o);
+      if (tr_better(ov, og, best, bestg)) best = ov, bestg = og;
+    }
+    if (threadIdx.x == 0) p.keys[(size_t)row * ncta + c] = bestg != 0x7fffffff ? argmax_key(best, bestg) : kTrNoKey;
   }
 }
 
@@ -495,7 +499,11 @@ static int launch_constrained_argmax(const TrParams& p, int64_t m, int record, i
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, constrained_argmax_kernel<T, VEC>, p);
+  // 64 bytes of groups a thread; bf16 with a tile a CTA one group: 4 rows of 151936 5.4
+  // us, with four 5.8 (fp32 with one group is 3% slower than with two).
+  constexpr int U = sizeof(T) == 2 ? 4 : 2, kSingle = sizeof(T) == 2 ? 1 : U;
+  cudaError_t e = ncta >= tiles ? cudaLaunchKernelEx(&cfg, constrained_argmax_kernel<T, VEC, kSingle>, p)
+                                : cudaLaunchKernelEx(&cfg, constrained_argmax_kernel<T, VEC, U>, p);
   if (e == cudaSuccess) {
     cfg.gridDim = dim3((unsigned)m);
     cfg.blockDim = dim3(kTrPickThreads);
