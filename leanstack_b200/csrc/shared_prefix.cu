@@ -375,7 +375,11 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
     if (!ok) s_abort = 1;
     // ---------------- epilogue ----------------
     const int wd = MODE == kKeys ? 0 : w;  // the warp that issued this stream's products
-    const bool fin = ntiles > 0 && __all_sync(0xffffffffu, ok && (wd == 1 && !two ? true : mbar_wait(&o_done[wd], 0u, p.err, 0x39)));
+    // kRows with two row tiles: the ring is idle only when the other stream's products are
+    // done too, which read the same tiles and may be some behind.
+    const bool fin = ntiles > 0 &&
+                     __all_sync(0xffffffffu, ok && (wd == 1 && !two ? true : mbar_wait(&o_done[wd], 0u, p.err, 0x39)) &&
+                                                 (MODE != kRows || !both || mbar_wait(&o_done[wd ^ 1], 0u, p.err, 0x3b)));
     tc_fence_after();
     // Partials go out through shared memory (the ring, idle now): a thread holds
     // a row, a warp writes whole 512-byte rows.  16-byte chunk c of row x sits at

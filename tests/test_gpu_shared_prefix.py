@@ -116,6 +116,16 @@ def test_few_rows(batch, q_len, hq, hkv, prefix):
     _check(batch, q_len, hq, hkv, prefix, [0] * batch, q_len)
 
 
+@pytest.mark.parametrize("batch,q_len,hq,hkv,prefix", [(1, 251, 32, 8, 6985), (3, 80, 32, 8, 3001), (130, 1, 32, 8, 5000),
+                                                       (20, 8, 16, 2, 2500)])
+def test_row_mode_gives_the_same_bits_every_time(batch, q_len, hq, hkv, prefix):
+    """Two streams share the K/V ring and stage their partials in it: neither before the other is done."""
+    lens = [(5 * i) % 17 for i in range(batch)]
+    first = _check(batch, q_len, hq, hkv, prefix, lens, 17 + q_len)
+    for _ in range(20):
+        assert torch.equal(_check(batch, q_len, hq, hkv, prefix, lens, 17 + q_len), first)
+
+
 def test_workspace_grows_with_the_prefix():
     for batch, q_len, hq, hkv in ((1, 1, 8, 8), (4, 1, 32, 8), (16, 1, 2, 2), (17, 1, 2, 2), (3, 5, 32, 8)):
         need = [K.shared_prefix_attention_workspace_bytes(batch, q_len, hq, hkv, 128, p)
