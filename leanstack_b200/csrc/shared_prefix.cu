@@ -35,10 +35,12 @@
 //     rows): they hold the same rows and take alternate K/V tiles; their results
 //     join in the epilogue, and 114 KB of shared memory and 128 registers leave
 //     room for five strip CTAs on the same SM.
-//   * P is rounded to bf16 (2^-8 of each probability, independent from key to
-//     key, against one more 2^-8 when the output is rounded), the row sum is
-//     taken before that rounding in fp32.  The maximum in use moves only when a
-//     score exceeds it by 2^8; then O is rescaled in TMEM.
+//   * P goes into the product as two bf16, hi = bf16(p) and lo = bf16(p - hi), so
+//     to 2^-16 of itself, as in the attention kernels without a prefix; one bf16
+//     (2^-8) shifts every key of equal score the same way, against a row sum that
+//     is taken in fp32.  The pair takes the place of the scores: columns 0 - 31 and
+//     32 - 63 of their buffer.  The maximum in use moves only when a score exceeds
+//     it by 2^8; then O is rescaled in TMEM.
 //   * kFull: a prompt's rows.  A CTA owns 256 rows of one (sequence, kv head)
 //     and walks the prefix tiles, then the sequence's own tiles with the causal
 //     mask, and writes the finished rows: no partials, no join.
@@ -244,8 +246,9 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
         ok = ok && mbar_wait(&p_full[2 * w + (j & 1)], (uint32_t)(j >> 1) & 1u, p.err, 0x34);
         if (!ok) break;
         tc_fence_after();
-        umma_ta_k64(tmem + 256 + w * 128, tmem + w * 128 + (j & 1) * kSpKeys, v_desc + sv * (kSpSlot >> 4), idesc_pv,
-                    j > 0 ? 1u : 0u);  // O += P V
+        const uint32_t tP = tmem + w * 128 + (j & 1) * kSpKeys;
+        umma_ta_k64(tmem + 256 + w * 128, tP, v_desc + sv * (kSpSlot >> 4), idesc_pv, j > 0 ? 1u : 0u);  // O += P V
+        umma_ta_k64(tmem + 256 + w * 128, tP + kSpKeys / 2, v_desc + sv * (kSpSlot >> 4), idesc_pv, 1u);
         if (more) issue_s(w, j + 2, sk);
         umma_commit_warp(&o_part[2 * w + (j & 1)]);
         umma_commit_warp(&empty[sv]);
@@ -341,17 +344,19 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
         const float neg_m = m_run == -INFINITY ? 0.f : -m_run;  // a row without keys so far: exp2(-inf) = 0
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), neg2 = make_float2(neg_m, neg_m);
         float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t pk[kSpKeys / 2];
+        uint32_t hi[kSpKeys / 2], lo[kSpKeys / 2];
 #pragma unroll
         for (int e = 0; e < kSpKeys / 2; ++e) {
           float2 x = fma2(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale2, neg2);
           x.x = ex2_approx(x.x);
           x.y = ex2_approx(x.y);
           ls[e & 1] = add2(ls[e & 1], x);
-          const __nv_bfloat162 v2 = __floats2bfloat162_rn(x.x, x.y);
-          pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
+          hi[e] = pack_bf16(x.x, x.y);
+          x = fma2(make_float2(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xffff0000u)), make_float2(-1.f, -1.f), x);
+          lo[e] = pack_bf16(x.x, x.y);
         }
-        tmem_st32(tS, pk);
+        tmem_st32(tS, hi);
+        tmem_st32(tS + kSpKeys / 2, lo);
         l_run = l_run * corr + ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y));
         tmem_st_wait();
       }
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
 
 // Groups of a sequence's own strip: one warp per (sequence, kv head, 16 query
 // rows, key chunk), mma.sync m16n8k16 on 16-key tiles from a 2-stage cp.async
-// ring, online softmax in registers, P rounded to bf16 as in prefix_tc_kernel.
+// ring, online softmax in registers, P as two bf16 as in prefix_tc_kernel.
 // A chunk is a row's share of its sequence's keys, at least kStMinBlocks tiles; a
 // chunk behind the end leaves a group without weight.  Single warps: nothing to
 // merge, and the SM's scheduler evens out strips of different lengths.  kFew: a short
@@ -611,15 +616,21 @@ __global__ void __launch_bounds__(32) strip_groups_kernel(StParams p) {
           o[nt][3] *= corr[1];
         }
       }
-      uint32_t pa[4];
+      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) pa[x] = pack_bf16(sc[x >> 1][(x & 1) * 2], sc[x >> 1][(x & 1) * 2 + 1]);
+      for (int x = 0; x < 4; ++x) {
+        const float x0 = sc[x >> 1][(x & 1) * 2], x1 = sc[x >> 1][(x & 1) * 2 + 1];
+        hi[x] = pack_bf16(x0, x1);
+        lo[x] = pack_bf16(x0 - __uint_as_float(hi[x] << 16), x1 - __uint_as_float(hi[x] & 0xffff0000u));
+      }
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         uint32_t v0, v1, v2, v3;
         ldsm_x4_t(stV + ta_swz((lane & 7) + (((lane >> 3) & 1) << 3), 2 * c + (lane >> 4)), v0, v1, v2, v3);
-        mma_bf16(o[2 * c], pa, v0, v1);
-        mma_bf16(o[2 * c + 1], pa, v2, v3);
+        mma_bf16(o[2 * c], hi, v0, v1);
+        mma_bf16(o[2 * c + 1], hi, v2, v3);
+        mma_bf16(o[2 * c], lo, v0, v1);
+        mma_bf16(o[2 * c + 1], lo, v2, v3);
       }
       __syncwarp();
       if (n + kStStages < nb) load_block(n + kStStages);
