@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
           tmem_ld32(tmem + 256 + lane_off + (uint32_t)(w * 64 + c32 * 32), o0);
           if (two) tmem_ld32(tmem + 384 + lane_off + (uint32_t)(w * 64 + c32 * 32), o1);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o0[e] = (fa != 0.f ? o0[e] * fa : 0.f) + (two && fc != 0.f ? o1[e] * fc : 0.f);
+          for (int e = 0; e < 32; ++e) o0[e] = o0[e] * fa + (two ? o1[e] * fc : 0.f);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             stage[r * 32 + ((w * 16 + c32 * 8 + e) ^ (r & 31))] =
@@ -417,7 +417,9 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
       named_bar_sync(1, kSpSoft);
     } else if (fin && warp_valid) {
       const int tok = valid ? row / p.G : 0;
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      // A row without a key has no weight at all and gives zeros; a NaN or infinite score
+      // makes the sum NaN, and NaN goes out.
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       if (MODE == kRows && valid) p.part_ml[((size_t)h * p.rows + row) * p.n_part + split] = make_float2(m_run, l_run);
 #pragma unroll 1
       for (int c16 = 0; c16 < 8; ++c16) {
@@ -432,8 +434,8 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
           uint32_t pk[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const __nv_bfloat162 v2 = __floats2bfloat162_rn(l_run > 0.f ? ov[2 * e] * inv : 0.f,
-                                                            l_run > 0.f ? ov[2 * e + 1] * inv : 0.f);
+            const __nv_bfloat162 v2 = __floats2bfloat162_rn(l_run == 0.f ? 0.f : ov[2 * e] * inv,
+                                                            l_run == 0.f ? 0.f : ov[2 * e + 1] * inv);
             pk[e] = *reinterpret_cast<const uint32_t*>(&v2);
           }
           uint4* dst = reinterpret_cast<uint4*>(
@@ -681,22 +683,26 @@ __global__ void __launch_bounds__(kSpJoinWarps * 32) prefix_join_kernel(const fl
       if (u < n) v[u] = __ldcg(po + (size_t)(c0 + u) * (kSpHeadDim / 2));
     const float2 ml = lane < n ? __ldcg(part_ml + at + c0 + lane) : make_float2(-INFINITY, 0.f);
     const float mn = fmaxf(M, warp_max(ml.x));
-    if (mn == -INFINITY) continue;  // no key so far
+    if (mn == -INFINITY) {  // no key so far, or scores that are all NaN: then the sum is
+      l += warp_sum(ml.y);
+      continue;
+    }
     const float corr = exp2f(M - mn), f = exp2f(ml.x - mn);
+    const uint32_t some = __ballot_sync(0xffffffffu, ml.y != 0.f);  // a group without keys may hold anything
     M = mn;
     l = l * corr + warp_sum(ml.y * f);
     o.x *= corr, o.y *= corr;
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
       const float fu = __shfl_sync(0xffffffffu, f, u);
-      if (u < n && fu != 0.f) {  // a group without weight may hold anything
+      if (u < n && (some >> u & 1u)) {
         o.x = fmaf(v[u].x, fu, o.x);
         o.y = fmaf(v[u].y, fu, o.y);
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const __nv_bfloat162 v2 = l > 0.f ? __floats2bfloat162_rn(o.x * inv, o.y * inv) : __floats2bfloat162_rn(0.f, 0.f);
+  const float inv = 1.f / l;
+  const __nv_bfloat162 v2 = l == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(o.x * inv, o.y * inv);
   const int t = row / G;
   *reinterpret_cast<__nv_bfloat162*>(out + ((size_t)t * Hq + h * G + (row - t * G)) * kSpHeadDim + dim) = v2;
 }
