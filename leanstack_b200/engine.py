@@ -223,7 +223,7 @@ class DecodeEngine:
         if need > self.attn_ws.numel():
             self.attn_ws = torch.zeros(need, device=self.rt.device, dtype=torch.uint8)
         if self.rules is not None:
-            self.rules.note_prompt(ids.expand(self.B, P).contiguous())
+            self.rules.set_prefix(ids)
 
     def _lora(self, li: int, target: str, x: torch.Tensor, splits: int, q_len: int) -> int:
         """The adapters' delta of a linear as one more partial behind its ``splits``; returns their number."""
@@ -510,7 +510,10 @@ class DecodeEngine:
 
     # ------------------------------------------------------------------
     def reset(self) -> None:
+        """Empty sequences; the shared prefix, the adapters and each row's rules stay."""
         self.kv.reset()
+        if self.rules is not None:
+            self.rules.restart()
 
     def prefill(self, prompt_ids: torch.Tensor) -> torch.Tensor:
         """Run ``prompt_ids [B, P]`` through the stack; returns the first greedy token per sequence ``[B]``.

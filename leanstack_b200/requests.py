@@ -97,8 +97,10 @@ class TokenRules:
     """Penalties, biases and grammar masks of each sequence for the greedy pick (:func:`kernels.constrained_argmax`).
 
     ``seen`` marks the tokens of prompt and answer, ``counts`` counts the
-    answer's; the engine keeps both.  ``allowed`` (with ``grammar=True``) holds
-    one bit per token, all set until a request's grammar writes its words.
+    answer's; the engine keeps both.  The tokens of a shared prefix belong to
+    every prompt: ``prefix_seen`` holds them, and whatever empties a row leaves
+    them in it.  ``allowed`` (with ``grammar=True``) holds one bit per token, all
+    set until a request's grammar writes its words.
     """
 
     def __init__(self, batch: int, vocab: int, device, max_biases: int = 0, grammar: bool = False):
@@ -109,6 +111,7 @@ class TokenRules:
 
         self.counts = full((batch, vocab), 0, torch.int32)
         self.seen = full((batch, self.words), 0, torch.int32)
+        self.prefix_seen = full((1, self.words), 0, torch.int32)
         self.repetition = full((batch,), 1.0, torch.float32)
         self.frequency = full((batch,), 0.0, torch.float32)
         self.presence = full((batch,), 0.0, torch.float32)
@@ -120,7 +123,7 @@ class TokenRules:
 
     def set_request(self, row: int, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
                     biases: dict[int, float] | None = None) -> None:
-        """The rules of the request in ``row``; its token counts start anew."""
+        """The rules of the request in ``row``; its token counts start anew, behind the present prefix."""
         if not 0 <= row < self.batch:
             raise ValueError(f"row {row} outside the batch of {self.batch}")
         if not repetition > 0:
@@ -140,7 +143,20 @@ class TokenRules:
         if self.allowed is not None:
             self.allowed[row].fill_(-1)
         self.counts[row].zero_()
-        self.seen[row].zero_()
+        self.seen[row].copy_(self.prefix_seen[0])
+
+    def restart(self) -> None:
+        """Empty sequences in every row: no answer, and of the prompt only the shared prefix.  The rules stay."""
+        self.counts.zero_()
+        self.seen.copy_(self.prefix_seen.expand_as(self.seen))
+
+    def set_prefix(self, ids: torch.Tensor) -> None:
+        """The tokens ``ids [P]`` as every prompt's shared prefix, in place of the one before; the sequences are empty."""
+        self.counts.zero_()
+        self.seen.bitwise_and_(~self.prefix_seen)
+        self.prefix_seen.zero_()
+        K.token_stats_add(ids.view(1, -1), self.prefix_seen, self.vocab)
+        self.seen.bitwise_or_(self.prefix_seen)
 
     def note_prompt(self, ids: torch.Tensor) -> None:
         """Mark the prompt tokens ``ids [batch, n]`` (negative: padding) as seen."""
