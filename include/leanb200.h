@@ -458,6 +458,7 @@ int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const 
  *   bias_ids, bias_values  [m, bias_cap]; ids outside the vocabulary are skipped
  *   allowed   uint32 [m, ceil(vocab / 32)] or NULL (every token)
  *   record    count the picked token and mark it seen
+ * out_logits must not overlap logits (not in place: LS_ERR_INVALID_ARGUMENT).
  * NaN logits are never picked (-1 where nothing else is allowed); vocab <= 2^20,
  * bias_cap <= 2^14; the workspace needs no filling.
  * ls_token_stats_add enters ids [batch, len]

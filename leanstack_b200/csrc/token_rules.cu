@@ -550,6 +550,11 @@ int ls_constrained_argmax(const void* logits, int logits_f32, int64_t m, int64_t
              "ls_constrained_argmax: logits must be 16-byte aligned");
   LS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, LS_ERR_WORKSPACE,
              "ls_constrained_argmax: workspace needs %lld bytes, 8-byte aligned", (long long)need);
+  // The pick reads the logits of a group again after the main pass has written them processed.
+  const uintptr_t in = reinterpret_cast<uintptr_t>(logits), to = reinterpret_cast<uintptr_t>(out_logits);
+  const uint64_t elements = (uint64_t)m * (uint64_t)vocab;
+  LS_REQUIRE(!out_logits || to >= in + elements * (logits_f32 ? 4 : 2) || in >= to + elements * 4, LS_ERR_INVALID_ARGUMENT,
+             "ls_constrained_argmax: out_logits overlaps logits (not in place)");
   TrParams p = {};
   p.logits = logits;
   p.counts = counts;

@@ -754,8 +754,8 @@ def constrained_argmax(logits: torch.Tensor, *, counts: torch.Tensor | None = No
     words ``[m, ceil(vocab / 32)]``, bit ``v % 32`` of word ``v // 32``.  Lowest
     id on ties, -1 where nothing is allowed.  ``record`` enters the pick into
     ``counts`` and ``seen``; ``out_logits`` fp32 ``[m, vocab]`` receives the
-    processed logits (-inf where not allowed).  ``workspace`` needs no filling;
-    calls on one stream may share it.
+    processed logits (-inf where not allowed) and must not overlap ``logits``.
+    ``workspace`` needs no filling; calls on one stream may share it.
     """
     done = (nat._FRONT or nat.front()).constrained_argmax(
         logits, counts, seen, repetition, frequency, presence, bias_ids, bias_values, allowed, record, out_ids,
