@@ -30,6 +30,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "token_groups.cuh"
 
 namespace lsb {
 
@@ -168,7 +169,8 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
   // tiles of 256 groups in turn: frequent tokens have low ids, and
   // with them the counts to read.
   const long long row0 = (long long)row * p.V;
-  const int a = VEC ? 0 : (int)(row0 & 7), ngroups = (p.V + a + 7) / 8;
+  const int a = VEC ? 0 : tr_offset(row, p.V), ngroups = tr_groups(a, p.V);
+  const int left = VEC ? 0 : tr_left(row, p.V, gridDim.y);
   const int stride = ncta << lg;  // groups from one own tile to the next
   const T* logits = static_cast<const T*>(p.logits) + row0 - a;
   const uint32_t* seen = p.seen ? p.seen + (size_t)row * p.W : nullptr;
@@ -206,8 +208,8 @@ __global__ void __launch_bounds__(kTrThreads, 4) constrained_argmax_kernel(TrPar
       sb[u] &= ab[u];
       raw[u] = {};  // (a value in any case: what no bit keeps is masked, not unknown)
       if (ab[u] == 0u) continue;
-      if (!VEC && row == (int)gridDim.y - 1 && g * 8 - a + 8 > p.V) raw[u].load(logits + g * 8, 0, p.V - (g * 8 - a));
-      else raw[u].load(logits + g * 8);  // (the array does not end inside the group)
+      if (!VEC && g * 8 + 8 > left) raw[u].load(logits + g * 8, 0, left - g * 8);  // (the array ends inside the group)
+      else raw[u].load(logits + g * 8);
       if (sb[u]) n0[u] = counts[g * 8 + __ffs(sb[u]) - 1];
     }
   };
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(kTrPickThreads) constrained_pick_kernel(TrPara
   top = tr_warp_max(top);
   if (top != kTrNoKey) {
     if (tid >= 32) return;
-    const int a = p.V % 8 ? (int)(row_v & 7) : 0, v0 = (int)argmax_key_id(top) * 8 - a;
+    const int v0 = (int)argmax_key_id(top) * 8 - tr_offset(row, p.V);
     bool free = false;
     v = v0 + tid;
     if (tid < 8 && v >= 0 && v < p.V) x = token(v, free);
