@@ -22,7 +22,8 @@ A batch of different requests (one GPU; ``requests.py``): ``prefix_capacity``
 makes room for a prompt prefix that all sequences share, held once
 (``prefill_prefix``); ``adapters`` is a bank of low-rank adapters, of which each
 sequence uses one or none (``set_adapters``); ``rules`` constrains each
-sequence's greedy pick.
+sequence's greedy pick.  A row whose rules allow no token reads -1 in
+``current_ids`` and takes the next step as padding (token 0).
 """
 
 from __future__ import annotations
@@ -106,6 +107,8 @@ class DecodeEngine:
         self.prefix = SharedPrefix(g, prefix_capacity, dev, runtime.dtype) if prefix_capacity else None
         self.prefix_epoch = 0  # moves when the prefix changes: steps captured before are stale
         self.adapters, self.rules = adapters, rules
+        if rules is not None:
+            self.step_ids = torch.zeros(batch_size, device=dev, dtype=torch.int64)
         ws = max(K.attention_workspace_bytes(batch_size, q, g.num_attention_heads, g.num_key_value_heads, g.head_dim,
                                              self.S) for q in range(1, self.T // batch_size + 1))
         self.attn_ws = torch.zeros(max(ws, 256), device=dev, dtype=torch.uint8)
@@ -249,13 +252,14 @@ class DecodeEngine:
                                   workspace=self.attn_ws)
 
     # ------------------------------------------------------------------
-    def _forward(self, q_len: int, head, advance: bool = True) -> None:
+    def _forward(self, q_len: int, head, advance: bool = True, picked: bool = False) -> None:
         """Enqueue one step of ``q_len`` tokens per sequence on the current stream.
 
         ``head``: falsy (no head), ``True`` / ``"last"`` (greedy token of each
         sequence's last position into ``ids[:B]``) or ``"all"`` (greedy token
         after every position into ``verdict[:m]``, the verify pass).
         ``advance``: move the device cursors by ``q_len`` at the end.
+        ``picked``: the ids are the last step's picks.
         """
         B, g, a, rt = self.B, self.g, self.arenas, self.rt
         m = B * q_len
@@ -267,7 +271,10 @@ class DecodeEngine:
         P = self.prefix_len
         cos, sin = self.cos[P:], self.sin[P:]  # own token j of a sequence sits at position P + j
         s_down = 0
-        K.embed_gather(a.ids[:m], rt.embed_tokens_weight, out=a.x[:m])
+        ids = a.ids[:m]
+        if picked and self.rules is not None:  # a row whose rules left no token (-1) goes on as padding
+            ids = torch.clamp(ids, min=0, out=self.step_ids)
+        K.embed_gather(ids, rt.embed_tokens_weight, out=a.x[:m])
         for li, layer in enumerate(rt.layers):
             att, mlp = layer.attention, layer.mlp
             tt = self.tc_tiles[li] if (tc and self.tc_tiles is not None) else {}
@@ -543,7 +550,7 @@ class DecodeEngine:
         self.arenas.ids[:self.B].copy_(ids.reshape(-1).to(self.arenas.ids.device))
 
     def _decode_once(self) -> None:
-        self._forward(1, head=True)
+        self._forward(1, head=True, picked=True)
 
     def capture(self) -> None:
         """Capture one decode step (q_len 1 + head + cursor advance) as a CUDA graph."""
@@ -665,8 +672,8 @@ class DecodeEngine:
             per_layer += 2 if self.backend == "tc" else 3
         if self.adapters is not None:  # shrink and expand beside each linear
             per_layer += 2 * len(self.adapters.targets)
-        if self.rules is not None:  # rules and pick instead of the argmax (after an lm_head of its own)
-            head += 1 if self.backend == "tc" else 2
+        if self.rules is not None:  # rules and pick instead of the argmax (after an lm_head of its own), ids without -1
+            head += 2 if self.backend == "tc" else 3
         if self.tp is not None:  # + all-reduce / residual-add kernels after each row-split linear, + keys-to-ids
             if self.tp.p2p is None or self.backend == "tc":
                 per_layer += 2
