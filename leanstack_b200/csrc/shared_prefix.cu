@@ -51,6 +51,7 @@
 // keys 23.4 us; 6 prompts of 384 behind 8192 keys 293 us (1088 TFLOP/s: scores of 64 keys
 // keep the tensor pipe waiting for shared memory); 2 sequences behind 300 keys 6.0 us.
 #include <algorithm>
+#include <cmath>
 
 #include "mma_sync.cuh"
 #include "tcgen05.cuh"
@@ -85,7 +86,10 @@ struct SpParams {
   int* err;
   int rows;                // kKeys / kRows: B q_len G; kFull: q_len G
   int q_len, Hq, Hkv, G, P, prefix_cap, max_seq, splits, n_part;
+  // The maximum is taken before the scale, which is positive here: the sign of the
+  // caller's goes to the query rows (q ^ q_flip), and a scale of 0 makes them 0 (q & q_keep).
   float scale_log2;
+  uint32_t q_keep, q_flip;
 };
 
 template <int MODE>
@@ -278,8 +282,13 @@ __global__ void __launch_bounds__(MODE == kKeys ? 512 : sp_threads(MODE), 1)  //
                         (threadIdx.x & 15));
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < 8; ++u) {
+        v[u].x = (v[u].x & p.q_keep) ^ p.q_flip;
+        v[u].y = (v[u].y & p.q_keep) ^ p.q_flip;
+        v[u].z = (v[u].z & p.q_keep) ^ p.q_flip;
+        v[u].w = (v[u].w & p.q_keep) ^ p.q_flip;
         *reinterpret_cast<uint4*>(smem + tile * kSpQ + pt_off((threadIdx.x >> 4) + 16 * u, threadIdx.x & 15, kSpQHalf)) = v[u];
+      }
     }
     fence_proxy_async_smem();
     mbar_arrive(q_full);
@@ -824,7 +833,10 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   p.max_seq = (int)max_seq;
   p.splits = pl.splits;
   p.n_part = pl.splits + pl.chunks;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale == 0.f ? 1.f : std::fabs(scale_log2);
+  p.q_keep = scale == 0.f ? 0u : 0xffffffffu;
+  p.q_flip = scale < 0.f ? 0x80008000u : 0u;
   CUtensorMap kp, vp, kc, vc;
   int rc = LS_OK;
   if (prefix_len > 0 && pl.mode != kFew) {
@@ -872,7 +884,7 @@ static int launch_shared_prefix_attention(const void* q, const void* k_prefix, c
   st.max_seq = p.max_seq;
   st.n_pre = pl.splits;
   st.n_part = p.n_part;
-  st.scale_log2 = p.scale_log2;
+  st.scale_log2 = scale_log2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(few && pl.splits > pl.chunks ? pl.splits : pl.chunks), (unsigned)(hkv * st.RG),
                      (unsigned)(few ? batch + 1 : batch));
