@@ -423,6 +423,9 @@ int ls_spec_accept(int64_t* ids, const int64_t* verdict, int64_t batch, int64_t 
  * workspace needs no filling. */
 int ls_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t q_len, int64_t num_heads, int64_t num_kv_heads,
                                                int64_t head_dim, int64_t prefix_len, int64_t* bytes);
+/* Kernels that one call launches at these sizes. */
+int ls_shared_prefix_attention_launches(int64_t batch, int64_t q_len, int64_t num_heads, int64_t num_kv_heads,
+                                        int64_t head_dim, int64_t prefix_len, int64_t* launches);
 int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
                                int64_t prefix_cap, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
                                int64_t uniform_past, int64_t batch, int64_t q_len, int64_t num_heads,
@@ -440,6 +443,8 @@ int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* 
  * id past the bank counts as none and raises LS_ERR_INVALID_ARGUMENT in the
  * device error flag.  The workspace needs no filling. */
 int ls_lora_delta_workspace_bytes(int64_t batch, int64_t q_len, int64_t k, int64_t n, int64_t rank, int64_t* bytes);
+/* Kernels that one call launches at these sizes. */
+int ls_lora_delta_launches(int64_t batch, int64_t q_len, int64_t k, int64_t n, int64_t rank, int64_t* launches);
 int ls_lora_delta(const void* x, int64_t batch, int64_t q_len, int64_t k, const void* a, const void* b,
                   const float* scaling, int64_t adapters, int64_t n, int64_t rank, const int32_t* adapter_ids,
                   int accumulate, float* out, void* workspace, int64_t workspace_bytes, ls_stream_t stream);

@@ -109,9 +109,11 @@ SIGNATURES: dict[str, list] = {
     "ls_sum_splits_f32": [_p, _i64, _i64, _p, _p],
     "ls_advance_cursors": [_p, _p, _i64, _i64, _p],
     "ls_shared_prefix_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "ls_shared_prefix_attention_launches": [_i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "ls_shared_prefix_attention": [_p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
                                    _p, _p, _i64, _p],
     "ls_lora_delta_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "ls_lora_delta_launches": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "ls_lora_delta": [_p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _int, _p, _p, _i64, _p],
     "ls_constrained_argmax_workspace_bytes": [_i64, _i64, ctypes.POINTER(_i64)],
     "ls_constrained_argmax": [_p, _int, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _int, _p, _p, _p, _i64, _p],

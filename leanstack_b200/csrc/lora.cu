@@ -611,8 +611,8 @@ static int64_t lora_splits(int64_t batch, int64_t q_len, int64_t k) {
 // Threads: 512 halve a CTA's steps, 256 let more CTAs stay: rank 16, 6144 outputs,
 // 256 / 512: 6.1 / 5.6 (1 sequence), 7.4 / 8.1 (32); 19456 outputs: 16.5 / 14.8 (100);
 // rank 64: 15.3 / 22.9 (32).
-static bool lora_one_launch(int64_t batch, int64_t n, int64_t rank) {
-  return batch >= 32 || (rank <= 32 && n <= 8192);
+static bool lora_one_launch(int64_t batch, int64_t q_len, int64_t n, int64_t rank) {
+  return q_len < kLoPrompt && rank <= kLoOneRanks && (batch >= 32 || (rank <= 32 && n <= 8192));
 }
 
 static int64_t lora_workspace(int64_t batch, int64_t q_len, int64_t k, int64_t rank) {
@@ -640,7 +640,7 @@ static cudaError_t launch_lora_kernel(void (*kernel)(LoraParams), dim3 grid, uns
 
 static int launch_lora(LoraParams p, cudaStream_t stream) {
   const bool prompt = p.q_len >= kLoPrompt;
-  if (!prompt && p.R <= kLoOneRanks && lora_one_launch(p.batch, p.N, p.R)) {
+  if (lora_one_launch(p.batch, p.q_len, p.N, p.R)) {
     p.k_chunk = ((p.K + 7) / 8 + 31) / 32 * 32;
     p.n_block = ((p.N + 7) / 8 + 15) / 16 * 16;
     const bool wide = p.R <= 32 && (p.batch < 16 || p.N > 8192);
@@ -703,6 +703,15 @@ int ls_lora_delta_workspace_bytes(int64_t batch, int64_t q_len, int64_t k, int64
   LS_REQUIRE(batch <= 65535 && (q_len + 63) / 64 * 2 <= 65535, LS_ERR_UNSUPPORTED_SHAPE,
              "ls_lora_delta: %lld sequences of %lld tokens exceed the grid", (long long)batch, (long long)q_len);
   *bytes = lora_workspace(batch, q_len, k, rank);
+  return LS_OK;
+}
+
+int ls_lora_delta_launches(int64_t batch, int64_t q_len, int64_t k, int64_t n, int64_t rank, int64_t* launches) {
+  LS_REQUIRE(launches, LS_ERR_INVALID_ARGUMENT, "ls_lora_delta_launches: launches is null");
+  int64_t bytes = 0;
+  const int rc = ls_lora_delta_workspace_bytes(batch, q_len, k, n, rank, &bytes);
+  if (rc) return rc;
+  *launches = lora_one_launch(batch, q_len, n, rank) ? 1 : 2;
   return LS_OK;
 }
 

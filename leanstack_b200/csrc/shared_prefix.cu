@@ -923,6 +923,18 @@ int ls_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t q_len, int
   return LS_OK;
 }
 
+int ls_shared_prefix_attention_launches(int64_t batch, int64_t q_len, int64_t num_heads, int64_t num_kv_heads,
+                                        int64_t head_dim, int64_t prefix_len, int64_t* launches) {
+  LS_REQUIRE(launches, LS_ERR_INVALID_ARGUMENT, "ls_shared_prefix_attention_launches: launches is null");
+  int64_t bytes = 0;
+  const int rc = ls_shared_prefix_attention_workspace_bytes(batch, q_len, num_heads, num_kv_heads, head_dim, prefix_len,
+                                                            &bytes);
+  if (rc) return rc;
+  const int mode = sp_plan(batch, q_len, num_heads, num_kv_heads, prefix_len, 1).mode;  // (for any max_seq)
+  *launches = mode == kFull ? 1 : prefix_len > 0 && mode != kFew ? 3 : 2;
+  return LS_OK;
+}
+
 int ls_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_len,
                                int64_t prefix_cap, const void* k_cache, const void* v_cache, const int32_t* cache_pos,
                                int64_t uniform_past, int64_t batch, int64_t q_len, int64_t num_heads,

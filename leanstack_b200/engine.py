@@ -668,10 +668,14 @@ class DecodeEngine:
         """Kernels one decode step launches (embedding, layers, head, cursor advance)."""
         per_layer = (9 if self.gu_plain else 8) if self.backend == "tc" else 5  # CUDA cores: attention takes the q/k norm
         head = 3 if self.backend == "tc" else 1
-        if self.prefix_len:  # prefix, strips and join instead of one attention (after a q/k norm of its own)
-            per_layer += 2 if self.backend == "tc" else 3
-        if self.adapters is not None:  # shrink and expand beside each linear
-            per_layer += 2 * len(self.adapters.targets)
+        g = self.g
+        if self.prefix_len:  # instead of one attention, and after a q/k norm of its own
+            per_layer += K.shared_prefix_attention_launches(self.B, 1, g.num_attention_heads, g.num_key_value_heads,
+                                                            g.head_dim, self.prefix_len)
+            per_layer -= 1 if self.backend == "tc" else 0
+        if self.adapters is not None:
+            per_layer += sum(K.lora_delta_launches(self.B, 1, *self.adapters.shapes[t], self.adapters.rank)
+                             for t in self.adapters.targets)
         if self.rules is not None:  # rules and pick instead of the argmax (after an lm_head of its own), ids without -1
             head += 2 if self.backend == "tc" else 3
         if self.tp is not None:  # + all-reduce / residual-add kernels after each row-split linear, + keys-to-ids

@@ -634,6 +634,14 @@ def shared_prefix_attention_workspace_bytes(batch: int, q_len: int, num_heads: i
     return v.value
 
 
+def shared_prefix_attention_launches(batch: int, q_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                     prefix_len: int) -> int:
+    v = ctypes.c_int64(0)
+    nat.call("ls_shared_prefix_attention_launches", batch, q_len, num_heads, num_kv_heads, head_dim, prefix_len,
+             ctypes.byref(v))
+    return v.value
+
+
 def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
                             v_cache: torch.Tensor, batch: int, q_len: int, num_heads: int, num_kv_heads: int,
                             head_dim: int, prefix_len: int, max_seq: int, scale: float, *,
@@ -685,6 +693,12 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 def lora_delta_workspace_bytes(batch: int, q_len: int, k: int, n: int, rank: int) -> int:
     v = ctypes.c_int64(0)
     nat.call("ls_lora_delta_workspace_bytes", batch, q_len, k, n, rank, ctypes.byref(v))
+    return v.value
+
+
+def lora_delta_launches(batch: int, q_len: int, k: int, n: int, rank: int) -> int:
+    v = ctypes.c_int64(0)
+    nat.call("ls_lora_delta_launches", batch, q_len, k, n, rank, ctypes.byref(v))
     return v.value
 
 
