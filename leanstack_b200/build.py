@@ -8,14 +8,17 @@ the default build has none of them.  The library links
 the shared CUDA runtime (``libcudart.so.12``), so inside a PyTorch process it
 binds to the runtime PyTorch already loaded and sees the same current device
 and streams.  ``csrc/torch_front.cpp`` becomes ``_lib/_torch_front.so``, a Python
-module on the installed PyTorch's headers that calls the library.  No GPU is
-needed to build.
+module on the installed PyTorch's headers that calls the library; without PyTorch
+or Python's headers it is left out, with a note, and the library alone serves the
+C ABI.  No GPU is needed to build.
 """
 
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -31,6 +34,7 @@ LIB = OUT_DIR / "libleanb200.so"
 OBJ_DIR = PKG / "_build"
 FRONT_SRC = CSRC / "torch_front.cpp"
 FRONT = OUT_DIR / "_torch_front.so"
+FRONT_STAMP = OUT_DIR / "front_torch.txt"  # the PyTorch version that the front end was built for
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
@@ -73,14 +77,36 @@ def _compile(src: Path, verbose: bool, ptxas_verbose: bool, defines: list[str]) 
     return obj, res.stderr
 
 
+def torch_version() -> str | None:
+    """Version of the installed PyTorch, None without one (PyTorch is not imported)."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    return importlib.metadata.version("torch")
+
+
+def front_lacks() -> str | None:
+    """What the front end needs and this machine does not have, None if all is there."""
+    if torch_version() is None:
+        return "PyTorch"
+    if not (Path(importlib.util.find_spec("torch").origin).parent / "lib" / "libc10_cuda.so").exists():
+        return "PyTorch with CUDA"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "Python's headers"
+    return None
+
+
 def needs_front() -> bool:
-    if not FRONT.exists():
+    if not FRONT.exists() or not FRONT_STAMP.exists() or FRONT_STAMP.read_text().strip() != torch_version():
         return True
     return any(p.stat().st_mtime > FRONT.stat().st_mtime for p in [FRONT_SRC, *INCLUDE.glob("*.h"), Path(__file__)])
 
 
-def build_front(verbose: bool = False) -> Path:
+def build_front(verbose: bool = False) -> Path | None:
     """Compile the front end against the installed PyTorch and link it to libleanb200.so beside it."""
+    lacks = front_lacks()
+    if lacks:
+        print(f"{FRONT.name} is left out: no {lacks}; {LIB.name} serves the C ABI", file=sys.stderr)
+        return None
     import torch
 
     home = Path(torch.__file__).parent
@@ -97,6 +123,7 @@ def build_front(verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"the front end failed to build:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, FRONT)
+    FRONT_STAMP.write_text(torch_version() + "\n")
     return FRONT
 
 
