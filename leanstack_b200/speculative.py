@@ -96,6 +96,8 @@ class SpeculativeDecoder:
         if self.use_graph:
             key = self._graph_key(k)
             if key not in self.graphs:
+                for old in [o for o in self.graphs if o[1:] != key[1:]]:  # no prefix comes back: its steps are stale for good
+                    del self.graphs[old]
                 self._capture(k)
             self.graphs[key].replay()
         else:
