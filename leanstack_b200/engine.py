@@ -76,7 +76,8 @@ class DecodeEngine:
         if adapters is not None:
             if linear_backend == "cuda_core":
                 raise ValueError("adapters ride on the split partials of the tc linears")
-            if adapters.shapes["qkv"] != (runtime.config.hidden_size, runtime.config.qkv_dim) or \
+            own = AdapterBank.linear_shapes(runtime.config)
+            if any(adapters.shapes[t] != own[t] for t in adapters.targets) or \
                     len(adapters.layers) != len(runtime.layers):
                 raise ValueError("the adapter bank is of another geometry")
             linear_backend = "tc"

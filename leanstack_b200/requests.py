@@ -56,10 +56,7 @@ class AdapterBank:
         unknown = [t for t in targets if t not in self.TARGETS]
         if unknown:
             raise ValueError(f"unknown adapter targets {unknown}; choose from {self.TARGETS}")
-        g = geometry
-        self.shapes = {"qkv": (g.hidden_size, g.qkv_dim), "o": (g.q_dim, g.hidden_size),
-                       "gate_up": (g.hidden_size, 2 * g.intermediate_size),
-                       "down": (g.intermediate_size, g.hidden_size)}
+        self.shapes = self.linear_shapes(geometry)
         self.adapters, self.rank = adapters, rank
         self.targets = tuple(t for t in self.TARGETS if t in targets)
         self.scaling = torch.zeros(adapters, device=device, dtype=torch.float32)
@@ -68,7 +65,13 @@ class AdapterBank:
             return torch.zeros(shape, device=device, dtype=torch.bfloat16)
 
         self.layers = [{t: (z(adapters, rank, self.shapes[t][0]), z(adapters, self.shapes[t][1], rank))
-                        for t in self.targets} for _ in range(g.num_hidden_layers)]
+                        for t in self.targets} for _ in range(geometry.num_hidden_layers)]
+
+    @staticmethod
+    def linear_shapes(g: QwenGeometry) -> dict[str, tuple[int, int]]:
+        """(inputs, outputs) of each target's linear."""
+        return {"qkv": (g.hidden_size, g.qkv_dim), "o": (g.q_dim, g.hidden_size),
+                "gate_up": (g.hidden_size, 2 * g.intermediate_size), "down": (g.intermediate_size, g.hidden_size)}
 
     def load(self, index: int, weights: dict, scaling: float) -> None:
         """Put an adapter at ``index``: ``weights[(layer, target)] = (a [r, in], b [out, r])`` with r up to
