@@ -213,14 +213,16 @@ class DecodeEngine:
         adapter_ids = None
         if self.adapters is not None:
             adapter_ids = torch.full((1,), adapter, device=self.rt.device, dtype=torch.int32)
+        # No prefix from here until the new one is complete: captured steps hold the old length and workspace.
         self.prefix.length = 0
-        self._prompt_pass(ids, 1, P, [k[None] for k in self.prefix.key], [v[None] for v in self.prefix.value],
-                          self.prefix.capacity, None, adapter_ids)
-        self.prefix.length = P
-        # Captured steps hold the old length and workspace.
         self.graph = None
         self.verify_graphs.clear()
         self.prefix_epoch += 1
+        if self.rules is not None:
+            self.rules.set_prefix(ids[:0])
+        self._prompt_pass(ids, 1, P, [k[None] for k in self.prefix.key], [v[None] for v in self.prefix.value],
+                          self.prefix.capacity, None, adapter_ids)
+        self.prefix.length = P
         g = self.g
         need = max(K.shared_prefix_attention_workspace_bytes(self.B, q, g.num_attention_heads, g.num_key_value_heads,
                                                              g.head_dim, P) for q in range(1, self.T // self.B + 1))
