@@ -46,10 +46,11 @@
 //     mask, and writes the finished rows: no partials, no join.
 //
 // Measured with 32 / 8 heads, all kernels together: 32 sequences behind 8192 keys, 372
-// own ones each, 26.6 us (83 MB, 3.1 TB/s: from release to first tile 2.4 us, tiles 5.7,
-// epilogue 2, then the last strips and the join); 13 x 5 rows (16 / 8 heads) behind 5003
-// keys 23.4 us; 6 prompts of 384 behind 8192 keys 293 us (1088 TFLOP/s: scores of 64 keys
-// keep the tensor pipe waiting for shared memory); 2 sequences behind 300 keys 6.0 us.
+// own ones each, 27.9 us (83 MB, 3.0 TB/s; each kernel alone and cold: prefix 16.7, strips
+// 15.4 in two to three waves of single warps, join 6.3); 13 x 5 rows (16 / 8 heads) behind
+// 5003 keys 24.9 us; 6 prompts of 384 behind 8192 keys 351 us (909 TFLOP/s, 1360 with the
+// products of the low halves; 410 in runs long enough for the power cap); 2 sequences
+// behind 300 keys 6.6 us.  With P as one bf16 these were 26.7, 23.5, 293 and 6.1 us.
 #include <algorithm>
 #include <cmath>
 
@@ -742,13 +743,14 @@ static SpPlan sp_plan(int64_t batch, int64_t q_len, int64_t hq, int64_t hkv, int
   const int64_t rows = batch * q_len * g;
   // Few rows: each K/V tile serves 128 rows and what little is computed leaves room
   // for the strips on the same SM; many: 256 rows share a tile.  Measured at 32 / 8
-  // heads and 8192 shared keys, kKeys / kRows: 192 rows 34 / 37 us, 384 rows 53 / 56,
-  // 768 rows 52 / 49.
+  // heads and 8192 shared keys, kKeys / kRows, up to 20 own keys: 192 rows 21.8 / 25.2
+  // us, 384 rows 32.2 / 34.2, 768 rows 50.6 / 49.7; 40 to 700 own keys: 36.7 / 40.3,
+  // 58.8 / 64.3, 104.5 / 107.9.
   pl.mode = rows <= 512 ? kKeys : kRows;
   // One row tile and a short prefix: its keys go to the strips' kernel, a launch less.
-  // us without / with, and with the host's time, 1 - 4 sequences of 4 rows: 64 keys
-  // 7.2 / 6.7 and 9.4 / 7.5, 300 keys 7.9 / 7.2 and 9.4 / 7.5, 2000 keys 9.6 / 8.6 and
-  // 9.9 / 9.3, 8192 keys 14.6 / 21.4.  8 sequences (two row tiles): 300 keys 8.2 / 9.1.
+  // us without / with, and with the host's time, 4 sequences of 4 rows: 64 keys 7.4 / 6.5
+  // and 8.9 / 7.4, 300 keys 7.9 / 6.6 and 9.0 / 7.3, 2000 keys 8.6 / 8.7 and 9.4 / 9.4,
+  // 8192 keys 13.3 / 18.1; 1 sequence: 2000 keys 8.1 / 7.5, 8192 keys 12.7 / 17.0.
   const bool few = rows <= 16 && prefix_len <= kSpFewKeys;
   if (few) pl.mode = kFew;
   const int64_t per = pl.mode == kKeys ? kSpRows : 2 * kSpRows;
