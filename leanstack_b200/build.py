@@ -78,10 +78,15 @@ def _compile(src: Path, verbose: bool, ptxas_verbose: bool, defines: list[str]) 
 
 
 def torch_version() -> str | None:
-    """Version of the installed PyTorch, None without one (PyTorch is not imported)."""
+    """Version of the installed PyTorch, None without one (imported only if it has no package data)."""
     if importlib.util.find_spec("torch") is None:
         return None
-    return importlib.metadata.version("torch")
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a PyTorch that was not installed as a package
+        import torch
+
+        return torch.__version__
 
 
 def front_lacks() -> str | None:
